@@ -120,7 +120,18 @@ enum mh_kernel_kind {
     MH_GEOM_STRAIN = 81, /* stress displacement: strained positions and shifts                                 */
     MH_GEOM_DET = 82,    /* determinants of 3x3 matrices                                                       */
     MH_MLP_BWD_W = 83,   /* radial MLP backward, column slices: their sum walked back through the hidden layers */
-    MH_NUM_KINDS = 84
+    MH_MM_ROWS = 84,     /* matrix product with its epilogue: BM rows x BN columns a workgroup                 */
+    MH_MM_OUTER = 85,    /* weight gradient: sums of outer products over rows, BM x BN of one group's          */
+    MH_MM_SUM = 86,      /* the sum of a split sum's parts, rounded to the output's type                       */
+    MH_MM_SLOPE = 87,    /* g act'(a) and the sums of its columns                                              */
+    MH_EXPERT_HIST = 88, /* assignments per expert of each block                                               */
+    MH_EXPERT_PLACE = 89, /* their places in the order by expert                                               */
+    MH_DISPATCH = 90,    /* rows to their places                                                               */
+    MH_COMBINE = 91,     /* weighted sums of rows back                                                         */
+    MH_COMBINE_BWD = 92, /* gradients of the rows and the weights                                              */
+    MH_NORM_FWD = 93,    /* norms around a block: one row per wave or per workgroup                            */
+    MH_NORM_BWD = 94,    /* its gradients                                                                      */
+    MH_NUM_KINDS = 95
 };
 
 /* flags of mh_conv_bwd */
@@ -686,6 +697,68 @@ int mh_geom_fwd(mh_module* m, const float* pos, const int32_t* send, const int32
 int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* gvec, const float* glen,
                 const int32_t* rowptr_r, const int32_t* eids_r, const int32_t* rowptr_s, const int32_t* eids_s,
                 float* gpos, float* gshifts, int32_t N, void* stream);
+
+/* The trainable layers on node features (no reference counterparts: the reference has no layers with weight gradients).
+ * `type` of a module is the tensors': float32, bfloat16 or float16 (compiled in: matmul.source, experts.source,
+ * norms.source).  Rows of x, g and residuals lie `ld` elements apart (ld >= their length); everything else is contiguous.
+ * Workspaces are the caller's; nothing is kept between calls.  Sizes past 2^31 - 1 rows or columns are refused.
+ *
+ * Groups: offsets [E + 1] int32 on the device, group e = rows offsets[e] .. offsets[e + 1] - 1 (not decreasing, within
+ * [0, R]; other contents give wrong rows, never an access outside the tensors).  offsets NULL: one group of all rows, E = 1.
+ *
+ * mh_mm_rows: C[r] = act(A[r] B_e^T + bias_e) + res[r] for the R rows of A [R, K] and their group's weights B [E, N, K]
+ * (modules of matmul.source(.., 'fwd')) or [E, K, N] ('dx', where it is the input gradient A B_e); C [R, N]; bias [E, N],
+ * res [R, N] and slope may be NULL.  Rows of no group are zero.  act: 0 none, 1 relu, 2 silu, 3 gelu (erf).  slope [R, N]
+ * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types uint16 fixed point (steps of 2^-15
+ * from -0.5; 65535: NaN).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
+ *
+ * mh_mm_outer: C[e] [M, N] = sum over the group's rows of A[r, :]^T B[r, :] (A [R, M], B [R, N]; an empty group: zeros).
+ * L > 0: the groups' rows are cut into pieces of L, `slots` >= the number of pieces, whose float32 sums go to
+ * part [slots, M, N]; mh_mm_sum then adds them: out[e, i] = sum of part[s, i] over e's pieces in order, i < n.  With
+ * L = 0 part may be NULL.  Bind MH_MM_OUTER as MH_MM_ROWS, MH_MM_SUM with 256 threads.
+ *
+ * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1) for rows g [R, N], and the sums of p's columns before
+ * rounding over each piece of L rows, part [slots, N] (NULL: none).  Rows of no group are left alone.  Bind MH_MM_SLOPE
+ * with 256 threads.
+ *
+ * mh_expert_order: the A = T k assignments experts [T, k] (int32, or int64 where wide), values outside [0, E) dropped,
+ * stably sorted by expert: offsets [E + 1], rows [A] (flat assignment at each place; -1 from offsets[E] on), place [A]
+ * (place of each; -1: dropped).  hist: scratch of `blocks` (E + 1) int32, blocks >= 1 workgroups sharing the work (hist
+ * may be NULL for one); E <= 1024.  Bind MH_EXPERT_HIST and MH_EXPERT_PLACE with 1024 threads.
+ * mh_dispatch: y[place[t, j]] = x[t] (y [T k, C]; rows of no assignment zero).
+ * mh_combine: out[t] = res[t] + sum of w[t, j] y[place[t, j]] over the kept j (w [T, k] float32 or NULL: 1; res or NULL).
+ * mh_combine_bwd: dy[place[t, j]] = w[t, j] g[t] (rows of no assignment zero) and dw[t, j] = <g[t], y[place[t, j]]> (0 where
+ * dropped); dy or dw may be NULL, y only with dw.  lg: log2 of the lanes that share a row (0 .. 6).  Bind the three with
+ * 256 threads.
+ *
+ * mh_norm_fwd: u = norm(y), h = x + scale gate u wp, n = norm(h) wn per row of C; gate, scale, wp, wn NULL: 1 (gate's shape is
+ * compiled in); modules without a branch take y, h NULL.  stats [T, 4] float32 (NULL: none) for mh_norm_bwd, which gives dx,
+ * dy, dgate (each may be NULL) and part [groups, 3, C], the sums of the gradients of scale, wp and wn over the rows of each of
+ * `groups` row groups (NULL: none), from gh and gn (NULL: 0).  Bind MH_NORM_FWD and MH_NORM_BWD as
+ * norms.module does; groups = blocks times the rows that a workgroup takes at once. */
+int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
+               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, int32_t act,
+               void* stream);
+int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
+                const int32_t* offsets, int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,
+              void* stream);
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, const int32_t* offsets,
+                int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
+                    int32_t* offsets, int32_t* rows, int32_t* place, void* stream);
+int mh_dispatch(mh_module* m, const void* x, int64_t ldx, const int32_t* place, const int32_t* offsets, void* y, int32_t T,
+                int32_t k, int32_t C, int32_t E, int32_t lg, void* stream);
+int mh_combine(mh_module* m, const void* y, const float* w, const int32_t* place, const void* res, int64_t ldr, void* out,
+               int32_t T, int32_t k, int32_t C, int32_t lg, void* stream);
+int mh_combine_bwd(mh_module* m, const void* g, int64_t ldg, const void* y, const float* w, const int32_t* place,
+                   const int32_t* offsets, void* dy, float* dw, int32_t T, int32_t k, int32_t C, int32_t E, int32_t lg,
+                   void* stream);
+int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, const void* scale, const void* wp,
+                const void* wn, void* h, void* n, float* stats, int32_t T, int32_t C, float eps, void* stream);
+int mh_norm_bwd(mh_module* m, const void* gh, const void* gn, const void* x, const void* y, const void* gate,
+                const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy, void* dgate,
+                float* part, int32_t T, int32_t C, int32_t blocks, void* stream);
 
 #ifdef __cplusplus
 }

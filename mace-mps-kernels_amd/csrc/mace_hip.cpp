@@ -104,13 +104,14 @@ int launch(mh_module* m, int kind, int64_t rows, void** args, void* stream, cons
     return 0;
 }
 
-// Launch `kind` on an explicit 1-D grid of `blocks` workgroups (kernels that size their own grid).
-int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* stream, const char* what) {
+// Launch `kind` on an explicit grid of `blocks` x `grid_y` workgroups (kernels that size their own grid).
+int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* stream, const char* what,
+                  int64_t grid_y = 1) {
     if (!m) return fail(-1, std::string(what) + ": null module");
     const Kernel& k = m->k[kind];
     if (!k.fn) return fail(-1, std::string(what) + ": kernel slot not bound in this module");
-    if (blocks <= 0) return 0;
-    if (blocks > 0x7fffffffLL) return fail(-1, std::string(what) + ": launch too large");
+    if (blocks <= 0 || grid_y <= 0) return 0;
+    if (blocks > 0x7fffffffLL || grid_y > 65535) return fail(-1, std::string(what) + ": launch too large");
     int dev = -1;
     MH_HIP(hipGetDevice(&dev));
     if (dev != m->device) {
@@ -118,8 +119,8 @@ int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* str
         os << what << ": module was loaded on device " << m->device << " but device " << dev << " is current";
         return fail(-1, os.str());
     }
-    hipError_t e = hipModuleLaunchKernel(k.fn, static_cast<unsigned>(blocks), 1, 1, static_cast<unsigned>(k.block), 1,
-                                         1, 0, static_cast<hipStream_t>(stream), args, nullptr);
+    hipError_t e = hipModuleLaunchKernel(k.fn, static_cast<unsigned>(blocks), static_cast<unsigned>(grid_y), 1,
+                                         static_cast<unsigned>(k.block), 1, 1, 0, static_cast<hipStream_t>(stream), args, nullptr);
     if (e != hipSuccess) return hip_fail(e, what);
     {
         std::lock_guard<std::mutex> lock(g_log_mu);
@@ -147,7 +148,7 @@ extern "C" {
 
 const char* mh_last_error(void) { return g_err.c_str(); }
 
-int mh_version(void) { return 48; }
+int mh_version(void) { return 49; }
 
 int mh_launch_log(int enable) {
     std::lock_guard<std::mutex> lock(g_log_mu);
@@ -1203,6 +1204,144 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
         return fail(-1, "mh_geom_bwd: NULL operand");
     void* args[] = {&vec, &len, &gvec, &glen, &rowptr_r, &eids_r, &rowptr_s, &eids_s, &gpos, &gshifts, &N};
     return launch(m, MH_GEOM_BWD, N, args, stream, "mh_geom_bwd");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------- trainable node layers
+namespace {
+
+// Pieces of at most L rows that R rows in E groups can make, with the rows of no group counted as one group more.
+int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
+    return (R + L - 1) / L + (offsets ? E + 1 : 0);
+}
+
+}  // namespace
+
+extern "C" {
+
+int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
+               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, int32_t act,
+               void* stream) {
+    if (R < 0 || N < 0 || K < 0 || E < 1 || (E > 1 && !offsets)) return fail(-1, "mh_mm_rows: bad sizes");
+    if (act < 0 || act > 3) return fail(-1, "mh_mm_rows: unknown activation");
+    if (R == 0 || N == 0) return 0;
+    if (!C || (K > 0 && (!A || !B))) return fail(-1, "mh_mm_rows: NULL operand");
+    if (lda < K || (res && ldr < N)) return fail(-1, "mh_mm_rows: rows overlap (ld below the row's length)");
+    if (!m || !m->k[MH_MM_ROWS].fn) return fail(-1, "mh_mm_rows: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_MM_ROWS];
+    if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_mm_rows: too many rows");
+    const int64_t tiles = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldr, &R, &N, &K, &E, &act};
+    return launch_blocks(m, MH_MM_ROWS, tiles, args, stream, "mh_mm_rows");
+}
+
+int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
+                const int32_t* offsets, int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
+    if (R < 0 || M < 0 || N < 0 || E < 1 || (E > 1 && !offsets) || L < 0) return fail(-1, "mh_mm_outer: bad sizes");
+    if (M == 0 || N == 0) return 0;
+    if ((R > 0 && (!A || !B)) || (L ? !part : !C)) return fail(-1, "mh_mm_outer: NULL operand");
+    if (lda < M || ldb < N) return fail(-1, "mh_mm_outer: rows overlap (ld below the row's length)");
+    if (L && (slots < 1 || R > 0x7fffffff - L)) return fail(-1, "mh_mm_outer: bad pieces");
+    if (!m || !m->k[MH_MM_OUTER].fn) return fail(-1, "mh_mm_outer: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_MM_OUTER];
+    const int64_t tiles = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
+                          ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    void* args[] = {&A, &B, &C, &part, &offsets, &lda, &ldb, &R, &M, &N, &E, &L};
+    return launch_blocks(m, MH_MM_OUTER, tiles, args, stream, "mh_mm_outer", L ? slots : E);
+}
+
+int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,
+              void* stream) {
+    if (R < 0 || E < 1 || (E > 1 && !offsets) || L < 1 || n < 0 || R > 0x7fffffff - L)
+        return fail(-1, "mh_mm_sum: bad sizes");
+    if (n == 0) return 0;
+    if (!out || (R > 0 && !part)) return fail(-1, "mh_mm_sum: NULL operand");
+    void* args[] = {&part, &out, &offsets, &R, &E, &L, &n};
+    return launch_blocks(m, MH_MM_SUM, (n + 1023) / 1024, args, stream, "mh_mm_sum", E);
+}
+
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, const int32_t* offsets,
+                int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
+    if (R < 0 || N < 0 || E < 1 || (E > 1 && !offsets) || L < 1 || slots < 0 || R > 0x7fffffff - L)
+        return fail(-1, "mh_mm_slope: bad sizes");
+    if (R == 0 || N == 0) return 0;
+    if (!g || (!p && !part)) return fail(-1, "mh_mm_slope: NULL operand");
+    if (ldg < N) return fail(-1, "mh_mm_slope: rows overlap (ld below the row's length)");
+    void* args[] = {&g, &slope, &p, &part, &offsets, &ldg, &R, &N, &E, &L};
+    return launch_blocks(m, MH_MM_SLOPE, slots, args, stream, "mh_mm_slope", (static_cast<int64_t>(N) + 255) / 256);
+}
+
+int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
+                    int32_t* offsets, int32_t* rows, int32_t* place, void* stream) {
+    if (A < 0 || E < 1 || E > 1024 || blocks < 1 || A > 0x7fffffff - 1024) return fail(-1, "mh_expert_order: bad sizes");
+    if (!offsets || (A > 0 && (!experts || !rows || !place)) || (blocks > 1 && !hist))
+        return fail(-1, "mh_expert_order: NULL operand");
+    // a block's share, whole chunks of 1024
+    const int64_t share = ((static_cast<int64_t>(A) + blocks - 1) / blocks + 1023) / 1024 * 1024;
+    if (share * blocks > 0x7fffffff) return fail(-1, "mh_expert_order: too many assignments");
+    int32_t per = static_cast<int32_t>(share);
+    if (blocks > 1) {
+        void* args[] = {&experts, &wide, &A, &E, &per, &hist};
+        if (int rc = launch_blocks(m, MH_EXPERT_HIST, blocks, args, stream, "mh_expert_order")) return rc;
+    }
+    void* args[] = {&experts, &wide, &A, &E, &per, &hist, &offsets, &rows, &place};
+    return launch_blocks(m, MH_EXPERT_PLACE, blocks, args, stream, "mh_expert_order");
+}
+
+int mh_dispatch(mh_module* m, const void* x, int64_t ldx, const int32_t* place, const int32_t* offsets, void* y, int32_t T,
+                int32_t k, int32_t C, int32_t E, int32_t lg, void* stream) {
+    if (T < 0 || k < 1 || C < 0 || E < 1 || lg < 0 || lg > 6 || static_cast<int64_t>(T) * k > 0x7fffffff)
+        return fail(-1, "mh_dispatch: bad sizes");
+    if (T == 0 || C == 0) return 0;
+    if (!x || !place || !offsets || !y) return fail(-1, "mh_dispatch: NULL operand");
+    if (ldx < C) return fail(-1, "mh_dispatch: rows overlap (ld below the row's length)");
+    void* args[] = {&x, &place, &offsets, &y, &ldx, &T, &k, &C, &E, &lg};
+    return launch_blocks(m, MH_DISPATCH, (T + (256LL >> lg) - 1) / (256 >> lg), args, stream, "mh_dispatch");
+}
+
+int mh_combine(mh_module* m, const void* y, const float* w, const int32_t* place, const void* res, int64_t ldr, void* out,
+               int32_t T, int32_t k, int32_t C, int32_t lg, void* stream) {
+    if (T < 0 || k < 1 || C < 0 || lg < 0 || lg > 6 || static_cast<int64_t>(T) * k > 0x7fffffff)
+        return fail(-1, "mh_combine: bad sizes");
+    if (T == 0 || C == 0) return 0;
+    if (!y || !place || !out) return fail(-1, "mh_combine: NULL operand");
+    if (res && ldr < C) return fail(-1, "mh_combine: rows overlap (ld below the row's length)");
+    void* args[] = {&y, &w, &place, &res, &out, &ldr, &T, &k, &C, &lg};
+    return launch_blocks(m, MH_COMBINE, (T + (256LL >> lg) - 1) / (256 >> lg), args, stream, "mh_combine");
+}
+
+int mh_combine_bwd(mh_module* m, const void* g, int64_t ldg, const void* y, const float* w, const int32_t* place,
+                   const int32_t* offsets, void* dy, float* dw, int32_t T, int32_t k, int32_t C, int32_t E, int32_t lg,
+                   void* stream) {
+    if (T < 0 || k < 1 || C < 0 || E < 1 || lg < 0 || lg > 6 || static_cast<int64_t>(T) * k > 0x7fffffff)
+        return fail(-1, "mh_combine_bwd: bad sizes");
+    if (T == 0) return 0;
+    if (!place || !offsets || (C > 0 && (!g || (dw && !y)))) return fail(-1, "mh_combine_bwd: NULL operand");
+    if (ldg < C) return fail(-1, "mh_combine_bwd: rows overlap (ld below the row's length)");
+    void* args[] = {&g, &y, &w, &place, &offsets, &dy, &dw, &ldg, &T, &k, &C, &E, &lg};
+    return launch_blocks(m, MH_COMBINE_BWD, (T + (256LL >> lg) - 1) / (256 >> lg), args, stream, "mh_combine_bwd");
+}
+
+int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, const void* scale, const void* wp,
+                const void* wn, void* h, void* n, float* stats, int32_t T, int32_t C, float eps, void* stream) {
+    if (T < 0 || C < 0) return fail(-1, "mh_norm_fwd: bad sizes");
+    if (T == 0 || C == 0) return 0;
+    if (!x || !n || (y == nullptr) != (h == nullptr)) return fail(-1, "mh_norm_fwd: NULL operand");
+    if (!m) return fail(-1, "mh_norm_fwd: null module");
+    const int per = m->k[MH_NORM_FWD].rows_per_block;
+    void* args[] = {&x, &y, &gate, &scale, &wp, &wn, &h, &n, &stats, &T, &C, &eps};
+    return launch_blocks(m, MH_NORM_FWD, (static_cast<int64_t>(T) + per - 1) / per, args, stream, "mh_norm_fwd");
+}
+
+int mh_norm_bwd(mh_module* m, const void* gh, const void* gn, const void* x, const void* y, const void* gate,
+                const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy, void* dgate,
+                float* part, int32_t T, int32_t C, int32_t blocks, void* stream) {
+    if (T < 0 || C < 0 || blocks < 0) return fail(-1, "mh_norm_bwd: bad sizes");
+    if (T == 0 || C == 0) return 0;
+    if (!x || !stats) return fail(-1, "mh_norm_bwd: NULL operand");
+    void* args[] = {&gh, &gn, &x, &y, &gate, &scale, &wp, &wn, &stats, &dx, &dy, &dgate, &part, &T, &C};
+    return launch_blocks(m, MH_NORM_BWD, blocks, args, stream, "mh_norm_bwd");
 }
 
 }  // extern "C"

@@ -1,0 +1,252 @@
+// mh_norms.h — norms before and after a block, fused with its gate and residual scale; prepended with mh_device.h and
+// mh_matmul.h.
+//
+// With N(v) = (v - mean v) / sqrt(var v + eps) (LAYER) or v / sqrt(mean v^2 + eps), per row of C values:
+//   u = N(y),  h = x + s gate u wp,  v = N(h),  n = v wn                       (s, gate, wp, wn: 1 where absent)
+// and backward, with q = gn wn and M the mean over the row:
+//   dh = gh + r_h (q - v M(q v) [- M(q)]),  dx = dh,  dwn = sum_t gn v
+//   e = dh s gate wp,  dy = r_y (e - u M(e u) [- M(e)]),  ds = sum dh gate u wp,  dwp = sum dh s gate u,
+//   dgate = dh s u wp (summed over the row for a gate of one value per row).
+// A row's values stay in registers between the sums that they need (one read of each input), all sums are float32.
+#pragma once
+
+// A row of up to TPR NV V values, thread l holding vectors l, l + TPR, ...; TPR 64: a wave (four rows a workgroup), more: the
+// workgroup.
+template <int TY, int TPR, int NV>
+struct nm_row {
+    typedef typename mm_type<TY>::t T;
+    static constexpr int V = mm_vec<TY>::V;
+    mm_vec<TY> r[NV];
+    __device__ __forceinline__ void get(const T* p, int C, int l) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (l + i * TPR) * V;
+            if (c < C) r[i].get(p + c, C - c);
+            else r[i].zero();
+        }
+    }
+    __device__ __forceinline__ void put(T* p, int C, int l) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (l + i * TPR) * V;
+            if (c < C) r[i].put(p + c, C - c);
+        }
+    }
+    __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j) r[i].v[j] = x;
+    }
+    // f(vector, element) for every value of the row that this thread holds (values past C are left out)
+    template <typename F>
+    __device__ __forceinline__ static void each(int C, int l, F f) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if ((l + i * TPR) * V + j < C) f(i, j);
+    }
+};
+
+// The row's sums of a and b, to every thread of it.  `slot` alternates between two LDS places from call to call, so one
+// barrier per call is enough.
+template <int TPR>
+__device__ __forceinline__ void nm_sum2(float& a, float& b, float (*ws)[2][TPR / MH_WAVE], int slot) {
+#pragma unroll
+    for (int d = 1; d < MH_WAVE; d <<= 1) {
+        a += __shfl_xor(a, d, MH_WAVE);
+        b += __shfl_xor(b, d, MH_WAVE);
+    }
+    if constexpr (TPR > MH_WAVE) {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            ws[slot][0][w] = a;
+            ws[slot][1][w] = b;
+        }
+        __syncthreads();
+        a = b = 0.f;
+#pragma unroll
+        for (int k = 0; k < TPR / MH_WAVE; ++k) {
+            a += ws[slot][0][k];
+            b += ws[slot][1][k];
+        }
+    }
+}
+
+// mean and 1 / sqrt(var + eps) of a row held in registers; the variance from the differences to the mean
+template <int TY, int TPR, int NV, bool LAYER>
+__device__ __forceinline__ void nm_stats(const nm_row<TY, TPR, NV>& y, int C, int l, float eps, float (*ws)[2][TPR / MH_WAVE], int& slot,
+                                         float& mean, float& rstd) {
+    typedef nm_row<TY, TPR, NV> row;
+    float s = 0.f, z = 0.f;
+    mean = 0.f;
+    if (LAYER) {
+        row::each(C, l, [&](int i, int j) { s += y.r[i].v[j]; });
+        nm_sum2<TPR>(s, z, ws, slot);
+        slot ^= 1;
+        mean = s / C;
+        s = 0.f;
+    }
+    row::each(C, l, [&](int i, int j) {
+        const float d = y.r[i].v[j] - mean;
+        s += d * d;
+    });
+    nm_sum2<TPR>(s, z, ws, slot);
+    slot ^= 1;
+    rstd = 1.f / sqrtf(s / C + eps);
+}
+
+// GATE 0: none, 1: one value a row, 2: one a channel; Y: a branch y to add.  stats [T, 4]: mean and 1 / std of y and of h.
+template <int TY, int TPR, int NV, bool LAYER, bool Y, int GATE>
+__device__ __forceinline__ void nm_fwd_body(const void* x_, const void* y_, const void* gate_, const void* scale_,
+                                            const void* wp_, const void* wn_, void* h_, void* n_, float* stats, int T, int C,
+                                            float eps) {
+    typedef nm_row<TY, TPR, NV> row;
+    typedef typename mm_type<TY>::t S;
+    __shared__ float ws[2][2][TPR / MH_WAVE];
+    constexpr int PER = TPR > MH_WAVE ? 1 : 4;           // rows of a workgroup
+    const int l = threadIdx.x % TPR;
+    const long long t = (long long)blockIdx.x * PER + threadIdx.x / TPR;
+    if (t >= T) return;                                  // a whole wave or a whole workgroup
+    int slot = 0;
+    row h, w;
+    float my = 0.f, ry = 0.f, mh, rh;
+    h.get(static_cast<const S*>(x_) + t * C, C, l);
+    if (Y) {
+        row y, k;
+        y.get(static_cast<const S*>(y_) + t * C, C, l);
+        if (GATE == 2) k.get(static_cast<const S*>(gate_) + t * C, C, l);
+        nm_stats<TY, TPR, NV, LAYER>(y, C, l, eps, ws, slot, my, ry);
+        const float gr = GATE == 1 ? mm_get<TY>(static_cast<const S*>(gate_) + t) : 1.f;
+        row::each(C, l, [&](int i, int j) { y.r[i].v[j] = (y.r[i].v[j] - my) * ry; });
+        if (wp_) {
+            w.get(static_cast<const S*>(wp_), C, l);
+            row::each(C, l, [&](int i, int j) { y.r[i].v[j] *= w.r[i].v[j]; });
+        }
+        if (scale_) {
+            w.get(static_cast<const S*>(scale_), C, l);
+            row::each(C, l, [&](int i, int j) { y.r[i].v[j] *= w.r[i].v[j]; });
+        }
+        row::each(C, l, [&](int i, int j) {
+            h.r[i].v[j] += (GATE == 2 ? k.r[i].v[j] : GATE == 1 ? gr : 1.f) * y.r[i].v[j];
+        });
+        h.put(static_cast<S*>(h_) + t * C, C, l);
+    }
+    nm_stats<TY, TPR, NV, LAYER>(h, C, l, eps, ws, slot, mh, rh);
+    if (wn_) w.get(static_cast<const S*>(wn_), C, l);
+    else w.fill(1.f);
+    row::each(C, l, [&](int i, int j) { h.r[i].v[j] = (h.r[i].v[j] - mh) * rh * w.r[i].v[j]; });
+    h.put(static_cast<S*>(n_) + t * C, C, l);
+    if (stats && l == 0) *reinterpret_cast<mh_f4*>(stats + 4 * t) = mh_f4{my, ry, mh, rh};
+}
+
+// Rows walked by a fixed number of row groups (a wave or a workgroup each); the sums over rows of the three weights'
+// gradients stay in registers and go to part[row group][3][C] (scale, wp, wn) at the end, added by mm_sum in order.
+template <int TY, int TPR, int NV, bool LAYER, bool Y, int GATE>
+__device__ __forceinline__ void nm_bwd_body(const void* gh_, const void* gn_, const void* x_, const void* y_, const void* gate_,
+                                            const void* scale_, const void* wp_, const void* wn_, const float* stats, void* dx_,
+                                            void* dy_, void* dgate_, float* part, int T, int C) {
+    typedef nm_row<TY, TPR, NV> row;
+    typedef typename mm_type<TY>::t S;
+    __shared__ float ws[2][2][TPR / MH_WAVE];
+    constexpr int PER = TPR > MH_WAVE ? 1 : 4;           // rows of a workgroup
+    const int l = threadIdx.x % TPR, groups = gridDim.x * PER;
+    const int me = blockIdx.x * PER + threadIdx.x / TPR;
+    int slot = 0;
+    row as, ap, an;
+    as.fill(0.f);
+    ap.fill(0.f);
+    an.fill(0.f);
+    for (long long t = me; t < T; t += groups) {
+        const mh_f4 st = *reinterpret_cast<const mh_f4*>(stats + 4 * t);
+        row u, v, d, q, w;
+        v.get(static_cast<const S*>(x_) + t * C, C, l);
+        if (gn_) q.get(static_cast<const S*>(gn_) + t * C, C, l);
+        else q.fill(0.f);
+        const float gr = Y && GATE == 1 ? mm_get<TY>(static_cast<const S*>(gate_) + t) : 1.f;
+        row k;
+        if (Y) {
+            u.get(static_cast<const S*>(y_) + t * C, C, l);
+            if (GATE == 2) k.get(static_cast<const S*>(gate_) + t * C, C, l);
+            row::each(C, l, [&](int i, int j) { u.r[i].v[j] = (u.r[i].v[j] - st[0]) * st[1]; });
+            // d: s gate wp
+            d.fill(1.f);
+            if (scale_) d.get(static_cast<const S*>(scale_), C, l);
+            if (wp_) {
+                w.get(static_cast<const S*>(wp_), C, l);
+                row::each(C, l, [&](int i, int j) { d.r[i].v[j] *= w.r[i].v[j]; });
+            }
+            row::each(C, l, [&](int i, int j) {
+                v.r[i].v[j] += (GATE == 2 ? k.r[i].v[j] : gr) * d.r[i].v[j] * u.r[i].v[j];
+            });
+        }
+        row::each(C, l, [&](int i, int j) { v.r[i].v[j] = (v.r[i].v[j] - st[2]) * st[3]; });
+        row::each(C, l, [&](int i, int j) { an.r[i].v[j] += q.r[i].v[j] * v.r[i].v[j]; });
+        if (wn_) {
+            w.get(static_cast<const S*>(wn_), C, l);
+            row::each(C, l, [&](int i, int j) { q.r[i].v[j] *= w.r[i].v[j]; });
+        }
+        float sv = 0.f, s1 = 0.f;
+        row::each(C, l, [&](int i, int j) {
+            sv += q.r[i].v[j] * v.r[i].v[j];
+            if (LAYER) s1 += q.r[i].v[j];
+        });
+        nm_sum2<TPR>(sv, s1, ws, slot);
+        slot ^= 1;
+        sv /= C;
+        s1 /= C;
+        if (gh_) w.get(static_cast<const S*>(gh_) + t * C, C, l);
+        else w.fill(0.f);
+        row::each(C, l, [&](int i, int j) {              // w: dh
+            w.r[i].v[j] += st[3] * (q.r[i].v[j] - v.r[i].v[j] * sv - s1);
+        });
+        if (dx_) w.put(static_cast<S*>(dx_) + t * C, C, l);
+        if (Y) {
+            // the weights of u in h, one by one, for their gradients
+            row sc, wp;
+            sc.fill(1.f);
+            wp.fill(1.f);
+            if (scale_) sc.get(static_cast<const S*>(scale_), C, l);
+            if (wp_) wp.get(static_cast<const S*>(wp_), C, l);
+            float se = 0.f, s0 = 0.f, sg = 0.f, z = 0.f;
+            row::each(C, l, [&](int i, int j) {
+                const float dh = w.r[i].v[j], g = GATE == 2 ? k.r[i].v[j] : gr, uu = u.r[i].v[j];
+                as.r[i].v[j] += dh * g * uu * wp.r[i].v[j];
+                ap.r[i].v[j] += dh * g * uu * sc.r[i].v[j];
+                const float dg = dh * uu * d.r[i].v[j];
+                if (GATE == 1) sg += dg;
+                if (GATE == 2) q.r[i].v[j] = dg;
+                const float e = dh * g * d.r[i].v[j];
+                w.r[i].v[j] = e;
+                se += e * uu;
+                if (LAYER) s0 += e;
+            });
+            nm_sum2<TPR>(se, s0, ws, slot);
+            slot ^= 1;
+            se /= C;
+            s0 /= C;
+            row::each(C, l, [&](int i, int j) { w.r[i].v[j] = st[1] * (w.r[i].v[j] - u.r[i].v[j] * se - s0); });
+            if (dy_) w.put(static_cast<S*>(dy_) + t * C, C, l);
+            if (GATE == 2 && dgate_) q.put(static_cast<S*>(dgate_) + t * C, C, l);
+            if (GATE == 1 && dgate_) {
+                nm_sum2<TPR>(sg, z, ws, slot);
+                slot ^= 1;
+                if (l == 0) {
+                    if constexpr (TY == MM_F32) static_cast<float*>(dgate_)[t] = sg;
+                    else static_cast<unsigned short*>(dgate_)[t] = mm_round<TY>(sg);
+                }
+            }
+        }
+    }
+    if (!part) return;
+    float* p = part + (long long)me * 3 * C;
+    row::each(C, l, [&](int i, int j) {
+        const int c = (l + i * TPR) * row::V + j;
+        if (Y) {
+            p[c] = as.r[i].v[j];
+            p[C + c] = ap.r[i].v[j];
+        }
+        p[2 * C + c] = an.r[i].v[j];
+    });
+}

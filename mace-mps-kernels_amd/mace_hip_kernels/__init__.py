@@ -40,13 +40,17 @@ from . import _native
 from . import conv as _conv
 from . import geometry as _geometry
 from .conv import check_graphs
+from .matmul import dense, expert_dense
+from .experts import ExpertOrder, combine, dispatch, expert_order
 from .neighbours import NeighbourList, neighbour_list, update_batch
+from .norms import block_norm
 
 __version__ = '0.1.0'
 __all__ = ['patch_model', 'unpatch_model', 'HipConvTP', 'HipSymmetricContraction', 'HipSphericalHarmonics',
            'HipNodeLinear', 'HipRadialMLP', 'HipRadialEmbedding', 'conv_supported', 'sc_supported', 'sh_supported', 'lin_supported',
            'mlp_supported', 'emb_supported', 'HipReshapeIrreps', 'reshape_supported', 'HipReadout',
-           'readout_supported', 'neighbour_list', 'update_batch', 'NeighbourList', 'check_graphs']
+           'readout_supported', 'neighbour_list', 'update_batch', 'NeighbourList', 'check_graphs', 'dense', 'expert_dense',
+           'ExpertOrder', 'expert_order', 'dispatch', 'combine', 'block_norm']
 
 _LINEAR_CLASSES = ('Linear', 'FullyConnectedTensorProduct')
 

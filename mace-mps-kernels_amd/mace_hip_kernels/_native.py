@@ -28,9 +28,10 @@ MH_CONV_FWD, MH_CONV_BWD, MH_CONV_BWD_WY, MH_SC_FWD, MH_SC_BWD, MH_CONV_BWD_R, M
     MH_NL_FILL, MH_SPECIES_ORDER, MH_MLP_JVP, MH_MLP_BWD2, MH_GEOM_SEGSUM, MH_NL_BASES, MH_EDGE_COUNT, \
     MH_EDGE_PLACE, MH_GEOM_SEGSUM1, MH_EDGE_PAIR, MH_CONV_FWD_CR, MH_MLP_H3, MH_MLP_OUT, MH_EDGE_FWD, \
     MH_EDGE_BWD, MH_MLP_BWD_P, MH_LIN_BWD_SUM, MH_MLP_H3T, MH_CONV_BWD_T, \
-    MH_GEOM_STRAIN, MH_GEOM_DET, MH_MLP_BWD_W = range(84)
+    MH_GEOM_STRAIN, MH_GEOM_DET, MH_MLP_BWD_W, MH_MM_ROWS, MH_MM_OUTER, MH_MM_SUM, MH_MM_SLOPE, MH_EXPERT_HIST, \
+    MH_EXPERT_PLACE, MH_DISPATCH, MH_COMBINE, MH_COMBINE_BWD, MH_NORM_FWD, MH_NORM_BWD = range(95)
 MH_WANT_GX, MH_WANT_GWY, MH_CUT_MASKED, MH_CUT_NOZERO = 1, 2, 4, 8
-ABI_VERSION = 48
+ABI_VERSION = 49
 
 # hipcc/hipRTC options for every generated layer: gfx950 code, -O3, and packed-FP32 instructions disabled.
 ARCH = os.environ.get('MACE_HIP_ARCH', 'gfx950')
@@ -42,6 +43,7 @@ _code_cache = {}
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int32
+_L = ctypes.c_int64
 _SIGS = {
     'mh_last_error': (ctypes.c_char_p, []),
     'mh_version': (ctypes.c_int, []),
@@ -130,6 +132,16 @@ _SIGS = {
     'mh_neighbour_list_work_size': (ctypes.c_size_t, [_I, _I, ctypes.c_int64]),
     'mh_neighbour_list': (ctypes.c_int, [_P] * 5 + [_I, _I, ctypes.c_double, ctypes.c_int64, ctypes.c_int64]
                           + [_P] * 3 + [_I] + [_P] * 3),
+    'mh_mm_rows': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_L, _P, _P] + [_I] * 5 + [_P]),
+    'mh_mm_outer': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 3 + [_I] * 6 + [_P]),
+    'mh_mm_sum': (ctypes.c_int, [_P] * 4 + [_I] * 3 + [_L, _P]),
+    'mh_mm_slope': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_I] * 5 + [_P]),
+    'mh_expert_order': (ctypes.c_int, [_P, _P] + [_I] * 3 + [_P, _I] + [_P] * 4),
+    'mh_dispatch': (ctypes.c_int, [_P, _P, _L] + [_P] * 3 + [_I] * 5 + [_P]),
+    'mh_combine': (ctypes.c_int, [_P] * 5 + [_L, _P] + [_I] * 4 + [_P]),
+    'mh_combine_bwd': (ctypes.c_int, [_P, _P, _L] + [_P] * 6 + [_I] * 5 + [_P]),
+    'mh_norm_fwd': (ctypes.c_int, [_P] * 10 + [_I, _I, ctypes.c_float, _P]),
+    'mh_norm_bwd': (ctypes.c_int, [_P] * 14 + [_I] * 3 + [_P]),
 }
 EXPORTS = tuple(_SIGS)
 
@@ -169,6 +181,15 @@ def check(rc, what=''):
 def device_header():
     with open(DEVICE_HEADER) as f:
         return f.read()
+
+
+def layer_header(*names):
+    """The device header and the named ones of the trainable node layers (``csrc/mh_<name>.h``) behind it."""
+    text = device_header()
+    for name in names:
+        with open(os.path.join(os.path.dirname(DEVICE_HEADER), f'mh_{name}.h')) as f:
+            text += f.read()
+    return text
 
 
 def dual_header():
