@@ -708,18 +708,25 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  *
  * mh_mm_rows: C[r] = act(A[r] B_e^T + bias_e) + res[r] for the R rows of A [R, K] and their group's weights B [E, N, K]
  * (modules of matmul.source(.., 'fwd')) or [E, K, N] ('dx', where it is the input gradient A B_e); C [R, N]; bias [E, N],
- * res [R, N] and slope may be NULL.  Rows of no group are zero.  act: 0 none, 1 relu, 2 silu, 3 gelu (erf).  slope [R, N]
+ * res [R, N] and slope may be NULL.  Rows of no group are zero.  act (none, relu, silu, gelu by erf) is compiled in.  slope [R, N]
  * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types uint16 fixed point (steps of 2^-15
  * from -0.5; 65535: NaN).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
+ * Modules of a tile in matmul.FAST need every row distance, contiguous length and address to be multiples of 16 bytes.
  *
  * mh_mm_outer: C[e] [M, N] = sum over the group's rows of A[r, :]^T B[r, :] (A [R, M], B [R, N]; an empty group: zeros).
  * L > 0: the groups' rows are cut into pieces of L, `slots` >= the number of pieces, whose float32 sums go to
  * part [slots, M, N]; mh_mm_sum then adds them: out[e, i] = sum of part[s, i] over e's pieces in order, i < n.  With
- * L = 0 part may be NULL.  Bind MH_MM_OUTER as MH_MM_ROWS, MH_MM_SUM with 256 threads.
+ * L = 0 part may be NULL.  Bind MH_MM_OUTER as MH_MM_ROWS, MH_MM_SUM with 1024 threads.
  *
  * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1) for rows g [R, N], and the sums of p's columns before
- * rounding over each piece of L rows, part [slots, N] (NULL: none).  Rows of no group are left alone.  Bind MH_MM_SLOPE
- * with 256 threads.
+ * rounding: over each piece of L rows into part [slots, N], or with one slot of all rows into db [N] (both NULL: none).
+ * Rows of no group are left alone.  Bind MH_MM_SLOPE with 256 threads.
+ *
+ * mh_mm_bwd: the backward of mh_mm_rows 'fwd' in one call, from g [R, N]: p = g act' (scratch [R, N]; NULL with slope NULL),
+ * db, dx = p W_e and dW = p^T x per group, each left out where its pointer is NULL.  sums, rows, outer: modules of
+ * matmul.source 'sum', 'dx' and 'dw'.  Ls / slots_s and Lo / slots_o are the pieces of db's and dW's sums over rows, part
+ * scratch for the larger of [slots_s, N] and [slots_o, N, K] (the first not needed for one slot without offsets, the
+ * second not for Lo = 0).
  *
  * mh_expert_order: the A = T k assignments experts [T, k] (int32, or int64 where wide), values outside [0, E) dropped,
  * stably sorted by expert: offsets [E + 1], rows [A] (flat assignment at each place; -1 from offsets[E] on), place [A]
@@ -733,18 +740,21 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  *
  * mh_norm_fwd: u = norm(y), h = x + scale gate u wp, n = norm(h) wn per row of C; gate, scale, wp, wn NULL: 1 (gate's shape is
  * compiled in); modules without a branch take y, h NULL.  stats [T, 4] float32 (NULL: none) for mh_norm_bwd, which gives dx,
- * dy, dgate (each may be NULL) and part [groups, 3, C], the sums of the gradients of scale, wp and wn over the rows of each of
- * `groups` row groups (NULL: none), from gh and gn (NULL: 0).  Bind MH_NORM_FWD and MH_NORM_BWD as
- * norms.module does; groups = blocks times the rows that a workgroup takes at once. */
+ * dy, dgate and dw [3, C] = the gradients of scale, wp and wn (each may be NULL) from gh and gn (NULL: 0); part [groups, 3, C]
+ * is scratch for the sums of the `groups` row groups (blocks times the rows that a workgroup takes at once) and sums a
+ * module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD as norms.module does. */
 int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
-               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, int32_t act,
-               void* stream);
+               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream);
 int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
                 const int32_t* offsets, int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
 int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,
               void* stream);
-int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, const int32_t* offsets,
-                int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, void* db,
+                const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g, int64_t ldg, const void* slope,
+              const void* W, const void* x, int64_t ldx, const int32_t* offsets, void* p, void* dx, void* dW, void* db,
+              float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
+              int32_t slots_o, void* stream);
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
                     int32_t* offsets, int32_t* rows, int32_t* place, void* stream);
 int mh_dispatch(mh_module* m, const void* x, int64_t ldx, const int32_t* place, const int32_t* offsets, void* y, int32_t T,
@@ -756,9 +766,9 @@ int mh_combine_bwd(mh_module* m, const void* g, int64_t ldg, const void* y, cons
                    void* stream);
 int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, const void* scale, const void* wp,
                 const void* wn, void* h, void* n, float* stats, int32_t T, int32_t C, float eps, void* stream);
-int mh_norm_bwd(mh_module* m, const void* gh, const void* gn, const void* x, const void* y, const void* gate,
-                const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy, void* dgate,
-                float* part, int32_t T, int32_t C, int32_t blocks, void* stream);
+int mh_norm_bwd(mh_module* m, mh_module* sums, const void* gh, const void* gn, const void* x, const void* y,
+                const void* gate, const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy,
+                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, int32_t groups, void* stream);
 
 #ifdef __cplusplus
 }

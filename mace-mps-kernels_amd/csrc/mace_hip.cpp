@@ -1211,9 +1211,10 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
 // ---------------------------------------------------------------------------------------------- trainable node layers
 namespace {
 
-// Pieces of at most L rows that R rows in E groups can make, with the rows of no group counted as one group more.
+// Pieces of at most L rows that R rows in E groups can make, with the rows of no group counted as one group more (no more
+// groups have rows than there are rows).
 int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
-    return (R + L - 1) / L + (offsets ? E + 1 : 0);
+    return (R + L - 1) / L + (offsets ? std::min(E, R) + 1 : 0);
 }
 
 }  // namespace
@@ -1221,10 +1222,8 @@ int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
 extern "C" {
 
 int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
-               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, int32_t act,
-               void* stream) {
+               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream) {
     if (R < 0 || N < 0 || K < 0 || E < 1 || (E > 1 && !offsets)) return fail(-1, "mh_mm_rows: bad sizes");
-    if (act < 0 || act > 3) return fail(-1, "mh_mm_rows: unknown activation");
     if (R == 0 || N == 0) return 0;
     if (!C || (K > 0 && (!A || !B))) return fail(-1, "mh_mm_rows: NULL operand");
     if (lda < K || (res && ldr < N)) return fail(-1, "mh_mm_rows: rows overlap (ld below the row's length)");
@@ -1232,7 +1231,7 @@ int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C,
     const Kernel& k = m->k[MH_MM_ROWS];
     if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_mm_rows: too many rows");
     const int64_t tiles = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
-    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldr, &R, &N, &K, &E, &act};
+    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldr, &R, &N, &K, &E};
     return launch_blocks(m, MH_MM_ROWS, tiles, args, stream, "mh_mm_rows");
 }
 
@@ -1257,19 +1256,52 @@ int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets
         return fail(-1, "mh_mm_sum: bad sizes");
     if (n == 0) return 0;
     if (!out || (R > 0 && !part)) return fail(-1, "mh_mm_sum: NULL operand");
-    void* args[] = {&part, &out, &offsets, &R, &E, &L, &n};
-    return launch_blocks(m, MH_MM_SUM, (n + 1023) / 1024, args, stream, "mh_mm_sum", E);
+    // waves that share a column's slots: as many as there are slots, sixteen at most
+    const int64_t slots = (static_cast<int64_t>(R) + L - 1) / L;
+    int32_t lg = 0;
+    while (lg < 4 && (1LL << lg) < slots) ++lg;
+    const int64_t columns = 256LL * (16 >> lg);
+    void* args[] = {&part, &out, &offsets, &R, &E, &L, &lg, &n};
+    return launch_blocks(m, MH_MM_SUM, (n + columns - 1) / columns, args, stream, "mh_mm_sum", E);
 }
 
-int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, const int32_t* offsets,
-                int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, void* db,
+                const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
     if (R < 0 || N < 0 || E < 1 || (E > 1 && !offsets) || L < 1 || slots < 0 || R > 0x7fffffff - L)
         return fail(-1, "mh_mm_slope: bad sizes");
-    if (R == 0 || N == 0) return 0;
-    if (!g || (!p && !part)) return fail(-1, "mh_mm_slope: NULL operand");
+    if (db && (offsets || slots != 1 || L < R)) return fail(-1, "mh_mm_slope: db itself takes one slot of all rows");
+    if (N == 0 || (R == 0 && !db)) return 0;
+    if ((R > 0 && !g) || (!p && !part && !db)) return fail(-1, "mh_mm_slope: NULL operand");
     if (ldg < N) return fail(-1, "mh_mm_slope: rows overlap (ld below the row's length)");
-    void* args[] = {&g, &slope, &p, &part, &offsets, &ldg, &R, &N, &E, &L};
+    void* args[] = {&g, &slope, &p, &part, &db, &offsets, &ldg, &R, &N, &E, &L};
     return launch_blocks(m, MH_MM_SLOPE, slots, args, stream, "mh_mm_slope", (static_cast<int64_t>(N) + 255) / 256);
+}
+
+int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g, int64_t ldg, const void* slope,
+              const void* W, const void* x, int64_t ldx, const int32_t* offsets, void* p, void* dx, void* dW, void* db,
+              float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
+              int32_t slots_o, void* stream) {
+    if ((slope != nullptr) != (p != nullptr)) return fail(-1, "mh_mm_bwd: p goes with slope");
+    if (p || db) {
+        const bool whole = db && !offsets && slots_s == 1;
+        if (int rc = mh_mm_slope(sums, g, ldg, slope, p, db && !whole ? part : nullptr, whole ? db : nullptr, offsets, R, N, E,
+                                 Ls, slots_s, stream))
+            return rc;
+        if (db && !whole)
+            if (int rc = mh_mm_sum(sums, part, db, offsets, R, E, Ls, N, stream)) return rc;
+    }
+    if (p) {
+        g = p;
+        ldg = N;
+    }
+    if (dx)
+        if (int rc = mh_mm_rows(rows, g, ldg, W, dx, nullptr, nullptr, 0, nullptr, offsets, R, K, N, E, stream)) return rc;
+    if (dW) {
+        // the parts of db have been added by now: their place is free
+        if (int rc = mh_mm_outer(outer, g, ldg, x, ldx, dW, part, offsets, R, N, K, E, Lo, slots_o, stream)) return rc;
+        if (Lo) return mh_mm_sum(sums, part, dW, offsets, R, E, Lo, static_cast<int64_t>(N) * K, stream);
+    }
+    return 0;
 }
 
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
@@ -1334,14 +1366,16 @@ int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, co
     return launch_blocks(m, MH_NORM_FWD, (static_cast<int64_t>(T) + per - 1) / per, args, stream, "mh_norm_fwd");
 }
 
-int mh_norm_bwd(mh_module* m, const void* gh, const void* gn, const void* x, const void* y, const void* gate,
-                const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy, void* dgate,
-                float* part, int32_t T, int32_t C, int32_t blocks, void* stream) {
-    if (T < 0 || C < 0 || blocks < 0) return fail(-1, "mh_norm_bwd: bad sizes");
-    if (T == 0 || C == 0) return 0;
-    if (!x || !stats) return fail(-1, "mh_norm_bwd: NULL operand");
+int mh_norm_bwd(mh_module* m, mh_module* sums, const void* gh, const void* gn, const void* x, const void* y,
+                const void* gate, const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy,
+                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, int32_t groups, void* stream) {
+    if (T < 0 || C < 0 || blocks < 1 || groups < 1) return fail(-1, "mh_norm_bwd: bad sizes");
+    if (C == 0) return 0;
+    if ((T > 0 && (!x || !stats)) || (dw && !part)) return fail(-1, "mh_norm_bwd: NULL operand");
+    if (!dw) part = nullptr;
     void* args[] = {&gh, &gn, &x, &y, &gate, &scale, &wp, &wn, &stats, &dx, &dy, &dgate, &part, &T, &C};
-    return launch_blocks(m, MH_NORM_BWD, blocks, args, stream, "mh_norm_bwd");
+    if (int rc = launch_blocks(m, MH_NORM_BWD, blocks, args, stream, "mh_norm_bwd")) return rc;
+    return dw ? mh_mm_sum(sums, part, dw, nullptr, groups, 1, 1, 3LL * C, stream) : 0;
 }
 
 }  // extern "C"

@@ -140,30 +140,57 @@ struct mm_vec {
 #define MM_SILU 2
 #define MM_GELU 3
 
-// relu keeps NaN (comparisons with it are false); silu(a) = a / (1 + e^-a); gelu(a) = a Phi(a), Phi the normal
-// distribution function by erf
-__device__ __forceinline__ float mm_act(int act, float a) {
-    if (act == MM_RELU) return a < 0.f ? 0.f : a;
-    if (act == MM_SILU) return a / (1.f + expf(-a));
-    if (act == MM_GELU) return 0.5f * a * (1.f + erff(a * 0.70710678f));
-    return a;
+// act(a), and act'(a) in `slope`, from one exponential: relu (NaN stays NaN), silu(a) = a q with q = 1 / (1 + e^-a) and slope
+// q + a q (1 - q), gelu(a) = a Phi(a) with Phi the normal distribution function and slope Phi + a e^(-a^2/2) / sqrt(2 pi).
+// For 128 values a thread these are a large part of a tile's time (a call of expf and two divisions each were 190 of 316 us
+// at 16,384 x 4,096 x 1,024 in bfloat16), so: the hardware's 2^x and 1/x (one ulp each), with the rounding error of
+// a log2(e) carried along for float32, and for the 16-bit types erf by Abramowitz and Stegun 7.1.26, erfc(z) =
+// poly(1 / (1 + p z)) e^(-z^2) to 1.5e-7, which shares the slope's exponential; float32 calls erff.
+template <int TY>
+__device__ __forceinline__ float mm_exp(float a) {
+    const float t = a * 1.44269504f;
+    const float e = __builtin_amdgcn_exp2f(t);
+    if constexpr (TY != MM_F32) return e;
+    // 2^r = 1 + r ln 2 for what rounding left out of t; nothing to add to 0 and infinity
+    const float r = __builtin_fmaf(a, 1.44269504f, -t) + a * 1.92596298e-8f;
+    return e > 0.f && e < __builtin_inff() ? __builtin_fmaf(e * r, 0.69314718f, e) : e;
 }
 
-__device__ __forceinline__ float mm_act_slope(int act, float a) {
-    if (act == MM_RELU) return a > 0.f ? 1.f : 0.f;
-    if (act == MM_SILU) {
-        const float q = 1.f / (1.f + expf(-a));
-        return q * (1.f + a * (1.f - q));
+template <int TY, int ACT>
+__device__ __forceinline__ float mm_activate(float a, float& slope) {
+    if constexpr (ACT == MM_RELU) {
+        slope = a > 0.f ? 1.f : 0.f;
+        return a < 0.f ? 0.f : a;
+    } else if constexpr (ACT == MM_SILU) {
+        const float q = __builtin_amdgcn_rcpf(1.f + mm_exp<TY>(-a)), y = a * q;
+        slope = __builtin_fmaf(y, 1.f - q, q);
+        return y;
+    } else if constexpr (ACT == MM_GELU) {
+        const float g = mm_exp<TY>(-0.5f * a * a);
+        float phi;
+        if constexpr (TY == MM_F32) {
+            phi = 0.5f * (1.f + erff(a * 0.70710678f));
+        } else {
+            const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f * 0.70710678f, __builtin_fabsf(a), 1.f));
+            float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+            p = __builtin_fmaf(t, p, 1.421413741f);
+            p = __builtin_fmaf(t, p, -0.284496736f);
+            p = __builtin_fmaf(t, p, 0.254829592f);
+            const float c = 0.5f * t * p * g;            // Phi(-|a|)
+            phi = a < 0.f ? c : 1.f - c;
+        }
+        slope = __builtin_fmaf(a * 0.39894228f, g, phi);
+        return a * phi;
     }
-    if (act == MM_GELU) return 0.5f * (1.f + erff(a * 0.70710678f)) + a * 0.39894228f * expf(-0.5f * a * a);
-    return 1.f;
+    slope = 1.f;
+    return a;
 }
 
 // act'(a) as the forward keeps it for the backward: float32, or for the 16-bit types fixed point with steps of 2^-15 from
 // -0.5 (the slopes of all activations lie in [-0.13, 1.13]; 0 and 1 are exact; 65535 stands for NaN): its error of 2^-16
 // is far below the 2^-8 (2^-11) to which these types round the product p, where a slope kept in them would add its own.
 __device__ __forceinline__ unsigned mm_slope_code(float d) {
-    return d == d ? (unsigned)__float2int_rn((d + 0.5f) * 32768.f) : 65535u;
+    return d == d ? (unsigned)(int)__builtin_rintf(__builtin_fmaf(d, 32768.f, 16384.f)) : 65535u;
 }
 __device__ __forceinline__ float mm_slope_value(unsigned c) {
     return c == 65535u ? __uint_as_float(0x7FC00000u) : (float)(int)c * 3.0517578125e-5f - 0.5f;
@@ -444,6 +471,177 @@ struct mm_tile {
     }
 };
 
+// The same sums for 16-bit operands that come to LDS without passing through registers: 16-byte buffer loads straight into it,
+// double-buffered.  An operand contiguous along k is laid out as above; a strided one keeps its rows of k, [k][ROWS], and its
+// fragments are read by transposing LDS reads (four k of 16 rows at a time).  Sixteen rows of a fragment are 32 bytes of a
+// row of k, and the 32-byte pieces of row k are exchanged by f(k) so that the rows which one read touches fall into different
+// banks.  Every operand's contiguous length, its row distance and its address are multiples of 16 bytes (the caller
+// checks); a load past the rows' end repeats the last ones, and one past kend is out of the buffer's range and gives zeros.
+typedef __attribute__((address_space(3))) void mm_lds_void;
+
+__device__ __forceinline__ int mm_turn(int k) { return (k & 3) | (k >> 1 & 4); }
+__device__ __forceinline__ unsigned mm_lds_at(const void* p) {
+    return (unsigned)(unsigned long long)(const __attribute__((address_space(3))) void*)p;
+}
+
+// Pairs of transposing reads at LDS bytes at[c] and at[c] + STEP, complete at the end of the block.  Written out because the
+// compiler's own form of them waits for all loads into LDS that are under way, those of the next tile too.
+template <int STEP>
+__device__ __forceinline__ void mm_read_turned(const unsigned (&at)[4], mh_u2 (&lo)[4], mh_u2 (&hi)[4]) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %4, %8 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %1, %9\n\tds_read_b64_tr_b16 %5, %9 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %2, %10\n\tds_read_b64_tr_b16 %6, %10 offset:%12\n\t"
+        "ds_read_b64_tr_b16 %3, %11\n\tds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(lo[2]), "=&v"(lo[3]), "=&v"(hi[0]), "=&v"(hi[1]), "=&v"(hi[2]), "=&v"(hi[3])
+        : "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(STEP)
+        : "memory");
+}
+template <int STEP>
+__device__ __forceinline__ void mm_read_turned(const unsigned (&at)[2], mh_u2 (&lo)[2], mh_u2 (&hi)[2]) {
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %2, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %1, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
+        : "v"(at[0]), "v"(at[1]), "n"(STEP)
+        : "memory");
+}
+
+template <bool STRIDED, int ROWS, int BK, int THREADS>
+struct mm_mover {
+    static constexpr int OPR = BK / 8, ITEMS = ROWS * OPR / THREADS;
+    static_assert(ROWS * OPR % THREADS == 0, "a tile is a whole number of loads per thread");
+    unsigned off[ITEMS];                                 // byte offset of each load from the tile's first element
+    int at[ITEMS];                                       // its k within the tile
+
+    __device__ __forceinline__ void init(long long ld, int rows) {
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j) {
+            const int s = threadIdx.x + j * THREADS;
+            if constexpr (STRIDED) {
+                const int k = s / (ROWS / 8), p = s % (ROWS / 8);
+                const int c = ((p >> 1) ^ (mm_turn(k) & (ROWS / 16 - 1))) * 16 + (p & 1) * 8;
+                at[j] = k;
+                off[j] = (unsigned)(k * ld + min(c, rows - 8)) * 2;
+            } else {
+                const int r = s / OPR, o = (s % OPR) ^ (r / (16 / OPR) & (OPR - 1));
+                at[j] = 8 * o;
+                off[j] = (unsigned)(min(r, rows - 1) * ld + 8 * o) * 2;
+            }
+        }
+    }
+    // `left`: the k that exist from the tile's first on
+    __device__ __forceinline__ void issue(const unsigned short* p, int left, mh_u4* tile) const {
+        const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<unsigned short*>(p), 0, 0x7fffffff, 0x00020000);
+        const int w = threadIdx.x & ~63;
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (mm_lds_void*)(tile + w + j * THREADS), 16,
+                                                     at[j] < left ? off[j] : 0x80000000u, 0, 0, 0);
+    }
+};
+
+template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK>
+struct mm_fast_tile {
+    typedef unsigned short T;
+    static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
+    static constexpr int TA = BM * BK / 8, TB = BN * BK / 8, LDS = 2 * (TA + TB);
+    mh_f4 acc[FM][FN];
+
+    // Fragments of 16 rows each from row0 on at k 32 ks .. + 31: contiguous operands by 16-byte reads; strided ones by
+    // transposing reads, where sixteen lanes read four k of 16 rows (lane i: four rows of k i / 4) and lane i receives the
+    // four k of row i.
+    template <bool STRIDED, int ROWS, int N>
+    __device__ __forceinline__ static void fragments(mh_u4 (&f)[N], mh_u4* tile, int row0, int ks) {
+        const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
+        if constexpr (STRIDED) {
+            const int k = 32 * ks + 8 * q + (i >> 2);
+            constexpr int G = N < 4 ? N : 4;
+#pragma unroll
+            for (int h = 0; h < N; h += G) {
+                unsigned at[G];
+                mh_u2 lo[G], hi[G];
+#pragma unroll
+                for (int c = 0; c < G; ++c)
+                    at[c] = mm_lds_at(tile) + 2 * (k * ROWS + ((row0 / 16 + h + c) ^ (mm_turn(k) & (ROWS / 16 - 1))) * 16 + (i & 3) * 4);
+                mm_read_turned<8 * ROWS>(at, lo, hi);
+#pragma unroll
+                for (int c = 0; c < G; ++c) f[h + c] = mh_u4{lo[c].x, lo[c].y, hi[c].x, hi[c].y};
+            }
+        } else {
+#pragma unroll
+            for (int c = 0; c < N; ++c) f[c] = tile[mm_place<BK / 8>(row0 + 16 * c + i, 4 * ks + q)];
+        }
+    }
+
+    __device__ __forceinline__ void products(mh_u4* a, mh_u4* b) {
+        const int wave = threadIdx.x >> 6, ra = (wave / WN) * 16 * FM, rb = (wave % WN) * 16 * FN;
+#pragma unroll
+        for (int ks = 0; ks < BK / 32; ++ks) {
+            mh_u4 fa[FM], fb[FN];
+            fragments<BS, BN, FN>(fb, b, rb, ks);
+            fragments<AS, BM, FM>(fa, a, ra, ks);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mm_mfma<TY>(fb[j], fa[i], acc[i][j]);
+        }
+    }
+
+    // The loads of the next tile (where `left` > 0) and this one's products.  The four places are distinct: without that the
+    // compiler waits for the loads before it reads the tile that is there.
+    __device__ __forceinline__ void step(const mm_mover<AS, BM, BK, THREADS>& ma, const mm_mover<BS, BN, BK, THREADS>& mb, const T* A,
+                                         const T* B, int left, mh_u4* __restrict__ a, mh_u4* __restrict__ b,
+                                         mh_u4* __restrict__ an, mh_u4* __restrict__ bn) {
+        if (left > 0) {
+            ma.issue(A, left, an);
+            mb.issue(B, left, bn);
+        }
+        products(a, b);
+    }
+
+    __device__ __forceinline__ void run(mh_u4* lds, const T* A, long long lda, int arows, const T* B, long long ldb, int brows,
+                                        int kbeg, int kend) {
+        mm_mover<AS, BM, BK, THREADS> ma;
+        mm_mover<BS, BN, BK, THREADS> mb;
+        ma.init(lda, arows);
+        mb.init(ldb, brows);
+        const long long sa = AS ? lda : 1, sb = BS ? ldb : 1;
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) acc[i][j] = mh_f4{0.f, 0.f, 0.f, 0.f};
+        if (kbeg >= kend) return;                       // uniform over the workgroup
+        mh_u4 *a0 = lds, *a1 = lds + TA, *b0 = lds + 2 * TA, *b1 = lds + 2 * TA + TB;
+        ma.issue(A + kbeg * sa, kend - kbeg, a0);
+        mb.issue(B + kbeg * sb, kend - kbeg, b0);
+        for (int k = kbeg; k < kend; k += BK) {
+            // the tile of this step is in LDS, and every wave is done with the other buffer
+            __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
+            __syncthreads();
+            step(ma, mb, A + (k + BK) * sa, B + (k + BK) * sb, kend - k - BK, a0, b0, a1, b1);
+            mh_u4* t = a0;
+            a0 = a1;
+            a1 = t;
+            t = b0;
+            b0 = b1;
+            b1 = t;
+        }
+    }
+
+    template <typename F>
+    __device__ __forceinline__ void each(F f) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        const int m0 = (wave / WN) * 16 * FM + (lane & 15), n0 = (wave % WN) * 16 * FN + 4 * (lane >> 4);
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) f(m0 + 16 * i, n0 + 16 * j, acc[i][j]);
+    }
+};
+
 // The tile (mt, nt) of a block among MT x NT: bands of eight row tiles, walked column by column, in one contiguous range
 // per XCD, so that blocks which share an L2 share operand tiles.
 __device__ __forceinline__ void mm_tile_of(int b, int blocks, int MT, int NT, int& mt, int& nt) {
@@ -452,13 +650,47 @@ __device__ __forceinline__ void mm_tile_of(int b, int blocks, int MT, int NT, in
     nt = i / high;
 }
 
+// What follows the sums v of four outputs, row r of the result and columns n to n + 3 of which `c` exist: bias (the group's),
+// activation with its slope kept where wanted, residual, one rounding.
+template <int TY, int ACT>
+__device__ __forceinline__ void mm_finish(mh_f4 v, long long r, int n, int c, const typename mm_type<TY>::t* bias,
+                                          const typename mm_type<TY>::t* res, long long ldr, void* slope_,
+                                          typename mm_type<TY>::t* C, int N) {
+    const long long at = r * N + n;
+    if (bias) v += mm_get4<TY>(bias + n, c);
+    if constexpr (ACT != MM_NONE) {
+        mh_f4 d;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float t;
+            v[j] = mm_activate<TY, ACT>(v[j], t);
+            d[j] = t;
+        }
+        if (slope_) {
+            if constexpr (TY == MM_F32) {
+                mm_put4<MM_F32>(static_cast<float*>(slope_) + at, d, c);
+            } else {
+                unsigned short* s = static_cast<unsigned short*>(slope_) + at;
+                if (c >= 4)
+                    *reinterpret_cast<mh_u2x*>(s) = mh_u2{mm_slope_code(d[0]) | mm_slope_code(d[1]) << 16,
+                                                          mm_slope_code(d[2]) | mm_slope_code(d[3]) << 16};
+                else
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+                        if (j < c) s[j] = (unsigned short)mm_slope_code(d[j]);
+            }
+        }
+    }
+    if (res) v += mm_get4<TY>(res + r * ldr + n, c);
+    mm_put4<TY>(C + at, v, c);
+}
+
 // Forward and input gradient: R rows of A [R, K] in groups, B the group's weights ([N, K], or [K, N] where BS), the
 // epilogue v = sums + bias[e]; slope = act'(v); C = act(v) + res.  Rows of no group are written as zeros.
-template <int TY, bool BS, int WM, int WN, int FM, int FN, int BK, int BUFS>
+template <int TY, bool BS, int ACT, typename tile_t>
 __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
                                              void* slope_, const int* off, long long lda, long long ldr, int R, int N, int K,
-                                             int E, int act) {
-    typedef mm_tile<TY, false, BS, WM, WN, FM, FN, BK, BUFS> tile_t;
+                                             int E) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
     const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT;
@@ -480,44 +712,120 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
     const T* A = static_cast<const T*>(A_) + (long long)r0 * lda;
     const T* B = static_cast<const T*>(B_) + (long long)e * N * K + (BS ? (long long)n0 : (long long)n0 * K);
     t.run(lds, A, lda, rows, B, BS ? N : K, min(N - n0, tile_t::BN), 0, K);
-    const T* bias = bias_ ? static_cast<const T*>(bias_) + (long long)e * N + n0 : nullptr;
-    const T* res = res_ ? static_cast<const T*>(res_) + (long long)r0 * ldr + n0 : nullptr;
+    const T* bias = bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr;
     t.each([&](int m, int n, mh_f4 v) {
         const int c = N - n0 - n;                       // columns that exist from here on
-        if (m >= rows || c <= 0) return;
-        if (bias) v += mm_get4<TY>(bias + n, c);
-        if (slope_) {
-            const long long at = ((long long)r0 + m) * N + n0 + n;
-            mh_f4 d;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) d[j] = mm_act_slope(act, v[j]);
-            if constexpr (TY == MM_F32) {
-                mm_put4<MM_F32>(static_cast<float*>(slope_) + at, d, c);
-            } else {
-                unsigned short* s = static_cast<unsigned short*>(slope_) + at;
-                if (c >= 4)
-                    *reinterpret_cast<mh_u2x*>(s) = mh_u2{mm_slope_code(d[0]) | mm_slope_code(d[1]) << 16,
-                                                          mm_slope_code(d[2]) | mm_slope_code(d[3]) << 16};
-                else
-#pragma unroll
-                    for (int j = 0; j < 3; ++j)
-                        if (j < c) s[j] = (unsigned short)mm_slope_code(d[j]);
-            }
-        }
-        if (act != MM_NONE)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = mm_act(act, v[j]);
-        if (res) v += mm_get4<TY>(res + (long long)m * ldr + n, c);
-        mm_put4<TY>(C + (long long)m * N + n, v, c);
+        if (m < rows && c > 0)
+            mm_finish<TY, ACT>(v, (long long)r0 + m, n0 + n, c, bias, static_cast<const T*>(res_), ldr, slope_,
+                               static_cast<T*>(C_), N);
     });
+}
+
+// The forward for few rows: a workgroup takes 16 TM rows of a group and 16 columns, its WAVES waves share the contraction and
+// add their sums through LDS in wave order.  Both operands go from memory to the matrix cores' registers: weights are read
+// once and no tile of rows is worth staging.  Bound by the weights' bytes and by latency: a wave keeps four 128-byte
+// pieces of 16 weight rows in flight.  float32 uses v_mfma_f32_16x16x4_f32 (k in the order 4 q + j of four steps).
+template <int TY, int ACT, int TM, int WAVES>
+__device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
+                                            void* slope_, const int* off, long long lda, long long ldr, int R, int N, int K,
+                                            int E) {
+    typedef typename mm_type<TY>::t T;
+    constexpr int V = TY == MM_F32 ? 4 : 8, STEP = 4 * V, BATCH = 4;
+    __shared__ mh_f4 sums[WAVES][TM][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, q = lane >> 4;
+    const int NT = (N + 15) / 16, mt = blockIdx.x / NT, n0 = blockIdx.x % NT * 16;
+    int e, r0, r1;
+    const bool live = mm_slot(off, E, R, 16 * TM, mt, e, r0, r1);
+    if (r0 >= R) return;
+    const int rows = r1 - r0, cols = min(N - n0, 16);
+    T* C = static_cast<T*>(C_);
+    if (!live) {
+        for (int j = threadIdx.x; j < rows * cols; j += 64 * WAVES) C[(long long)(r0 + j / cols) * N + n0 + j % cols] = 0;
+        return;
+    }
+    const T* b = static_cast<const T*>(B_) + ((long long)e * N + n0 + min(i, cols - 1)) * K + V * q;
+    const T* a[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t)
+        a[t] = static_cast<const T*>(A_) + (long long)(r0 + min(16 * t + i, rows - 1)) * lda + V * q;
+    mh_f4 acc[TM];
+#pragma unroll
+    for (int t = 0; t < TM; ++t) acc[t] = mh_f4{0.f, 0.f, 0.f, 0.f};
+    auto product = [&](mh_u4 w, mh_u4 x, mh_f4 c) {
+        if constexpr (TY == MM_F32) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(w[j]), __uint_as_float(x[j]), c, 0, 0, 0);
+            return c;
+        } else {
+            return mm_mfma<TY>(w, x, c);
+        }
+    };
+    // pairs of steps (128 bytes of a row), wave by wave
+    const int pairs = K / (2 * STEP);
+    int p = wave;
+    for (; p + (BATCH - 1) * WAVES < pairs; p += BATCH * WAVES) {
+        mh_u4 w[2 * BATCH], x[TM][2 * BATCH];
+#pragma unroll
+        for (int u = 0; u < 2 * BATCH; ++u)
+            w[u] = *reinterpret_cast<const mh_u4x*>(b + ((p + u / 2 * WAVES) * 2 + u % 2) * STEP);
+#pragma unroll
+        for (int t = 0; t < TM; ++t)
+#pragma unroll
+            for (int u = 0; u < 2 * BATCH; ++u)
+                x[t][u] = *reinterpret_cast<const mh_u4x*>(a[t] + ((p + u / 2 * WAVES) * 2 + u % 2) * STEP);
+#pragma unroll
+        for (int u = 0; u < 2 * BATCH; ++u)
+#pragma unroll
+            for (int t = 0; t < TM; ++t) acc[t] = product(w[u], x[t][u], acc[t]);
+    }
+    for (; p < pairs; p += WAVES)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const mh_u4 w = *reinterpret_cast<const mh_u4x*>(b + (p * 2 + u) * STEP);
+#pragma unroll
+            for (int t = 0; t < TM; ++t)
+                acc[t] = product(w, *reinterpret_cast<const mh_u4x*>(a[t] + (p * 2 + u) * STEP), acc[t]);
+        }
+    // what a pair does not fill, by the last wave; both operands are zero past K
+    if (wave == WAVES - 1)
+        for (int k = pairs * 2 * STEP; k < K; k += STEP) {
+            const int left = K - k - V * q;
+            auto get = [&](const T* s) {
+                if (left >= V) return (mh_u4) * reinterpret_cast<const mh_u4x*>(s);
+                mh_u4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (j < left) {
+                        if constexpr (TY == MM_F32) v[j] = __float_as_uint(s[j]);
+                        else v[j / 2] |= (unsigned)s[j] << (16 * (j & 1));
+                    }
+                return v;
+            };
+            const mh_u4 w = get(b + k);
+#pragma unroll
+            for (int t = 0; t < TM; ++t) acc[t] = product(w, get(a[t] + k), acc[t]);
+        }
+#pragma unroll
+    for (int t = 0; t < TM; ++t) sums[wave][t][lane] = acc[t];
+    __syncthreads();
+    for (int t = wave; t < TM; t += WAVES) {
+        mh_f4 v = sums[0][t][lane];
+#pragma unroll
+        for (int k = 1; k < WAVES; ++k) v += sums[k][t][lane];
+        const int c = cols - 4 * q;
+        if (16 * t + i < rows && c > 0)
+            mm_finish<TY, ACT>(v, (long long)r0 + 16 * t + i, n0 + 4 * q, c,
+                               bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr,
+                               static_cast<const T*>(res_), ldr, slope_, C, N);
+    }
 }
 
 // Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  blockIdx.y is
 // the group (L 0: all its rows; none give zeros), or a slot of at most L of its rows whose sums go to part[slot] in float32.
-template <int TY, int WM, int WN, int FM, int FN, int BK, int BUFS>
+template <int TY, typename tile_t>
 __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, void* C_, float* part, const int* off,
                                               long long lda, long long ldb, int R, int M, int N, int E, int L) {
-    typedef mm_tile<TY, true, true, WM, WN, FM, FN, BK, BUFS> tile_t;
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
     const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT;
@@ -544,12 +852,16 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
     });
 }
 
-// out[e, i] = sum of part[s, i] over the group's slots, in their order: what ends a sum that was split over rows.
+// out[e, i] = sum of part[s, i] over the group's slots in a fixed order: what ends a sum that was split over rows.  2^lg waves
+// share a column's slots (wave w takes every 2^lg-th) and are added in wave order, so that few columns of many slots are
+// not one wave's chain of loads; 1024 threads, four columns a lane.
 template <int TY>
-__device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const int* off, int R, int E, int L, long long n) {
+__device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const int* off, int R, int E, int L, int lg,
+                                            long long n) {
     typedef typename mm_type<TY>::t T;
-    const int e = blockIdx.y;
-    const long long i = ((long long)blockIdx.x * blockDim.x + threadIdx.x) * 4;
+    __shared__ mh_f4 sums[16][64];
+    const int e = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & ((1 << lg) - 1);
+    const long long i = ((long long)blockIdx.x * (16 >> lg) + (wave >> lg)) * 256 + 4 * lane;
     int s0 = 0, s1 = 0;
     if (!off) {
         s1 = (R + L - 1) / L;
@@ -562,57 +874,88 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
             top = hi;
         }
     }
-    if (i >= n) return;
-    const int c = (int)min((long long)4, n - i);
+    const int c = (int)max((long long)0, min((long long)4, n - i));
     mh_f4 v = {0.f, 0.f, 0.f, 0.f};
-    for (int s = s0; s < s1; ++s) v += mm_get4<MM_F32>(part + (long long)s * n + i, c);
-    mm_put4<TY>(static_cast<T*>(out_) + (long long)e * n + i, v, c);
+    if (c >= 4) {
+#pragma unroll 8
+        for (int s = s0 + w; s < s1; s += 1 << lg) v += mm_get4<MM_F32>(part + (long long)s * n + i);
+    } else if (c > 0) {
+        for (int s = s0 + w; s < s1; s += 1 << lg) v += mm_get4<MM_F32>(part + (long long)s * n + i, c);
+    }
+    if (lg) {
+        sums[wave][lane] = v;
+        __syncthreads();
+        if (w) return;
+        for (int k = 1; k < 1 << lg; ++k) v += sums[wave + k][lane];
+    }
+    if (c > 0) mm_put4<TY>(static_cast<T*>(out_) + (long long)e * n + i, v, c);
 }
 
-// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1) and the slots' sums of its columns in float32, before
-// rounding, into part [slots, N] (NULL: none).  A workgroup takes a slot of L rows and 256 columns, 64 threads of four
-// columns each by four rows at a time.
+// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1) and the sums of its columns in float32, before
+// rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows, rounded into db (both NULL: none).
+// A workgroup takes a slot and 256 columns, 64 threads of four columns each by four rows at a time.
 template <int TY>
-__device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, const int* off,
+__device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, void* db, const int* off,
                                               long long ldg, int R, int N, int E, int L) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_f4 sums[4][64];
     int e, r0, r1;
-    if (!mm_slot(off, E, R, L, blockIdx.x, e, r0, r1)) return;
+    if (!mm_slot(off, E, R, L, blockIdx.x, e, r0, r1) && !db) return;      // db without rows: zeros
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int n = blockIdx.y * 256 + 4 * lane, c = N - n;
+    const T* g = static_cast<const T*>(g_) + n;
+    T* P = static_cast<T*>(P_);
     mh_f4 s = {0.f, 0.f, 0.f, 0.f};
-    if (c > 0) {
+    auto times = [&](mh_f4 v, mh_u4 d) {                 // the slope as it was loaded
+        if constexpr (TY == MM_F32) {
+            return v * __builtin_bit_cast(mh_f4, d);
+        } else {
+            return v * mh_f4{mm_slope_value(d.x & 0xFFFFu), mm_slope_value(d.x >> 16), mm_slope_value(d.y & 0xFFFFu),
+                             mm_slope_value(d.y >> 16)};
+        }
+    };
+    if (c >= 4) {
+#pragma unroll 4
         for (int r = r0 + w; r < r1; r += 4) {
-            mh_f4 v = mm_get4<TY>(static_cast<const T*>(g_) + (long long)r * ldg + n, c);
+            mh_f4 v = mm_get4<TY>(g + (long long)r * ldg);
             const long long at = (long long)r * N + n;
             if (slope_) {
                 if constexpr (TY == MM_F32) {
-                    v *= mm_get4<MM_F32>(static_cast<const float*>(slope_) + at, c);
+                    v = times(v, *reinterpret_cast<const mh_u4x*>(static_cast<const float*>(slope_) + at));
                 } else {
-                    const unsigned short* q = static_cast<const unsigned short*>(slope_) + at;
-                    mh_u2 k = {0u, 0u};
-                    if (c >= 4) {
-                        k = *reinterpret_cast<const mh_u2x*>(q);
-                    } else {
-                        k.x = q[0] | (c > 1 ? (unsigned)q[1] << 16 : 0u);
-                        k.y = c > 2 ? q[2] : 0u;
-                    }
-                    v *= mh_f4{mm_slope_value(k.x & 0xFFFFu), mm_slope_value(k.x >> 16), mm_slope_value(k.y & 0xFFFFu),
-                               mm_slope_value(k.y >> 16)};
+                    const mh_u2 d = *reinterpret_cast<const mh_u2x*>(static_cast<const unsigned short*>(slope_) + at);
+                    v = times(v, mh_u4{d.x, d.y, 0u, 0u});
                 }
             }
-            if (P_) mm_put4<TY>(static_cast<T*>(P_) + at, v, c);
+            if (P) mm_put4<TY>(P + at, v);
+            s += v;
+        }
+    } else if (c > 0) {
+        for (int r = r0 + w; r < r1; r += 4) {
+            mh_f4 v = mm_get4<TY>(g + (long long)r * ldg, c);
+            const long long at = (long long)r * N + n;
+            if (slope_) {
+                mh_u4 d = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    if (j < c) {
+                        if constexpr (TY == MM_F32) d[j] = static_cast<const unsigned*>(slope_)[at + j];
+                        else d[j / 2] |= (unsigned)static_cast<const unsigned short*>(slope_)[at + j] << (16 * (j & 1));
+                    }
+                v = times(v, d);
+            }
+            if (P) mm_put4<TY>(P + at, v, c);
             s += v;
         }
     }
-    if (!part) return;
+    if (!part && !db) return;
     sums[w][lane] = s;
     __syncthreads();
     if (w == 0 && c > 0) {
         s += sums[1][lane];
         s += sums[2][lane];
         s += sums[3][lane];
-        mm_put4<MM_F32>(part + (long long)blockIdx.x * N + n, s, c);
+        if (db) mm_put4<TY>(static_cast<T*>(db) + n, s, c);
+        else mm_put4<MM_F32>(part + (long long)blockIdx.x * N + n, s, c);
     }
 }

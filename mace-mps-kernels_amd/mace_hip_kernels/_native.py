@@ -132,16 +132,17 @@ _SIGS = {
     'mh_neighbour_list_work_size': (ctypes.c_size_t, [_I, _I, ctypes.c_int64]),
     'mh_neighbour_list': (ctypes.c_int, [_P] * 5 + [_I, _I, ctypes.c_double, ctypes.c_int64, ctypes.c_int64]
                           + [_P] * 3 + [_I] + [_P] * 3),
-    'mh_mm_rows': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_L, _P, _P] + [_I] * 5 + [_P]),
+    'mh_mm_rows': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_L, _P, _P] + [_I] * 4 + [_P]),
     'mh_mm_outer': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 3 + [_I] * 6 + [_P]),
     'mh_mm_sum': (ctypes.c_int, [_P] * 4 + [_I] * 3 + [_L, _P]),
-    'mh_mm_slope': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_I] * 5 + [_P]),
+    'mh_mm_slope': (ctypes.c_int, [_P, _P, _L] + [_P] * 5 + [_I] * 5 + [_P]),
+    'mh_mm_bwd': (ctypes.c_int, [_P] * 4 + [_L] + [_P] * 3 + [_L] + [_P] * 6 + [_I] * 8 + [_P]),
     'mh_expert_order': (ctypes.c_int, [_P, _P] + [_I] * 3 + [_P, _I] + [_P] * 4),
     'mh_dispatch': (ctypes.c_int, [_P, _P, _L] + [_P] * 3 + [_I] * 5 + [_P]),
     'mh_combine': (ctypes.c_int, [_P] * 5 + [_L, _P] + [_I] * 4 + [_P]),
     'mh_combine_bwd': (ctypes.c_int, [_P, _P, _L] + [_P] * 6 + [_I] * 5 + [_P]),
     'mh_norm_fwd': (ctypes.c_int, [_P] * 10 + [_I, _I, ctypes.c_float, _P]),
-    'mh_norm_bwd': (ctypes.c_int, [_P] * 14 + [_I] * 3 + [_P]),
+    'mh_norm_bwd': (ctypes.c_int, [_P] * 16 + [_I] * 4 + [_P]),
 }
 EXPORTS = tuple(_SIGS)
 

@@ -96,22 +96,14 @@ class _BlockNormFn(torch.autograd.Function):
         T = x.numel() // C if C else 0
         dev, dt, P, lib = x.device, x.dtype, _native.ptr, _native.load()
         dx, dy, dgate = (torch.empty_like(t) if w else None for t, w in zip((x, y, gate), need[:3]))
-        sums = any(need[3:6])
-        dsum = torch.empty(3, C, device=dev, dtype=dt) if sums else None
-        if T:
-            tpr, nv = shape(C, dt)
-            per = rows_per_block(tpr)
-            blocks = min(-(-T // per), 4 * CUS)
-            part = torch.empty(blocks * per, 3, C, device=dev, dtype=torch.float32) if sums else None
-            s = _native.stream_of(x)
-            _native.launch('nm_bwd', lib.mh_norm_bwd, module(dev, dt, tpr, nv, layer, y is not None, gmode).handle, P(gh),
-                           P(gn), P(x), P(y), P(gate), P(scale), P(wp), P(wn), P(stats), P(dx), P(dy), P(dgate), P(part), T,
-                           C, blocks, s)
-            if sums:
-                _native.launch('mm_sum', lib.mh_mm_sum, mm_module(dev, dt, 'sum').handle, P(part), P(dsum), None,
-                               blocks * per, 1, 1, 3 * C, s)
-        elif sums:
-            dsum.zero_()
+        dsum = torch.empty((3, C), device=dev, dtype=dt) if any(need[3:6]) else None
+        tpr, nv = shape(C, dt)
+        per = rows_per_block(tpr)
+        blocks = max(1, min(-(-T // per), 4 * CUS))
+        part = None if dsum is None else torch.empty((blocks * per, 3, C), device=dev, dtype=torch.float32)
+        _native.launch('nm_bwd', lib.mh_norm_bwd, module(dev, dt, tpr, nv, layer, y is not None, gmode).handle,
+                       mm_module(dev, dt, 'sum').handle, P(gh), P(gn), P(x), P(y), P(gate), P(scale), P(wp), P(wn), P(stats),
+                       P(dx), P(dy), P(dgate), P(part), P(dsum), T, C, blocks, blocks * per, _native.stream_of(x))
         return (dx, dy, dgate, *(dsum[i] if w else None for i, w in enumerate(need[3:6])), None, None, None)
 
 

@@ -30,20 +30,22 @@ def test_c_entry_points_refuse_bad_arguments():
     one = torch.zeros(64)
     p = one.data_ptr()
     cases = [
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, -1, 4, 8, 1, 0, None), 'bad sizes'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 2, 0, None), 'bad sizes'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, 9, None), 'activation'),
-        (lambda: lib.mh_mm_rows(None, None, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, 0, None), 'NULL'),
-        (lambda: lib.mh_mm_rows(None, p, 7, p, p, None, None, 0, None, None, 2, 4, 8, 1, 0, None), 'overlap'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, p, 3, None, None, 2, 4, 8, 1, 0, None), 'overlap'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, 0, None), 'not bound'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, -1, 4, 8, 1, None), 'bad sizes'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 2, None), 'bad sizes'),
+        (lambda: lib.mh_mm_rows(None, None, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'NULL'),
+        (lambda: lib.mh_mm_rows(None, p, 7, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'overlap'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, p, 3, None, None, 2, 4, 8, 1, None), 'overlap'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'not bound'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, None, None, None, 2, 4, 4, 1, 0, 1, None), 'NULL'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, p, None, None, 2, 4, 4, 1, 16, 1, None), 'NULL'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, p, p, None, 2, 4, 4, 1, 16, 0, None), 'pieces'),
         (lambda: lib.mh_mm_outer(None, p, 3, p, 4, p, p, None, 2, 4, 4, 1, 0, 1, None), 'overlap'),
         (lambda: lib.mh_mm_sum(None, p, p, None, 4, 1, 0, 8, None), 'bad sizes'),
         (lambda: lib.mh_mm_sum(None, None, p, None, 4, 1, 4, 8, None), 'NULL'),
-        (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, None, 2, 4, 1, 4, 1, None), 'NULL'),
+        (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, None, None, 2, 4, 1, 4, 1, None), 'NULL'),
+        (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, p, None, 2, 4, 1, 1, 2, None), 'one slot'),
+        (lambda: lib.mh_mm_bwd(None, None, None, p, 4, p, p, p, 4, None, None, p, p, p, p, 2, 4, 4, 1, 4, 1, 0, 1, None),
+         'goes with slope'),
         (lambda: lib.mh_expert_order(None, p, 0, 4, 1025, None, 1, p, p, p, None), 'bad sizes'),
         (lambda: lib.mh_expert_order(None, p, 0, 4, 3, None, 2, p, p, p, None), 'NULL'),
         (lambda: lib.mh_dispatch(None, p, 8, p, p, p, 2, 1, 8, 1, 7, None), 'bad sizes'),
@@ -53,7 +55,8 @@ def test_c_entry_points_refuse_bad_arguments():
         (lambda: lib.mh_combine_bwd(None, p, 8, None, p, p, p, p, p, 2, 1, 8, 1, 1, None), 'NULL'),
         (lambda: lib.mh_norm_fwd(None, p, p, None, None, None, None, None, p, None, 2, 8, 1e-6, None), 'NULL'),
         (lambda: lib.mh_norm_fwd(None, p, None, None, None, None, None, None, p, None, 2, 8, 1e-6, None), 'null module'),
-        (lambda: lib.mh_norm_bwd(None, p, p, p, None, None, None, None, None, None, p, None, None, p, 2, 8, 1, None), 'NULL'),
+        (lambda: lib.mh_norm_bwd(None, None, p, p, p, None, None, None, None, None, None, p, None, None, p, p, 2, 8, 1, 4, None),
+         'NULL'),
     ]
     for i, (call, text) in enumerate(cases):
         assert call() != 0, i
@@ -84,7 +87,7 @@ def test_norm_shapes_hold_a_row():
 @pytest.mark.parametrize('dt', list(matmul.TYPES), ids=str)
 def test_every_module_compiles_for_gfx950(dt):
     sources = [matmul.source(dt, 'sum'), experts.source(dt), experts.order_source()]
-    sources += [matmul.source(dt, mode, tile) for mode in ('fwd', 'dx', 'dw') for tile in matmul.TILES]
+    sources += [matmul.source(dt, mode, tile) for mode in ('fwd', 'dx', 'dw') for tile in matmul.tiles(dt)]
     sources += [norms.source(dt, 64, 1, True, True, 0), norms.source(dt, 512, 2, False, True, 2)]
     for src in sources:
         assert _native.compile_source(src)[:4] == b'\x7fELF'

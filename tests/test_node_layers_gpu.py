@@ -122,6 +122,45 @@ def test_dense_over_many_tiles_and_split_sums(T, K, N, dt):
         assert torch.equal(t, u), f'{name} differs between two passes'
 
 
+@pytest.mark.parametrize('T,K,N', [(300, 200, 264), (1, 8, 8), (513, 64, 72), (260, 328, 520)])
+@pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+def test_every_tile_on_aligned_shapes(T, K, N, dt, monkeypatch):
+    """Each tile in all three products, one and three groups with a tail, whatever the sizes would have chosen."""
+    d = dev()
+    rng = np.random.default_rng(T)
+    cuts = sorted(rng.integers(0, T + 1, 3).tolist())
+    x, w, b, g = rand(rng, T, K, dt=dt), rand(rng, 3, N, K, dt=dt, scale=K ** -0.5), rand(rng, 3, N, dt=dt), rand(rng, T, N, dt=dt)
+    off = torch.tensor([0] + cuts, dtype=torch.int32)
+    one = dense_case(x, w[0], b[0], 'silu', None, g, dt)
+    three = [dense_case(x[i:j], w[e], b[e], 'silu', None, g[i:j], dt) for e, (i, j) in enumerate(zip([0] + cuts[:2], cuts))]
+    def choose(tile):
+        monkeypatch.setattr(matmul, '_choose_tile', lambda *a: 'slow64' if tile in matmul.FEW else tile)
+        monkeypatch.setattr(matmul, '_outer_tile', lambda *a: 'slow64' if tile in matmul.FEW else tile)
+        monkeypatch.setattr(matmul, '_few_tile', lambda *a: tile if tile in matmul.FEW else None)
+        matmul._rows_plan.cache_clear()
+        matmul._bwd_plan.cache_clear()
+
+    for tile in [*matmul.tiles(dt), *matmul.FEW]:
+        print(f'[case] tile {tile} T={T} K={K} N={N} {dt}', flush=True)
+        choose(tile)
+        leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+        y = mhk.dense(leaves[0], leaves[1][0], leaves[2][0], 'silu')
+        near('y', y, *one['y'])
+        grads = torch.autograd.grad(y, leaves, g.to(d))
+        for name, t in zip(('dx', 'dw', 'db'), (grads[0], grads[1][0], grads[2][0])):
+            near(name, t, *one[name])
+        y = mhk.expert_dense(*leaves[:2], off.to(d), leaves[2], 'silu')
+        grads = torch.autograd.grad(y, leaves, g.to(d))
+        assert (y[cuts[2]:] == 0).all() and (grads[0][cuts[2]:] == 0).all()
+        for e, want in enumerate(three):
+            i = slice(int(off[e]), int(off[e + 1]))
+            for name, t in zip(('y', 'dx', 'dw', 'db'), (y[i], grads[0][i], grads[1][e], grads[2][e])):
+                near(f'{name} of {e}', t, *want[name])
+    monkeypatch.undo()
+    matmul._rows_plan.cache_clear()
+    matmul._bwd_plan.cache_clear()
+
+
 @pytest.mark.parametrize('dt', [F32, BF16], ids=['f32', 'bf16'])
 def test_dense_takes_strides_leading_dimensions_and_no_rows(dt):
     d = dev()
