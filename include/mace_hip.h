@@ -740,9 +740,8 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  *
  * mh_norm_fwd: u = norm(y), h = x + scale gate u wp, n = norm(h) wn per row of C; gate, scale, wp, wn NULL: 1 (gate's shape is
  * compiled in); modules without a branch take y, h NULL.  stats [T, 4] float32 (NULL: none) for mh_norm_bwd, which gives dx,
- * dy, dgate and dw [3, C] = the gradients of scale, wp and wn (each may be NULL) from gh and gn (NULL: 0); part [groups, 3, C]
- * is scratch for the sums of the `groups` row groups (blocks times the rows that a workgroup takes at once) and sums a
- * module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD as norms.module does. */
+ * dy, dgate and dw [3, C] = the gradients of scale, wp and wn (each may be NULL) from gh and gn (NULL: 0); part [blocks, 3, C]
+ * is scratch for the workgroups' sums and sums a module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD as norms.module does. */
 int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
                int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream);
 int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
@@ -768,7 +767,7 @@ int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, co
                 const void* wn, void* h, void* n, float* stats, int32_t T, int32_t C, float eps, void* stream);
 int mh_norm_bwd(mh_module* m, mh_module* sums, const void* gh, const void* gn, const void* x, const void* y,
                 const void* gate, const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy,
-                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, int32_t groups, void* stream);
+                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1368,14 +1368,14 @@ int mh_norm_fwd(mh_module* m, const void* x, const void* y, const void* gate, co
 
 int mh_norm_bwd(mh_module* m, mh_module* sums, const void* gh, const void* gn, const void* x, const void* y,
                 const void* gate, const void* scale, const void* wp, const void* wn, const float* stats, void* dx, void* dy,
-                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, int32_t groups, void* stream) {
-    if (T < 0 || C < 0 || blocks < 1 || groups < 1) return fail(-1, "mh_norm_bwd: bad sizes");
+                void* dgate, float* part, void* dw, int32_t T, int32_t C, int32_t blocks, void* stream) {
+    if (T < 0 || C < 0 || blocks < 1) return fail(-1, "mh_norm_bwd: bad sizes");
     if (C == 0) return 0;
     if ((T > 0 && (!x || !stats)) || (dw && !part)) return fail(-1, "mh_norm_bwd: NULL operand");
     if (!dw) part = nullptr;
     void* args[] = {&gh, &gn, &x, &y, &gate, &scale, &wp, &wn, &stats, &dx, &dy, &dgate, &part, &T, &C};
     if (int rc = launch_blocks(m, MH_NORM_BWD, blocks, args, stream, "mh_norm_bwd")) return rc;
-    return dw ? mh_mm_sum(sums, part, dw, nullptr, groups, 1, 1, 3LL * C, stream) : 0;
+    return dw ? mh_mm_sum(sums, part, dw, nullptr, blocks, 1, 1, 3LL * C, stream) : 0;
 }
 
 }  // extern "C"

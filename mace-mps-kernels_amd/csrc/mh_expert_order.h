@@ -46,6 +46,7 @@ extern "C" __global__ __launch_bounds__(1024) void expert_place(const void* __re
         all = t < E ? run[t] : 0;
         __syncthreads();
     } else if (t < E) {
+#pragma unroll 8
         for (int k = 0; k < nb; ++k) {
             const int c = hist[(long long)k * (E + 1) + t];
             before += k < b ? c : 0;

@@ -97,19 +97,31 @@ template <int TY>
 struct mm_vec {
     static constexpr int V = TY == MM_F32 ? 4 : 8;
     float v[V];
-    __device__ __forceinline__ void get(const typename mm_type<TY>::t* p, int n) {
+    // the sixteen bytes as they lie in memory, and their values; STREAM: data that nothing reads again soon
+    template <bool STREAM = false>
+    __device__ __forceinline__ static mh_u4 raw(const typename mm_type<TY>::t* p, int n) {
         if (n >= V) {
-            const mh_u4 w = *reinterpret_cast<const mh_u4x*>(p);
+            if constexpr (STREAM) return __builtin_nontemporal_load(reinterpret_cast<const mh_u4x*>(p));
+            else return *reinterpret_cast<const mh_u4x*>(p);
+        }
+        mh_u4 w = {0u, 0u, 0u, 0u};
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                if constexpr (TY == MM_F32) v[j] = __uint_as_float(w[j]);
-                else v[j] = mm_widen<TY>((unsigned short)(w[j / 2] >> (16 * (j & 1))));
+        for (int j = 0; j < V; ++j)
+            if (j < n) {
+                if constexpr (TY == MM_F32) w[j] = __float_as_uint(p[j]);
+                else w[j / 2] |= (unsigned)p[j] << (16 * (j & 1));
             }
-        } else {
+        return w;
+    }
+    __device__ __forceinline__ void set(mh_u4 w) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = j < n ? mm_get<TY>(p + j) : 0.f;
+        for (int j = 0; j < V; ++j) {
+            if constexpr (TY == MM_F32) v[j] = __uint_as_float(w[j]);
+            else v[j] = mm_widen<TY>((unsigned short)(w[j / 2] >> (16 * (j & 1))));
         }
     }
+    __device__ __forceinline__ void get(const typename mm_type<TY>::t* p, int n) { set(raw(p, n)); }
+    template <bool STREAM = false>
     __device__ __forceinline__ void put(typename mm_type<TY>::t* p, int n) const {
         if (n >= V) {
             mh_u4 w;
@@ -118,7 +130,8 @@ struct mm_vec {
                 if constexpr (TY == MM_F32) w[j] = __float_as_uint(v[j]);
                 else w[j] = mm_round<TY>(v[2 * j]) | (unsigned)mm_round<TY>(v[2 * j + 1]) << 16;
             }
-            *reinterpret_cast<mh_u4x*>(p) = w;
+            if constexpr (STREAM) __builtin_nontemporal_store((mh_u4x)w, reinterpret_cast<mh_u4x*>(p));
+            else *reinterpret_cast<mh_u4x*>(p) = w;
         } else {
 #pragma unroll
             for (int j = 0; j < V; ++j)
@@ -378,7 +391,7 @@ __device__ __forceinline__ mh_f4 mm_mfma(mh_u4 a, mh_u4 b, mh_f4 c) {
 template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK, int BUFS>
 struct mm_tile {
     typedef typename mm_type<TY>::t T;
-    static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, OPR = BK / 8;
+    static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, OPR = BK / 8, ROWS = FM, COLS = FN;
     static constexpr int PLANES = TY == MM_F32 ? 3 : 1;
     static constexpr int TA = PLANES * BM * OPR, TB = PLANES * BN * OPR;      // octets of a buffer
     static constexpr int LDS = BUFS * (TA + TB);
@@ -451,23 +464,18 @@ struct mm_tile {
         }
     }
 
-    // Calls f(m, n, sums of D[m, n .. n + 3]) for the lane's fragments, m and n within the tile.
-    template <typename F>
-    __device__ __forceinline__ void each(F f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int m0 = (wave / WN) * 16 * FM + (lane & 15), n0 = (wave % WN) * 16 * FN + 4 * (lane >> 4);
+    // D[row(i), column(j) .. + 3] within the tile
+    __device__ __forceinline__ static int row(int i) { return ((threadIdx.x >> 6) / WN) * 16 * FM + (threadIdx.x & 15) + 16 * i; }
+    __device__ __forceinline__ static int column(int j) {
+        return ((threadIdx.x >> 6) % WN) * 16 * FN + 4 * (threadIdx.x >> 4 & 3) + 16 * j;
+    }
+    __device__ __forceinline__ mh_f4 value(int i, int j) const {
+        mh_f4 v = acc[i][j];
+        if constexpr (TY == MM_F32) {
 #pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) {
-                mh_f4 v = acc[i][j];
-                if constexpr (TY == MM_F32) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c)
-                        v[c] = __builtin_isfinite(v[c]) ? v[c] + low[i][j][c] : v[c];
-                }
-                f(m0 + 16 * i, n0 + 16 * j, v);
-            }
+            for (int c = 0; c < 4; ++c) v[c] = __builtin_isfinite(v[c]) ? v[c] + low[i][j][c] : v[c];
+        }
+        return v;
     }
 };
 
@@ -546,7 +554,7 @@ struct mm_mover {
 template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK>
 struct mm_fast_tile {
     typedef unsigned short T;
-    static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN;
+    static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, ROWS = FM, COLS = FN;
     static constexpr int TA = BM * BK / 8, TB = BN * BK / 8, LDS = 2 * (TA + TB);
     mh_f4 acc[FM][FN];
 
@@ -631,15 +639,11 @@ struct mm_fast_tile {
         }
     }
 
-    template <typename F>
-    __device__ __forceinline__ void each(F f) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        const int m0 = (wave / WN) * 16 * FM + (lane & 15), n0 = (wave % WN) * 16 * FN + 4 * (lane >> 4);
-#pragma unroll
-        for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) f(m0 + 16 * i, n0 + 16 * j, acc[i][j]);
+    __device__ __forceinline__ static int row(int i) { return ((threadIdx.x >> 6) / WN) * 16 * FM + (threadIdx.x & 15) + 16 * i; }
+    __device__ __forceinline__ static int column(int j) {
+        return ((threadIdx.x >> 6) % WN) * 16 * FN + 4 * (threadIdx.x >> 4 & 3) + 16 * j;
     }
+    __device__ __forceinline__ mh_f4 value(int i, int j) const { return acc[i][j]; }
 };
 
 // The tile (mt, nt) of a block among MT x NT: bands of eight row tiles, walked column by column, in one contiguous range
@@ -650,14 +654,10 @@ __device__ __forceinline__ void mm_tile_of(int b, int blocks, int MT, int NT, in
     nt = i / high;
 }
 
-// What follows the sums v of four outputs, row r of the result and columns n to n + 3 of which `c` exist: bias (the group's),
-// activation with its slope kept where wanted, residual, one rounding.
+// What follows the sums v of four outputs, at element `at` of the result, of which `c` exist: activation with its slope kept
+// where wanted, residual, one rounding (the bias is in v already).
 template <int TY, int ACT>
-__device__ __forceinline__ void mm_finish(mh_f4 v, long long r, int n, int c, const typename mm_type<TY>::t* bias,
-                                          const typename mm_type<TY>::t* res, long long ldr, void* slope_,
-                                          typename mm_type<TY>::t* C, int N) {
-    const long long at = r * N + n;
-    if (bias) v += mm_get4<TY>(bias + n, c);
+__device__ __forceinline__ void mm_finish(mh_f4 v, long long at, int c, mh_f4 res, void* slope_, typename mm_type<TY>::t* C) {
     if constexpr (ACT != MM_NONE) {
         mh_f4 d;
 #pragma unroll
@@ -681,8 +681,40 @@ __device__ __forceinline__ void mm_finish(mh_f4 v, long long r, int n, int c, co
             }
         }
     }
-    if (res) v += mm_get4<TY>(res + r * ldr + n, c);
-    mm_put4<TY>(C + at, v, c);
+    mm_put4<TY>(C + at, v + res, c);
+}
+
+// A tile's results to C at rows r0 .. + rows and columns n0 on.  The bias is loaded once for all rows, the residual a row of
+// fragments at a time: loaded one by one between the activations they were 85 of 274 us (bias, 16,384 x 4,096 x 1,024 in
+// bfloat16).  WHOLE: all columns of the tile exist.
+template <int TY, int ACT, bool WHOLE, typename tile_t>
+__device__ __forceinline__ void mm_store_tile(const tile_t& t, long long r0, int rows, int n0, int N,
+                                              const typename mm_type<TY>::t* bias, const typename mm_type<TY>::t* res,
+                                              long long ldr, void* slope, typename mm_type<TY>::t* C) {
+    constexpr int FM = tile_t::ROWS, FN = tile_t::COLS;
+    const mh_f4 zero = {0.f, 0.f, 0.f, 0.f};
+    mh_f4 bv[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + tile_t::column(j), c = WHOLE ? 4 : N - n;
+        bv[j] = bias && c > 0 ? mm_get4<TY>(bias + n, c) : zero;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = tile_t::row(i);
+        if (m >= rows) continue;
+        mh_f4 rv[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = n0 + tile_t::column(j), c = WHOLE ? 4 : N - n;
+            rv[j] = res && c > 0 ? mm_get4<TY>(res + (r0 + m) * ldr + n, c) : zero;
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            const int n = n0 + tile_t::column(j), c = WHOLE ? 4 : N - n;
+            if (c > 0) mm_finish<TY, ACT>(t.value(i, j) + bv[j], (r0 + m) * N + n, c, rv[j], slope, C);
+        }
+    }
 }
 
 // Forward and input gradient: R rows of A [R, K] in groups, B the group's weights ([N, K], or [K, N] where BS), the
@@ -713,12 +745,11 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
     const T* B = static_cast<const T*>(B_) + (long long)e * N * K + (BS ? (long long)n0 : (long long)n0 * K);
     t.run(lds, A, lda, rows, B, BS ? N : K, min(N - n0, tile_t::BN), 0, K);
     const T* bias = bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr;
-    t.each([&](int m, int n, mh_f4 v) {
-        const int c = N - n0 - n;                       // columns that exist from here on
-        if (m < rows && c > 0)
-            mm_finish<TY, ACT>(v, (long long)r0 + m, n0 + n, c, bias, static_cast<const T*>(res_), ldr, slope_,
-                               static_cast<T*>(C_), N);
-    });
+    const T* res = static_cast<const T*>(res_);
+    if (n0 + tile_t::BN <= N)
+        mm_store_tile<TY, ACT, true>(t, r0, rows, n0, N, bias, res, ldr, slope_, static_cast<T*>(C_));
+    else
+        mm_store_tile<TY, ACT, false>(t, r0, rows, n0, N, bias, res, ldr, slope_, static_cast<T*>(C_));
 }
 
 // The forward for few rows: a workgroup takes 16 TM rows of a group and 16 columns, its WAVES waves share the contraction and
@@ -813,11 +844,13 @@ __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void
         mh_f4 v = sums[0][t][lane];
 #pragma unroll
         for (int k = 1; k < WAVES; ++k) v += sums[k][t][lane];
-        const int c = cols - 4 * q;
-        if (16 * t + i < rows && c > 0)
-            mm_finish<TY, ACT>(v, (long long)r0 + 16 * t + i, n0 + 4 * q, c,
-                               bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr,
-                               static_cast<const T*>(res_), ldr, slope_, C, N);
+        const int c = cols - 4 * q, n = n0 + 4 * q;
+        const long long r = (long long)r0 + 16 * t + i;
+        if (16 * t + i < rows && c > 0) {
+            if (bias_) v += mm_get4<TY>(static_cast<const T*>(bias_) + (long long)e * N + n, c);
+            const mh_f4 res = res_ ? mm_get4<TY>(static_cast<const T*>(res_) + r * ldr + n, c) : mh_f4{0.f, 0.f, 0.f, 0.f};
+            mm_finish<TY, ACT>(v, r * N + n, c, res, slope_, C);
+        }
     }
 }
 
@@ -843,13 +876,16 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
     t.run(lds, static_cast<const T*>(A_) + (long long)r0 * lda + m0, lda, min(M - m0, tile_t::BM),
           static_cast<const T*>(B_) + (long long)r0 * ldb + n0, ldb, min(N - n0, tile_t::BN), 0, r1 - r0);
     const long long at = (long long)(L ? (int)blockIdx.y : e) * M * N;
-    t.each([&](int m, int n, mh_f4 v) {
-        const int c = N - n0 - n;
-        if (m0 + m >= M || c <= 0) return;
-        const long long i = at + (long long)(m0 + m) * N + n0 + n;
-        if (L) mm_put4<MM_F32>(part + i, v, c);
-        else mm_put4<TY>(static_cast<T*>(C_) + i, v, c);
-    });
+#pragma unroll
+    for (int i = 0; i < tile_t::ROWS; ++i)
+#pragma unroll
+        for (int j = 0; j < tile_t::COLS; ++j) {
+            const int m = m0 + tile_t::row(i), n = n0 + tile_t::column(j), c = N - n;
+            if (m >= M || c <= 0) continue;
+            const long long k = at + (long long)m * N + n;
+            if (L) mm_put4<MM_F32>(part + k, t.value(i, j), c);
+            else mm_put4<TY>(static_cast<T*>(C_) + k, t.value(i, j), c);
+        }
 }
 
 // out[e, i] = sum of part[s, i] over the group's slots in a fixed order: what ends a sum that was split over rows.  2^lg waves
@@ -893,7 +929,8 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
 
 // p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1) and the sums of its columns in float32, before
 // rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows, rounded into db (both NULL: none).
-// A workgroup takes a slot and 256 columns, 64 threads of four columns each by four rows at a time.
+// A workgroup takes a slot and 256 columns, 64 threads of four columns each by four rows at a time.  Bound by its bytes; the
+// slope is read for the last time, past the caches: 69 us at 16,384 x 4,096 bfloat16, 5.8 TB/s (81 as an ordinary read).
 template <int TY>
 __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, void* db, const int* off,
                                               long long ldg, int R, int N, int E, int L) {
@@ -921,9 +958,11 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
             const long long at = (long long)r * N + n;
             if (slope_) {
                 if constexpr (TY == MM_F32) {
-                    v = times(v, *reinterpret_cast<const mh_u4x*>(static_cast<const float*>(slope_) + at));
+                    v = times(v, __builtin_nontemporal_load(
+                                     reinterpret_cast<const mh_u4x*>(static_cast<const float*>(slope_) + at)));
                 } else {
-                    const mh_u2 d = *reinterpret_cast<const mh_u2x*>(static_cast<const unsigned short*>(slope_) + at);
+                    const mh_u2 d = __builtin_nontemporal_load(
+                        reinterpret_cast<const mh_u2x*>(static_cast<const unsigned short*>(slope_) + at));
                     v = times(v, mh_u4{d.x, d.y, 0u, 0u});
                 }
             }

@@ -142,7 +142,7 @@ _SIGS = {
     'mh_combine': (ctypes.c_int, [_P] * 5 + [_L, _P] + [_I] * 4 + [_P]),
     'mh_combine_bwd': (ctypes.c_int, [_P, _P, _L] + [_P] * 6 + [_I] * 5 + [_P]),
     'mh_norm_fwd': (ctypes.c_int, [_P] * 10 + [_I, _I, ctypes.c_float, _P]),
-    'mh_norm_bwd': (ctypes.c_int, [_P] * 16 + [_I] * 4 + [_P]),
+    'mh_norm_bwd': (ctypes.c_int, [_P] * 16 + [_I] * 3 + [_P]),
 }
 EXPORTS = tuple(_SIGS)
 

@@ -18,21 +18,32 @@ MAX_CHANNELS = 8192
 
 
 def shape(C, dtype):
-    """(threads per row, vectors of 16 bytes per thread): the fewest of a wave or a workgroup of 256, 512 or 1024 threads that
-    hold the row in at most two vectors each (the backward keeps about ten rows in registers; four vectors spilled)."""
+    """(threads per row, vectors of 16 bytes per thread): the fewest of a wave (four rows a workgroup) or a workgroup of 128
+    to 1024 threads that hold the row in one vector each, two for the longest rows of float32: the backward then keeps its
+    rows and the next one's loads in registers (two vectors of 16-bit values a thread take 300)."""
     vectors = -(-C * dtype.itemsize // 16)
-    tpr = next(t for t in (64, 256, 512, 1024) if vectors <= 2 * t)
+    tpr = next((t for t in (64, 128, 256, 512) if vectors <= t), 1024)
     return tpr, -(-vectors // tpr)
 
 
-def rows_per_block(tpr):
-    return 4 if tpr == 64 else 1
+def _launch(tpr):
+    """(threads, rows) of a workgroup."""
+    return (256, 4) if tpr == 64 else (tpr, 1)
+
+
+def _backward_blocks(T, tpr):
+    """Workgroups of the backward: two per compute unit for each 256 threads' worth of a row (measured at 32,768 rows, us, for
+    1 / 2 / 4 per compute unit: 2,048 channels bfloat16 264 / 212 / 231, 1,024 of them 158 / 128 / 176, 512 91 / 61 / 70, 1,024
+    of float32 224 / 215 / 226), one for each compute unit at least (4,096 of float32, 8,000 rows, 128 / 256 workgroups:
+    233 / 163), and no more than leave each row group four rows, whose sums cost as much as reading two."""
+    threads, rows = _launch(tpr)
+    return max(1, min(-(-T // (4 * rows)), max(CUS, 2 * CUS * 256 // threads)))
 
 
 def source(dtype, tpr, nv, layer, branch, gate):
     b = lambda v: 'true' if v else 'false'  # noqa: E731
     args = f'{TYPES[dtype]}, {tpr}, {nv}, {b(layer)}, {b(branch)}, {gate}'
-    sig = f'extern "C" __global__ __launch_bounds__({max(256, tpr)}) void '
+    sig = f'extern "C" __global__ __launch_bounds__({_launch(tpr)[0]}) void '
     return _native.layer_header('matmul', 'norms') + '\n'.join([
         sig + 'nm_fwd(const void* x, const void* y, const void* gate, const void* scale, const void* wp, const void* wn, '
         'void* h, void* n, float* stats, int T, int C, float eps) {',
@@ -51,8 +62,8 @@ def module(device, dtype, tpr, nv, layer, branch, gate):
     if m is None:
         code = _native.compile_source(source(dtype, tpr, nv, layer, branch, gate))
         with torch.cuda.device(device):
-            m = _native.Module(code, {_native.MH_NORM_FWD: ('nm_fwd', max(256, tpr), rows_per_block(tpr)),
-                                      _native.MH_NORM_BWD: ('nm_bwd', max(256, tpr), rows_per_block(tpr))})
+            m = _native.Module(code, {_native.MH_NORM_FWD: ('nm_fwd', *_launch(tpr)),
+                                      _native.MH_NORM_BWD: ('nm_bwd', *_launch(tpr))})
         _MODULES[key] = m
     return m
 
@@ -98,12 +109,11 @@ class _BlockNormFn(torch.autograd.Function):
         dx, dy, dgate = (torch.empty_like(t) if w else None for t, w in zip((x, y, gate), need[:3]))
         dsum = torch.empty((3, C), device=dev, dtype=dt) if any(need[3:6]) else None
         tpr, nv = shape(C, dt)
-        per = rows_per_block(tpr)
-        blocks = max(1, min(-(-T // per), 4 * CUS))
-        part = None if dsum is None else torch.empty((blocks * per, 3, C), device=dev, dtype=torch.float32)
+        blocks = _backward_blocks(T, tpr)
+        part = None if dsum is None else torch.empty((blocks, 3, C), device=dev, dtype=torch.float32)
         _native.launch('nm_bwd', lib.mh_norm_bwd, module(dev, dt, tpr, nv, layer, y is not None, gmode).handle,
                        mm_module(dev, dt, 'sum').handle, P(gh), P(gn), P(x), P(y), P(gate), P(scale), P(wp), P(wn), P(stats),
-                       P(dx), P(dy), P(dgate), P(part), P(dsum), T, C, blocks, blocks * per, _native.stream_of(x))
+                       P(dx), P(dy), P(dgate), P(part), P(dsum), T, C, blocks, _native.stream_of(x))
         return (dx, dy, dgate, *(dsum[i] if w else None for i, w in enumerate(need[3:6])), None, None, None)
 
 

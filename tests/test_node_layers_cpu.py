@@ -55,7 +55,7 @@ def test_c_entry_points_refuse_bad_arguments():
         (lambda: lib.mh_combine_bwd(None, p, 8, None, p, p, p, p, p, 2, 1, 8, 1, 1, None), 'NULL'),
         (lambda: lib.mh_norm_fwd(None, p, p, None, None, None, None, None, p, None, 2, 8, 1e-6, None), 'NULL'),
         (lambda: lib.mh_norm_fwd(None, p, None, None, None, None, None, None, p, None, 2, 8, 1e-6, None), 'null module'),
-        (lambda: lib.mh_norm_bwd(None, None, p, p, p, None, None, None, None, None, None, p, None, None, p, p, 2, 8, 1, 4, None),
+        (lambda: lib.mh_norm_bwd(None, None, p, p, p, None, None, None, None, None, None, p, None, None, p, p, 2, 8, 1, None),
          'NULL'),
     ]
     for i, (call, text) in enumerate(cases):
