@@ -1304,6 +1304,61 @@ int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g,
     return 0;
 }
 
+int mh_hv_rows(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, int32_t R, int32_t K, void* stream) {
+    if (R < 0 || K < 1 || K > 0x7fffffff - 32) return fail(-1, "mh_hv_rows: bad sizes");
+    if (R == 0) return 0;
+    if (!x || !y || !peak) return fail(-1, "mh_hv_rows: NULL operand");
+    if (ldx < K) return fail(-1, "mh_hv_rows: rows overlap (ld below the row's length)");
+    void* args[] = {&x, &y, &peak, &ldx, &R, &K};
+    return launch_blocks(m, MH_HV_ROWS, (static_cast<int64_t>(R) + 3) / 4, args, stream, "mh_hv_rows");
+}
+
+int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, const int32_t* offsets, int32_t R,
+                  int32_t C, int32_t E, int32_t G, int32_t L, int32_t slots, void* stream) {
+    if (R < 0 || C < 1 || E < 1 || G < 0 || L < 1 || slots < 0 || R > 0x7fffffff - L || C > 0x7fffffff - 256 ||
+        (!offsets && static_cast<int64_t>(E) * G != R))
+        return fail(-1, "mh_hv_columns: bad sizes");
+    if (R == 0) return 0;
+    if (!x || !y || !peak) return fail(-1, "mh_hv_columns: NULL operand");
+    if (ldx < C) return fail(-1, "mh_hv_columns: rows overlap (ld below the row's length)");
+    uint32_t* mark = peak + static_cast<int64_t>(E) * C;
+    const int64_t ny = (static_cast<int64_t>(C) + 255) / 256;
+    void* first[] = {&x, &peak, &mark, &offsets, &ldx, &R, &C, &E, &G, &L};
+    if (int rc = launch_blocks(m, MH_HV_PEAKS, slots, first, stream, "mh_hv_columns", ny)) return rc;
+    void* second[] = {&x, &y, &peak, &offsets, &ldx, &R, &C, &E, &G, &L};
+    return launch_blocks(m, MH_HV_COLUMNS, slots, second, stream, "mh_hv_columns", ny);
+}
+
+int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const float* bias, const float* res, int64_t ldr,
+             float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
+             int32_t N, int32_t K, int32_t E, void* stream) {
+    if (R < 0 || N < 0 || K < 1 || K > 0x3fffffff || E < 1 || (E > 1 && !offsets)) return fail(-1, "mh_hv_mm: bad sizes");
+    if (R == 0 || N == 0) return 0;
+    if (!A || !B || !C || !pa || !pb) return fail(-1, "mh_hv_mm: NULL operand");
+    if (res && ldr < N) return fail(-1, "mh_hv_mm: rows overlap (ld below the row's length)");
+    if (!m || !m->k[MH_HV_MM].fn) return fail(-1, "mh_hv_mm: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_HV_MM];
+    if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_hv_mm: too many rows");
+    const int64_t tiles = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &pa, &pb, &mb, &ldr, &R, &N, &K, &E};
+    return launch_blocks(m, MH_HV_MM, tiles, args, stream, "mh_hv_mm");
+}
+
+int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, float* part, const int32_t* offsets,
+                const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
+                int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
+    if (R < 1 || R > 0x3fffffff || M < 1 || N < 1 || E < 1 || (E > 1 && !offsets) || L < 0 || (L && slots < 1) ||
+        R > 0x7fffffff - L)
+        return fail(-1, "mh_hv_outer: bad sizes");
+    if (!A || !B || !pa || !ma || !pb || !mb || (L ? !part : !C)) return fail(-1, "mh_hv_outer: NULL operand");
+    if (!m || !m->k[MH_HV_OUTER].fn) return fail(-1, "mh_hv_outer: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_HV_OUTER];
+    const int64_t tiles = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
+                          ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &R, &M, &N, &E, &L};
+    return launch_blocks(m, MH_HV_OUTER, tiles, args, stream, "mh_hv_outer", L ? slots : E);
+}
+
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
                     int32_t* offsets, int32_t* rows, int32_t* place, void* stream) {
     if (A < 0 || E < 1 || E > 1024 || blocks < 1 || A > 0x7fffffff - 1024) return fail(-1, "mh_expert_order: bad sizes");

@@ -517,7 +517,7 @@ __device__ __forceinline__ void mm_read_turned(const unsigned (&at)[2], mh_u2 (&
         : "memory");
 }
 
-template <bool STRIDED, int ROWS, int BK, int THREADS>
+template <bool STRIDED, int ROWS, int BK, int THREADS, bool HALVES>
 struct mm_mover {
     static constexpr int OPR = BK / 8, ITEMS = ROWS * OPR / THREADS;
     static_assert(ROWS * OPR % THREADS == 0, "a tile is a whole number of loads per thread");
@@ -530,7 +530,7 @@ struct mm_mover {
             const int s = threadIdx.x + j * THREADS;
             if constexpr (STRIDED) {
                 const int k = s / (ROWS / 8), p = s % (ROWS / 8);
-                const int c = ((p >> 1) ^ (mm_turn(k) & (ROWS / 16 - 1))) * 16 + (p & 1) * 8;
+                const int c = ((p >> 1) ^ (mm_turn(HALVES ? k >> 1 : k) & (ROWS / 16 - 1))) * 16 + (p & 1) * 8;
                 at[j] = k;
                 off[j] = (unsigned)(k * ld + min(c, rows - 8)) * 2;
             } else {
@@ -551,7 +551,7 @@ struct mm_mover {
     }
 };
 
-template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK>
+template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK, bool HALVES = false>
 struct mm_fast_tile {
     typedef unsigned short T;
     static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, ROWS = FM, COLS = FN;
@@ -565,7 +565,7 @@ struct mm_fast_tile {
     __device__ __forceinline__ static void fragments(mh_u4 (&f)[N], mh_u4* tile, int row0, int ks) {
         const int lane = threadIdx.x & 63, i = lane & 15, q = lane >> 4;
         if constexpr (STRIDED) {
-            const int k = 32 * ks + 8 * q + (i >> 2);
+            const int k = (HALVES ? 0 : 32 * ks) + 8 * q + (i >> 2), r = HALVES ? 2 * k + ks : k;
             constexpr int G = N < 4 ? N : 4;
 #pragma unroll
             for (int h = 0; h < N; h += G) {
@@ -573,8 +573,8 @@ struct mm_fast_tile {
                 mh_u2 lo[G], hi[G];
 #pragma unroll
                 for (int c = 0; c < G; ++c)
-                    at[c] = mm_lds_at(tile) + 2 * (k * ROWS + ((row0 / 16 + h + c) ^ (mm_turn(k) & (ROWS / 16 - 1))) * 16 + (i & 3) * 4);
-                mm_read_turned<8 * ROWS>(at, lo, hi);
+                    at[c] = mm_lds_at(tile) + 2 * (r * ROWS + ((row0 / 16 + h + c) ^ (mm_turn(k) & (ROWS / 16 - 1))) * 16 + (i & 3) * 4);
+                mm_read_turned<(HALVES ? 16 : 8) * ROWS>(at, lo, hi);
 #pragma unroll
                 for (int c = 0; c < G; ++c) f[h + c] = mh_u4{lo[c].x, lo[c].y, hi[c].x, hi[c].y};
             }
@@ -584,8 +584,30 @@ struct mm_fast_tile {
         }
     }
 
+    template <bool TOP>
     __device__ __forceinline__ void products(mh_u4* a, mh_u4* b) {
         const int wave = threadIdx.x >> 6, ra = (wave / WN) * 16 * FM, rb = (wave % WN) * 16 * FN;
+        if constexpr (HALVES) {
+            // upper times upper, upper times lower, lower times upper (TOP: the first alone)
+            mh_u4 fa[FM], fb[2][FN];
+            fragments<BS, BN, FN>(fb[0], b, rb, 0);
+            if constexpr (!TOP) fragments<BS, BN, FN>(fb[1], b, rb, 1);
+            fragments<AS, BM, FM>(fa, a, ra, 0);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) {
+                    acc[i][j] = mm_mfma<TY>(fb[0][j], fa[i], acc[i][j]);
+                    if constexpr (!TOP) acc[i][j] = mm_mfma<TY>(fb[1][j], fa[i], acc[i][j]);
+                }
+            if constexpr (TOP) return;
+            fragments<AS, BM, FM>(fa, a, ra, 1);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = mm_mfma<TY>(fb[0][j], fa[i], acc[i][j]);
+            return;
+        }
 #pragma unroll
         for (int ks = 0; ks < BK / 32; ++ks) {
             mh_u4 fa[FM], fb[FN];
@@ -600,20 +622,25 @@ struct mm_fast_tile {
 
     // The loads of the next tile (where `left` > 0) and this one's products.  The four places are distinct: without that the
     // compiler waits for the loads before it reads the tile that is there.
-    __device__ __forceinline__ void step(const mm_mover<AS, BM, BK, THREADS>& ma, const mm_mover<BS, BN, BK, THREADS>& mb, const T* A,
-                                         const T* B, int left, mh_u4* __restrict__ a, mh_u4* __restrict__ b,
-                                         mh_u4* __restrict__ an, mh_u4* __restrict__ bn) {
+    template <bool TOP>
+    __device__ __forceinline__ void step(const mm_mover<AS, BM, BK, THREADS, HALVES>& ma,
+                                         const mm_mover<BS, BN, BK, THREADS, HALVES>& mb, const T* A, const T* B, int left,
+                                         int bleft, mh_u4* __restrict__ a, mh_u4* __restrict__ b, mh_u4* __restrict__ an,
+                                         mh_u4* __restrict__ bn) {
         if (left > 0) {
             ma.issue(A, left, an);
-            mb.issue(B, left, bn);
+            mb.issue(B, bleft, bn);
         }
-        products(a, b);
+        products<TOP>(a, b);
     }
 
+    // `bend`: where B's k end, if before A's (whose padding is zeros); 0: with A's
+    template <bool TOP = false>
     __device__ __forceinline__ void run(mh_u4* lds, const T* A, long long lda, int arows, const T* B, long long ldb, int brows,
-                                        int kbeg, int kend) {
-        mm_mover<AS, BM, BK, THREADS> ma;
-        mm_mover<BS, BN, BK, THREADS> mb;
+                                        int kbeg, int kend, int bend = 0) {
+        if (!bend) bend = kend;
+        mm_mover<AS, BM, BK, THREADS, HALVES> ma;
+        mm_mover<BS, BN, BK, THREADS, HALVES> mb;
         ma.init(lda, arows);
         mb.init(ldb, brows);
         const long long sa = AS ? lda : 1, sb = BS ? ldb : 1;
@@ -624,12 +651,12 @@ struct mm_fast_tile {
         if (kbeg >= kend) return;                       // uniform over the workgroup
         mh_u4 *a0 = lds, *a1 = lds + TA, *b0 = lds + 2 * TA, *b1 = lds + 2 * TA + TB;
         ma.issue(A + kbeg * sa, kend - kbeg, a0);
-        mb.issue(B + kbeg * sb, kend - kbeg, b0);
+        mb.issue(B + kbeg * sb, bend - kbeg, b0);
         for (int k = kbeg; k < kend; k += BK) {
             // the tile of this step is in LDS, and every wave is done with the other buffer
             __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
             __syncthreads();
-            step(ma, mb, A + (k + BK) * sa, B + (k + BK) * sb, kend - k - BK, a0, b0, a1, b1);
+            step<TOP>(ma, mb, A + (k + BK) * sa, B + (k + BK) * sb, kend - k - BK, bend - k - BK, a0, b0, a1, b1);
             mh_u4* t = a0;
             a0 = a1;
             a1 = t;

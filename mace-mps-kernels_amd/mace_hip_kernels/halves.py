@@ -1,0 +1,124 @@
+"""
+Large float32 products of ``dense`` and ``expert_dense`` as three float16 products (``csrc/mh_halves.h``): the operands are
+first written as two float16 halves each, scaled by a power of two per row or column, and the matrix cores then do three
+products where the direct kernels' bf16 parts take six.  Worth its extra passes where the products are long enough;
+``matmul`` decides by sizes.
+"""
+import functools
+
+import torch
+
+from . import _native
+
+# waves (rows x columns), 16 x 16 fragments per wave (rows x columns): 128 x 128 a workgroup, two of them on a compute unit
+# (256 x 256 with eight waves measured 167 us where these take 117, at 20,000 x 1,024 x 1,024)
+TILE = 2, 2, 4, 4
+SIDE = 128
+
+
+def pays(rows, n, K, groups, mode):
+    """Whether a product of [rows, K] and [groups, n, K] is faster by halves: by its operations at the rate of either path,
+    the bytes of the halves (read and written once by rows, read twice by columns), the launches, and a margin of three tenths.  Measured (us,
+    direct / halves): 20,000 x 1,024 x 1,024 forward 312 / 163, dx 335 / 162, dw 403 / 247; 8,192 x 512 x 2,048 119 / 72, 138 /
+    97, 176 / 130; 2,533 x 512 x 512 forward 10 / 29; 20,000 x 128 x 512 28 / 39, 32 / 46, 40 / 78."""
+    flops = 2.0 * rows * n * K
+    moved = {'fwd': 8 * (rows * K + groups * n * K), 'dx': 8 * rows * n + 12 * groups * n * K,
+             'dw': 12 * rows * (n + K)}[mode]
+    direct = flops / (104e12 if mode == 'dw' else 135e12)
+    return 1.3 * (flops / 370e12 + moved / 4.5e12 + (15e-6 if mode == 'dw' else 8e-6)) < direct
+
+
+def source(mode, act=0):
+    """HIP source of one module: 'split' (the halves of rows and columns), or 'fwd', 'dx', 'dw'."""
+    L = [_native.layer_header('matmul', 'halves')]
+    if mode == 'split':
+        return L[0]
+    b = lambda v: 'true' if v else 'false'  # noqa: E731
+    L += [f'typedef mm_fast_tile<MM_F16, {b(mode == "dw")}, {b(mode != "fwd")}, {", ".join(map(str, TILE))}, 64, true> '
+          'tile_t;',
+          f'extern "C" __global__ __launch_bounds__(tile_t::THREADS) void hv_{mode}(const unsigned short* A, '
+          'const unsigned short* B, float* C, ']
+    if mode == 'dw':
+        L += ['float* part, const int* off, const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb, '
+              'int R, int M, int N, int E, int L) {',
+              '  hv_outer_body<tile_t>(A, B, C, part, off, pa, ma, pb, mb, R, M, N, E, L);', '}']
+    else:
+        L += ['const float* bias, const float* res, float* slope, const int* off, const unsigned* pa, const unsigned* pb, '
+              'const unsigned* mb, long long ldr, int R, int N, int K, int E) {',
+              f'  hv_rows_body<{b(mode == "dx")}, {act}, tile_t>(A, B, C, bias, res, slope, off, pa, pb, mb, ldr, R, N, K, E);',
+              '}']
+    return '\n'.join(L) + '\n'
+
+
+@functools.lru_cache(maxsize=None)
+def module(device, mode, act=0):
+    """The loaded module (compiled on first use, kept per device)."""
+    code = _native.compile_source(source(mode, act))
+    with torch.cuda.device(device):
+        if mode == 'split':
+            return _native.Module(code, {_native.MH_HV_ROWS: ('hv_rows', 256, 1), _native.MH_HV_PEAKS: ('hv_peaks', 256, 1),
+                                         _native.MH_HV_COLUMNS: ('hv_columns', 256, 1)})
+        kind = _native.MH_HV_OUTER if mode == 'dw' else _native.MH_HV_MM
+        return _native.Module(code, {kind: (f'hv_{mode}', 64 * TILE[0] * TILE[1], SIDE, SIDE)})
+
+
+def _up(n, to):
+    return -(-n // to) * to
+
+
+def split_rows(x, ld, R, K):
+    """(halves, peaks) of R rows of K values."""
+    y = torch.empty(R * 2 * _up(K, 32), device=x.device, dtype=torch.uint16)
+    peak = torch.empty(R, device=x.device, dtype=torch.int32)
+    P = _native.ptr
+    _native.launch('hv_rows', _native.load().mh_hv_rows, module(x.device, 'split').handle, P(x), ld, P(y), P(peak), R, K,
+                   _native.stream_of(x))
+    return y, peak
+
+
+def split_columns(x, ld, R, C, groups, offsets=None):
+    """(halves, peaks and marks [2, groups, C]) of the columns of R rows, scaled per group of rows: by offsets, else equal
+    groups."""
+    y = torch.empty(R * 2 * _up(C, 8), device=x.device, dtype=torch.uint16)
+    peak = torch.zeros(2, groups, C, device=x.device, dtype=torch.int32)
+    G = R // groups if offsets is None else 0
+    # pieces of rows for about eight workgroups per compute unit
+    L = min(256, max(16, _up(-(-R * -(-C // 256) // 2048), 4)))
+    slots = groups * -(-G // L) if offsets is None else -(-R // L) + groups
+    P = _native.ptr
+    _native.launch('hv_columns', _native.load().mh_hv_columns, module(x.device, 'split').handle, P(x), ld, P(y), P(peak),
+                   P(offsets), R, C, groups, G, L, slots, _native.stream_of(x))
+    return y, peak
+
+
+def product(x, ld, weight, bias, res, ldr, act, slope, offsets, groups, out):
+    """out [R, n] = act(x weight^T + bias) + res (slope: act' there where given)."""
+    R, K = x.shape
+    n = out.shape[1]
+    xh, xp = split_rows(x, ld, R, K)
+    wh, wp = split_rows(weight, K, groups * n, K)
+    P = _native.ptr
+    _native.launch('hv_fwd', _native.load().mh_hv_mm, module(x.device, 'fwd', act).handle, P(xh), P(wh), P(out), P(bias),
+                   P(res), ldr, P(slope), P(offsets), P(xp), P(wp), None, R, n, K, groups, _native.stream_of(x))
+
+
+def input_gradient(p, ldp, weight, offsets, groups, out):
+    """out [R, K] = p weight per group, p [R, N], weight [groups, N, K]."""
+    R, N = p.shape
+    K = out.shape[1]
+    ph, pp = split_rows(p, ldp, R, N)
+    wh, wp = split_columns(weight, K, groups * N, K, groups)
+    P = _native.ptr
+    _native.launch('hv_dx', _native.load().mh_hv_mm, module(p.device, 'dx').handle, P(ph), P(wh), P(out), None, None, 0,
+                   None, P(offsets), P(pp), P(wp[0]), P(wp[1]), R, K, N, groups, _native.stream_of(p))
+
+
+def weight_gradient(p, ldp, x, ldx, offsets, groups, out, part, L, slots):
+    """out [groups, N, K] (or its parts, where L) = p^T x per group, p [R, N], x [R, K]."""
+    R, N = p.shape
+    K = x.shape[1]
+    ph, pp = split_columns(p, ldp, R, N, groups, offsets)
+    xh, xp = split_columns(x, ldx, R, K, groups, offsets)
+    P = _native.ptr
+    _native.launch('hv_dw', _native.load().mh_hv_outer, module(p.device, 'dw').handle, P(ph), P(xh), P(out), P(part),
+                   P(offsets), P(pp[0]), P(pp[1]), P(xp[0]), P(xp[1]), R, N, K, groups, L, slots, _native.stream_of(p))

@@ -9,15 +9,15 @@ bfloat16 and float16, for any number of rows from none on and any widths.
 
 A drop-in of ``patch_model`` holds its weights as constants; these are what a model trains next to it.  The kernels are in
 ``csrc/mh_matmul.h``, one hipRTC module per type, product and tile.  A float32 product runs on the bf16 matrix cores at
-float32 accuracy (operands split into three bf16 parts, six partial products); 16-bit operands run as they are; every sum
-is float32 and rounded once.  The backward keeps act'(a) of the forward, not a itself.  Sums over rows that are split over
+float32 accuracy (operands split into three bf16 parts, six partial products; large ones as three products of float16
+halves, ``halves``); 16-bit operands run as they are; every sum is float32 and rounded once.  The backward keeps act'(a) of the forward, not a itself.  Sums over rows that are split over
 workgroups are added in a fixed order, so results are bitwise repeatable.  The reference has no such layers.
 """
 import functools
 
 import torch
 
-from . import _native
+from . import _native, halves
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}
@@ -160,7 +160,9 @@ def _pieces(R, groups, per, tiles, step):
 # What a call's sizes lead to, kept by the sizes: modules are looked up and shapes chosen once per size, not per call.
 @functools.lru_cache(maxsize=4096)
 def _rows_plan(device, dtype, mode, R, n, K, groups, act, aligned):
-    """The module of a product over rows."""
+    """The module of a product over rows; None: by halves."""
+    if dtype == torch.float32 and mode == 'fwd' and halves.pays(R, n, K, groups, mode):
+        return None
     fast = dtype.itemsize == 2 and aligned and K % 8 == 0 and (mode == 'fwd' or n % 8 == 0)
     tile = (_few_tile(R, groups) if mode == 'fwd' else None) or _choose_tile(R, n, dtype, groups, fast)
     return module(device, dtype, mode, tile, act)
@@ -168,7 +170,11 @@ def _rows_plan(device, dtype, mode, R, n, K, groups, act, aligned):
 
 @functools.lru_cache(maxsize=4096)
 def _bwd_plan(device, dtype, R, N, K, groups, grouped, g_aligned, w_aligned, x_aligned, want_x, want_w, want_b):
-    """(modules of the sums, of dx and of dW; rows per piece and pieces of db; of dW; floats of scratch)."""
+    """(modules of the sums, of dx and of dW; rows per piece and pieces of db; of dW; floats of scratch; whether dx and dW go
+    by halves)."""
+    hx, hw = (want and dtype == torch.float32 and R > 0 and N > 0 and K > 0 and halves.pays(R, N, K, groups, mode)
+              for want, mode in ((want_x, 'dx'), (want_w, 'dw')))
+    want_x = want_x and not hx
     rows = _rows_plan(device, dtype, 'dx', R, K, N, groups, 0, g_aligned and w_aligned) if want_x and R and K else None
     # db: pieces of rows for about eight workgroups per compute unit (two / four / eight / sixteen: 100 / 100 / 69 / 73 us at
     # 16,384 x 4,096 bfloat16, 84 / 55 / 41 / 48 at 2,048 in eight groups); few rows are one piece that needs no second sum
@@ -177,13 +183,16 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, g_aligned, w_aligned, x_a
     slots = max(1, -(-R // Ls)) + (groups if grouped else 0)
     scratch = slots * N if want_b and (grouped or slots > 1) else 0
     outer, Lo, slots_o = None, 0, groups
-    if want_w and N and K:
+    if hw:
+        Lo, slots_o = _pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE), 64)
+        scratch = max(scratch, slots_o * N * K if Lo else 0)
+    elif want_w and N and K:
         tile = _outer_tile(N, K, dtype, dtype.itemsize == 2 and g_aligned and x_aligned and N % 8 == 0 and K % 8 == 0)
         outer = module(device, dtype, 'dw', tile)
         bm, bn = tile_shape(tile, dtype)
         Lo, slots_o = _pieces(R, groups, grouped, -(-N // bm) * -(-K // bn), 64)
         scratch = max(scratch, slots_o * N * K if Lo else 0)
-    return module(device, dtype, 'sum'), rows, outer, Ls, slots, Lo, slots_o, scratch
+    return module(device, dtype, 'sum'), rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw
 
 
 def _product(x, ld, weight, bias, res, act, offsets, groups, keep):
@@ -197,6 +206,9 @@ def _product(x, ld, weight, bias, res, act, offsets, groups, keep):
         m = _rows_plan(dev, dt, 'fwd', R, n, K, groups, act, _aligned(x, ld) and weight.data_ptr() % 16 == 0)
         P = _native.ptr
         r, ldr = (None, 0) if res is None else rows_of(res, n)
+        if m is None:
+            halves.product(x, ld, weight, bias, r, ldr, act, slope, offsets, groups, out)
+            return out, slope
         _native.launch('mm_fwd', _native.load().mh_mm_rows, m.handle, P(x), ld, P(weight), P(out), P(bias), P(r), ldr,
                        P(slope), P(offsets), R, n, K, groups, _native.stream_of(x))
     return out, slope
@@ -213,7 +225,7 @@ def _backward(g, ldg, slope, weight, x, ldx, offsets, groups, need):
     else:
         want_p = slope is not None
     g_aligned = want_p or _aligned(g, ldg)
-    sums, rows, outer, Ls, slots, Lo, slots_o, scratch = _bwd_plan(
+    sums, rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw = _bwd_plan(
         dev, dt, R, N, K, groups, offsets is not None, N % 8 == 0 if want_p else g_aligned,
         weight is not None and weight.data_ptr() % 16 == 0, x is not None and _aligned(x, ldx), want_x, want_w, want_b)
     p = torch.empty((R, N), device=dev, dtype=dt) if want_p else None
@@ -221,10 +233,21 @@ def _backward(g, ldg, slope, weight, x, ldx, offsets, groups, need):
     dw = torch.empty((groups, N, K), device=dev, dtype=dt) if want_w else None
     db = torch.empty((groups, N), device=dev, dtype=dt) if want_b else None
     part = torch.empty(scratch, device=dev, dtype=torch.float32) if scratch else None
-    _native.launch('mm_bwd', _native.load().mh_mm_bwd, sums.handle, None if rows is None else rows.handle,
+    if want_p or want_b or rows is not None or outer is not None:
+        _native.launch('mm_bwd', _native.load().mh_mm_bwd, sums.handle, None if rows is None else rows.handle,
                    None if outer is None else outer.handle, P(g), ldg, P(slope) if want_p else None, P(weight), P(x), ldx,
                    P(offsets), P(p), P(dx) if rows is not None else None, P(dw) if outer is not None else None, P(db), P(part),
                    R, N, K, groups, Ls, slots, Lo, slots_o, _native.stream_of(g))
+    if hx or hw:
+        if want_p:
+            g, ldg = p, N
+        if hx:
+            halves.input_gradient(g, ldg, weight, offsets, groups, dx)
+        if hw:
+            halves.weight_gradient(g, ldg, x, ldx, offsets, groups, dw, part, Lo, slots_o)
+            if Lo:
+                _native.launch('mm_sum', _native.load().mh_mm_sum, sums.handle, P(part), P(dw), P(offsets), R, groups, Lo,
+                               N * K, _native.stream_of(g))
     return dx, dw, db
 
 

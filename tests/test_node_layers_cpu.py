@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import mace_hip_kernels as mhk
-from mace_hip_kernels import _native, experts, matmul, norms
+from mace_hip_kernels import _native, experts, halves, matmul, norms
 
 
 def test_host_tensors_and_other_types_are_refused():
@@ -46,6 +46,10 @@ def test_c_entry_points_refuse_bad_arguments():
         (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, p, None, 2, 4, 1, 1, 2, None), 'one slot'),
         (lambda: lib.mh_mm_bwd(None, None, None, p, 4, p, p, p, 4, None, None, p, p, p, p, 2, 4, 4, 1, 4, 1, 0, 1, None),
          'goes with slope'),
+        (lambda: lib.mh_hv_rows(None, p, 3, p, p, 2, 4, None), 'overlap'),
+        (lambda: lib.mh_hv_columns(None, p, 4, p, p, None, 6, 4, 4, 2, 4, 4, None), 'bad sizes'),
+        (lambda: lib.mh_hv_mm(None, p, p, p, None, None, 0, None, None, p, None, None, 2, 4, 4, 1, None), 'NULL'),
+        (lambda: lib.mh_hv_outer(None, p, p, p, None, None, p, p, p, p, 2, 4, 4, 1, 4, 1, None), 'NULL'),
         (lambda: lib.mh_expert_order(None, p, 0, 4, 1025, None, 1, p, p, p, None), 'bad sizes'),
         (lambda: lib.mh_expert_order(None, p, 0, 4, 3, None, 2, p, p, p, None), 'NULL'),
         (lambda: lib.mh_dispatch(None, p, 8, p, p, p, 2, 1, 8, 1, 7, None), 'bad sizes'),
@@ -89,5 +93,7 @@ def test_every_module_compiles_for_gfx950(dt):
     sources = [matmul.source(dt, 'sum'), experts.source(dt), experts.order_source()]
     sources += [matmul.source(dt, mode, tile) for mode in ('fwd', 'dx', 'dw') for tile in matmul.tiles(dt)]
     sources += [norms.source(dt, 64, 1, True, True, 0), norms.source(dt, 512, 2, False, True, 2)]
+    if dt == torch.float32:
+        sources += [halves.source(mode) for mode in ('split', 'fwd', 'dx', 'dw')]
     for src in sources:
         assert _native.compile_source(src)[:4] == b'\x7fELF'

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import mace_hip_kernels as mhk
-from mace_hip_kernels import matmul, norms
+from mace_hip_kernels import halves, matmul, norms
 
 pytestmark = pytest.mark.gpu
 
@@ -120,6 +120,95 @@ def test_dense_over_many_tiles_and_split_sums(T, K, N, dt):
     for name, t, u in zip(('dx', 'dw', 'db'), first, torch.autograd.grad(y, leaves, g.to(d))):
         near(name, t, *want[name])
         assert torch.equal(t, u), f'{name} differs between two passes'
+
+
+@pytest.fixture
+def by_halves(monkeypatch):
+    """Float32 products by halves whatever their size."""
+    monkeypatch.setattr(halves, 'pays', lambda *a: True)
+    matmul._rows_plan.cache_clear()
+    matmul._bwd_plan.cache_clear()
+    yield
+    monkeypatch.undo()
+    matmul._rows_plan.cache_clear()
+    matmul._bwd_plan.cache_clear()
+
+
+@pytest.mark.parametrize('T,K,N', DENSE + [(260, 328, 520), (2600, 40, 136)])
+def test_products_by_halves(T, K, N, by_halves):
+    d = dev()
+    rng = np.random.default_rng(T + K)
+    cuts = [T // 3, T // 3, T - T // 5]
+    off = torch.tensor([0] + cuts, dtype=torch.int32)
+    for act in (None, 'gelu'):
+        print(f'[case] halves T={T} K={K} N={N} {act}', flush=True)
+        x, w, b, g = rand(rng, T, K), rand(rng, 3, N, K, scale=K ** -0.5), rand(rng, 3, N), rand(rng, T, N)
+        res = rand(rng, T, N)
+        x[cuts[2]:], g[cuts[2]:] = 1e30, float('nan')              # rows of no group
+        one = dense_case(x[:cuts[2]], w[0], b[0], act, res[:cuts[2]], g[:cuts[2]], F32)
+        leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+        y = mhk.dense(leaves[0][:cuts[2]], leaves[1][0], leaves[2][0], act, res[:cuts[2]].to(d))
+        near('y', y, *one['y'])
+        grads = torch.autograd.grad(y, leaves, g[:cuts[2]].to(d))
+        for name, t in zip(('dx', 'dw', 'db'), (grads[0][:cuts[2]], grads[1][0], grads[2][0])):
+            near(name, t, *one[name])
+        y = mhk.expert_dense(*leaves[:2], off.to(d), leaves[2], act, res.to(d))
+        grads = torch.autograd.grad(y, leaves, g.to(d))
+        assert (y[cuts[2]:] == 0).all() and (grads[0][cuts[2]:] == 0).all()
+        for e, (i, j) in enumerate(zip([0] + cuts[:2], cuts)):
+            want = dense_case(x[i:j], w[e], b[e], act, res[i:j], g[i:j], F32)
+            for name, t in zip(('y', 'dx', 'dw', 'db'), (y[i:j], grads[0][i:j], grads[1][e], grads[2][e])):
+                near(f'{name} of {e}', t, *want[name])
+
+
+def _odd_values(path):
+    """Infinities and NaN in x, the weight and the gradient reach what they reach in a float32 sum, and nothing else; rows
+    and columns of very different magnitudes keep float32 accuracy each."""
+    d = dev()
+    print(f'[case] odd values, {path}', flush=True)
+    rng = np.random.default_rng(21)
+    T, K, N = 200, 96, 160
+    x, w, g = rand(rng, T, K), rand(rng, N, K), rand(rng, T, N)
+    x = x * torch.logspace(-18, 18, T)[:, None]
+    w = w * torch.logspace(-9, 9, N)[:, None]
+    want = dense_case(x, w, None, None, None, None, F32)
+    near('y', mhk.dense(x.to(d), w.to(d)), *want['y'])
+    x, w = rand(rng, T, K) * torch.logspace(-15, 12, K), rand(rng, N, K) * torch.logspace(-9, 9, K)
+    g = rand(rng, T, N) * torch.logspace(-12, 9, N)
+    want = dense_case(x, w, None, None, None, g, F32)
+    lx, lw = x.to(d).requires_grad_(), w.to(d).requires_grad_()
+    dx, dw = torch.autograd.grad(mhk.dense(lx, lw), (lx, lw), g.to(d))
+    near('dw', dw, *want['dw'])
+    near('dx', dx, *want['dx'])
+    x, w, g = rand(rng, T, K), rand(rng, N, K), rand(rng, T, N)
+    w[:, 5], w[3, 5], w[4, 5] = 1.0, 0.0, -2.0
+    x[0, 5], x[150, 5], x[1, 7], w[9, 11] = float('inf'), float('-inf'), float('nan'), float('inf')
+    g[7, 9], g[8, 10], g[9, 140] = float('nan'), float('inf'), float('-inf')
+    for name, got, want in (('y', mhk.dense(x.to(d), w.to(d)), x.double() @ w.double().t()),):
+        odd = ~torch.isfinite(want)
+        assert odd[0].all() and torch.isinf(want[0, 0]) and torch.isnan(want[0, 3]) and not odd[2, 0]
+        assert torch.equal(torch.isnan(got.cpu()), torch.isnan(want)), name
+        inf = odd & ~torch.isnan(want)
+        assert torch.equal(got.cpu().double()[inf], want[inf]), name
+        near(name, got.cpu()[~odd], want[~odd], (K + 16) * E32 * (x.nan_to_num(0, 0, 0).double().abs()
+                                                                  @ w.nan_to_num(0, 0, 0).double().abs().t())[~odd])
+    x, w = x.nan_to_num(0.5, 0.5, 0.5), w.nan_to_num(0.5, 0.5, 0.5)
+    lx, lw = x.to(d).requires_grad_(), w.to(d).requires_grad_()
+    dx, dw = torch.autograd.grad(mhk.dense(lx, lw), (lx, lw), g.to(d))
+    for name, got, want, odd in (('dx', dx, g.double() @ w.double(), [7, 8, 9]), ('dw', dw, g.double().t() @ x.double(), [9, 10, 140])):
+        got = got.cpu()
+        rest = [i for i in range(len(want)) if i not in odd]
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.isfinite(got[rest]).all(), name
+        inf = torch.isinf(want)
+        assert inf.any() and torch.equal(got.double()[inf], want[inf]), name
+
+
+def test_odd_values_direct():
+    _odd_values('direct')
+
+
+def test_odd_values_by_halves(by_halves):
+    _odd_values('halves')
 
 
 @pytest.mark.parametrize('T,K,N', [(300, 200, 264), (1, 8, 8), (513, 64, 72), (260, 328, 520)])
