@@ -136,7 +136,8 @@ enum mh_kernel_kind {
     MH_HV_COLUMNS = 97,  /* float16 halves of float32 columns                                                  */
     MH_HV_MM = 98,       /* MH_MM_ROWS on halves                                                               */
     MH_HV_OUTER = 99,    /* MH_MM_OUTER on halves                                                              */
-    MH_NUM_KINDS = 100
+    MH_MM_PAD = 100,     /* rows of 16-bit values at whole steps of 16 bytes                                   */
+    MH_NUM_KINDS = 101
 };
 
 /* flags of mh_conv_bwd */
@@ -705,7 +706,8 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
 
 /* The trainable layers on node features (no reference counterparts: the reference has no layers with weight gradients).
  * `type` of a module is the tensors': float32, bfloat16 or float16 (compiled in: matmul.source, experts.source,
- * norms.source).  Rows of x, g and residuals lie `ld` elements apart (ld >= their length); everything else is contiguous.
+ * norms.source).  Rows of x, g, p, residuals and (per group one after the other) weights lie
+ * `ld` elements apart (ld >= their length); everything else is contiguous.
  * Workspaces are the caller's; nothing is kept between calls.  Sizes past 2^31 - 1 rows or columns are refused.
  *
  * Groups: offsets [E + 1] int32 on the device, group e = rows offsets[e] .. offsets[e + 1] - 1 (not decreasing, within
@@ -716,14 +718,15 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * res [R, N] and slope may be NULL.  Rows of no group are zero.  act (none, relu, silu, gelu by erf) is compiled in.  slope [R, N]
  * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types uint16 fixed point (steps of 2^-15
  * from -0.5; 65535: NaN).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
- * Modules of a tile in matmul.FAST need every row distance, contiguous length and address to be multiples of 16 bytes.
+ * Modules of a tile in matmul.FAST need every address and row distance to be multiples of 16 bytes and rows padded to such,
+ * with zeros in operands whose rows are contracted (mh_mm_pad: y [R, Kp] = x [R, K] and zeros, MH_MM_PAD with 256 threads).
  *
  * mh_mm_outer: C[e] [M, N] = sum over the group's rows of A[r, :]^T B[r, :] (A [R, M], B [R, N]; an empty group: zeros).
  * L > 0: the groups' rows are cut into pieces of L, `slots` >= the number of pieces, whose float32 sums go to
  * part [slots, M, N]; mh_mm_sum then adds them: out[e, i] = sum of part[s, i] over e's pieces in order, i < n.  With
  * L = 0 part may be NULL.  Bind MH_MM_OUTER as MH_MM_ROWS, MH_MM_SUM with 1024 threads.
  *
- * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1) for rows g [R, N], and the sums of p's columns before
+ * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1; zeros from N to ldp <= N + 8) for rows g [R, N], and the sums of p's columns before
  * rounding: over each piece of L rows into part [slots, N], or with one slot of all rows into db [N] (both NULL: none).
  * Rows of no group are left alone.  Bind MH_MM_SLOPE with 256 threads.
  *
@@ -758,18 +761,19 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * compiled in); modules without a branch take y, h NULL.  stats [T, 4] float32 (NULL: none) for mh_norm_bwd, which gives dx,
  * dy, dgate and dw [3, C] = the gradients of scale, wp and wn (each may be NULL) from gh and gn (NULL: 0); part [blocks, 3, C]
  * is scratch for the workgroups' sums and sums a module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD as norms.module does. */
-int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
-               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream);
+int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, const void* bias,
+               const void* res, int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream);
 int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
                 const int32_t* offsets, int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
 int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,
               void* stream);
-int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, void* db,
-                const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, int64_t ldp, float* part,
+                void* db, const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
 int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g, int64_t ldg, const void* slope,
-              const void* W, const void* x, int64_t ldx, const int32_t* offsets, void* p, void* dx, void* dW, void* db,
-              float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
+              const void* W, int64_t ldw, const void* x, int64_t ldx, const int32_t* offsets, void* p, int64_t ldp, void* dx,
+              void* dW, void* db, float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
               int32_t slots_o, void* stream);
+int mh_mm_pad(mh_module* m, const void* x, int64_t ldx, void* y, int32_t R, int32_t K, int32_t Kp, void* stream);
 int mh_hv_rows(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, int32_t R, int32_t K, void* stream);
 int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, const int32_t* offsets, int32_t R,
                   int32_t C, int32_t E, int32_t G, int32_t L, int32_t slots, void* stream);

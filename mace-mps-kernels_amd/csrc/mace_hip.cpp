@@ -1221,17 +1221,17 @@ int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
 
 extern "C" {
 
-int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, void* C, const void* bias, const void* res,
-               int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream) {
+int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, const void* bias,
+               const void* res, int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream) {
     if (R < 0 || N < 0 || K < 0 || E < 1 || (E > 1 && !offsets)) return fail(-1, "mh_mm_rows: bad sizes");
     if (R == 0 || N == 0) return 0;
     if (!C || (K > 0 && (!A || !B))) return fail(-1, "mh_mm_rows: NULL operand");
-    if (lda < K || (res && ldr < N)) return fail(-1, "mh_mm_rows: rows overlap (ld below the row's length)");
+    if (lda < K || ldb < 1 || (res && ldr < N)) return fail(-1, "mh_mm_rows: rows overlap (ld below the row's length)");
     if (!m || !m->k[MH_MM_ROWS].fn) return fail(-1, "mh_mm_rows: kernel slot not bound in this module");
     const Kernel& k = m->k[MH_MM_ROWS];
     if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_mm_rows: too many rows");
     const int64_t tiles = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
-    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldr, &R, &N, &K, &E};
+    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldb, &ldr, &R, &N, &K, &E};
     return launch_blocks(m, MH_MM_ROWS, tiles, args, stream, "mh_mm_rows");
 }
 
@@ -1265,26 +1265,28 @@ int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets
     return launch_blocks(m, MH_MM_SUM, (n + columns - 1) / columns, args, stream, "mh_mm_sum", E);
 }
 
-int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, float* part, void* db,
-                const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
+int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, int64_t ldp, float* part,
+                void* db, const int32_t* offsets, int32_t R, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
     if (R < 0 || N < 0 || E < 1 || (E > 1 && !offsets) || L < 1 || slots < 0 || R > 0x7fffffff - L)
         return fail(-1, "mh_mm_slope: bad sizes");
     if (db && (offsets || slots != 1 || L < R)) return fail(-1, "mh_mm_slope: db itself takes one slot of all rows");
     if (N == 0 || (R == 0 && !db)) return 0;
     if ((R > 0 && !g) || (!p && !part && !db)) return fail(-1, "mh_mm_slope: NULL operand");
-    if (ldg < N) return fail(-1, "mh_mm_slope: rows overlap (ld below the row's length)");
-    void* args[] = {&g, &slope, &p, &part, &db, &offsets, &ldg, &R, &N, &E, &L};
-    return launch_blocks(m, MH_MM_SLOPE, slots, args, stream, "mh_mm_slope", (static_cast<int64_t>(N) + 255) / 256);
+    if (ldg < N || (p && (ldp < N || ldp > N + 8LL)))
+        return fail(-1, "mh_mm_slope: rows overlap (ld below the row's length), or p padded by more than 8");
+    const int64_t width = p ? ldp : N;
+    void* args[] = {&g, &slope, &p, &part, &db, &offsets, &ldg, &ldp, &R, &N, &E, &L};
+    return launch_blocks(m, MH_MM_SLOPE, slots, args, stream, "mh_mm_slope", (width + 255) / 256);
 }
 
 int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g, int64_t ldg, const void* slope,
-              const void* W, const void* x, int64_t ldx, const int32_t* offsets, void* p, void* dx, void* dW, void* db,
-              float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
+              const void* W, int64_t ldw, const void* x, int64_t ldx, const int32_t* offsets, void* p, int64_t ldp, void* dx,
+              void* dW, void* db, float* part, int32_t R, int32_t N, int32_t K, int32_t E, int32_t Ls, int32_t slots_s, int32_t Lo,
               int32_t slots_o, void* stream) {
     if ((slope != nullptr) != (p != nullptr)) return fail(-1, "mh_mm_bwd: p goes with slope");
     if (p || db) {
         const bool whole = db && !offsets && slots_s == 1;
-        if (int rc = mh_mm_slope(sums, g, ldg, slope, p, db && !whole ? part : nullptr, whole ? db : nullptr, offsets, R, N, E,
+        if (int rc = mh_mm_slope(sums, g, ldg, slope, p, ldp, db && !whole ? part : nullptr, whole ? db : nullptr, offsets, R, N, E,
                                  Ls, slots_s, stream))
             return rc;
         if (db && !whole)
@@ -1292,16 +1294,25 @@ int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g,
     }
     if (p) {
         g = p;
-        ldg = N;
+        ldg = ldp;
     }
     if (dx)
-        if (int rc = mh_mm_rows(rows, g, ldg, W, dx, nullptr, nullptr, 0, nullptr, offsets, R, K, N, E, stream)) return rc;
+        if (int rc = mh_mm_rows(rows, g, ldg, W, ldw, dx, nullptr, nullptr, 0, nullptr, offsets, R, K, N, E, stream)) return rc;
     if (dW) {
         // the parts of db have been added by now: their place is free
         if (int rc = mh_mm_outer(outer, g, ldg, x, ldx, dW, part, offsets, R, N, K, E, Lo, slots_o, stream)) return rc;
         if (Lo) return mh_mm_sum(sums, part, dW, offsets, R, E, Lo, static_cast<int64_t>(N) * K, stream);
     }
     return 0;
+}
+
+int mh_mm_pad(mh_module* m, const void* x, int64_t ldx, void* y, int32_t R, int32_t K, int32_t Kp, void* stream) {
+    if (R < 0 || K < 1 || Kp < K || Kp % 8) return fail(-1, "mh_mm_pad: bad sizes");
+    if (R == 0) return 0;
+    if (!x || !y) return fail(-1, "mh_mm_pad: NULL operand");
+    if (ldx < K) return fail(-1, "mh_mm_pad: rows overlap (ld below the row's length)");
+    void* args[] = {&x, &y, &ldx, &R, &K, &Kp};
+    return launch_blocks(m, MH_MM_PAD, (static_cast<int64_t>(R) * (Kp / 8) + 255) / 256, args, stream, "mh_mm_pad");
 }
 
 int mh_hv_rows(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, int32_t R, int32_t K, void* stream) {

@@ -392,6 +392,7 @@ template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK, int 
 struct mm_tile {
     typedef typename mm_type<TY>::t T;
     static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, OPR = BK / 8, ROWS = FM, COLS = FN;
+    static constexpr bool WHOLE_STEPS = false;
     static constexpr int PLANES = TY == MM_F32 ? 3 : 1;
     static constexpr int TA = PLANES * BM * OPR, TB = PLANES * BN * OPR;      // octets of a buffer
     static constexpr int LDS = BUFS * (TA + TB);
@@ -483,8 +484,9 @@ struct mm_tile {
 // double-buffered.  An operand contiguous along k is laid out as above; a strided one keeps its rows of k, [k][ROWS], and its
 // fragments are read by transposing LDS reads (four k of 16 rows at a time).  Sixteen rows of a fragment are 32 bytes of a
 // row of k, and the 32-byte pieces of row k are exchanged by f(k) so that the rows which one read touches fall into different
-// banks.  Every operand's contiguous length, its row distance and its address are multiples of 16 bytes (the caller
-// checks); a load past the rows' end repeats the last ones, and one past kend is out of the buffer's range and gives zeros.
+// banks.  Every operand's row distance and address are multiples of 16 bytes, and so are its rows' lengths, or they are padded
+// to that, with zeros where the contraction runs along them (the caller sees to it); a load past the rows' end repeats the
+// last ones, and one past kend is out of the buffer's range and gives zeros.
 typedef __attribute__((address_space(3))) void mm_lds_void;
 
 __device__ __forceinline__ int mm_turn(int k) { return (k & 3) | (k >> 1 & 4); }
@@ -555,6 +557,7 @@ template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK, bool
 struct mm_fast_tile {
     typedef unsigned short T;
     static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, ROWS = FM, COLS = FN;
+    static constexpr bool WHOLE_STEPS = true;
     static constexpr int TA = BM * BK / 8, TB = BN * BK / 8, LDS = 2 * (TA + TB);
     mh_f4 acc[FM][FN];
 
@@ -673,6 +676,11 @@ struct mm_fast_tile {
     __device__ __forceinline__ mh_f4 value(int i, int j) const { return acc[i][j]; }
 };
 
+// The length of a strided operand's rows as a tile may load them: whole steps of 16 bytes where it goes straight to LDS (rows
+// are padded to that; what the padding holds reaches only results that are not stored).
+template <typename tile_t, bool STRIDED>
+__device__ __forceinline__ int mm_wide(int n) { return STRIDED && tile_t::WHOLE_STEPS ? (n + 7) & ~7 : n; }
+
 // The tile (mt, nt) of a block among MT x NT: bands of eight row tiles, walked column by column, in one contiguous range
 // per XCD, so that blocks which share an L2 share operand tiles.
 __device__ __forceinline__ void mm_tile_of(int b, int blocks, int MT, int NT, int& mt, int& nt) {
@@ -748,8 +756,8 @@ __device__ __forceinline__ void mm_store_tile(const tile_t& t, long long r0, int
 // epilogue v = sums + bias[e]; slope = act'(v); C = act(v) + res.  Rows of no group are written as zeros.
 template <int TY, bool BS, int ACT, typename tile_t>
 __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
-                                             void* slope_, const int* off, long long lda, long long ldr, int R, int N, int K,
-                                             int E) {
+                                             void* slope_, const int* off, long long lda, long long ldb, long long ldr, int R, int N,
+                                             int K, int E) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
     const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT;
@@ -769,8 +777,8 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
         return;
     }
     const T* A = static_cast<const T*>(A_) + (long long)r0 * lda;
-    const T* B = static_cast<const T*>(B_) + (long long)e * N * K + (BS ? (long long)n0 : (long long)n0 * K);
-    t.run(lds, A, lda, rows, B, BS ? N : K, min(N - n0, tile_t::BN), 0, K);
+    const T* B = static_cast<const T*>(B_) + (BS ? (long long)e * K * ldb + n0 : ((long long)e * N + n0) * ldb);
+    t.run(lds, A, lda, rows, B, ldb, min(mm_wide<tile_t, BS>(N) - n0, tile_t::BN), 0, K);
     const T* bias = bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr;
     const T* res = static_cast<const T*>(res_);
     if (n0 + tile_t::BN <= N)
@@ -785,8 +793,8 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
 // pieces of 16 weight rows in flight.  float32 uses v_mfma_f32_16x16x4_f32 (k in the order 4 q + j of four steps).
 template <int TY, int ACT, int TM, int WAVES>
 __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
-                                            void* slope_, const int* off, long long lda, long long ldr, int R, int N, int K,
-                                            int E) {
+                                            void* slope_, const int* off, long long lda, long long ldb, long long ldr, int R, int N,
+                                            int K, int E) {
     typedef typename mm_type<TY>::t T;
     constexpr int V = TY == MM_F32 ? 4 : 8, STEP = 4 * V, BATCH = 4;
     __shared__ mh_f4 sums[WAVES][TM][64];
@@ -801,7 +809,7 @@ __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void
         for (int j = threadIdx.x; j < rows * cols; j += 64 * WAVES) C[(long long)(r0 + j / cols) * N + n0 + j % cols] = 0;
         return;
     }
-    const T* b = static_cast<const T*>(B_) + ((long long)e * N + n0 + min(i, cols - 1)) * K + V * q;
+    const T* b = static_cast<const T*>(B_) + ((long long)e * N + n0 + min(i, cols - 1)) * ldb + V * q;
     const T* a[TM];
 #pragma unroll
     for (int t = 0; t < TM; ++t)
@@ -900,8 +908,9 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
     }
     const int m0 = mt * tile_t::BM, n0 = nt * tile_t::BN;
     tile_t t;
-    t.run(lds, static_cast<const T*>(A_) + (long long)r0 * lda + m0, lda, min(M - m0, tile_t::BM),
-          static_cast<const T*>(B_) + (long long)r0 * ldb + n0, ldb, min(N - n0, tile_t::BN), 0, r1 - r0);
+    t.run(lds, static_cast<const T*>(A_) + (long long)r0 * lda + m0, lda, min(mm_wide<tile_t, true>(M) - m0, tile_t::BM),
+          static_cast<const T*>(B_) + (long long)r0 * ldb + n0, ldb, min(mm_wide<tile_t, true>(N) - n0, tile_t::BN), 0,
+          r1 - r0);
     const long long at = (long long)(L ? (int)blockIdx.y : e) * M * N;
 #pragma unroll
     for (int i = 0; i < tile_t::ROWS; ++i)
@@ -954,13 +963,13 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
     if (c > 0) mm_put4<TY>(static_cast<T*>(out_) + (long long)e * n + i, v, c);
 }
 
-// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1) and the sums of its columns in float32, before
+// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1), rows ldp >= N apart with zeros behind N, and the sums of its columns in float32, before
 // rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows, rounded into db (both NULL: none).
 // A workgroup takes a slot and 256 columns, 64 threads of four columns each by four rows at a time.  Bound by its bytes; the
 // slope is read for the last time, past the caches: 69 us at 16,384 x 4,096 bfloat16, 5.8 TB/s (81 as an ordinary read).
 template <int TY>
 __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, void* db, const int* off,
-                                              long long ldg, int R, int N, int E, int L) {
+                                              long long ldg, long long ldp, int R, int N, int E, int L) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_f4 sums[4][64];
     int e, r0, r1;
@@ -993,7 +1002,7 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
                     v = times(v, mh_u4{d.x, d.y, 0u, 0u});
                 }
             }
-            if (P) mm_put4<TY>(P + at, v);
+            if (P) mm_put4<TY>(P + r * ldp + n, v);
             s += v;
         }
     } else if (c > 0) {
@@ -1010,9 +1019,11 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
                     }
                 v = times(v, d);
             }
-            if (P) mm_put4<TY>(P + at, v, c);
+            if (P) mm_put4<TY>(P + r * ldp + n, v, (int)min((long long)4, ldp - n));
             s += v;
         }
+    } else if (P && n < ldp) {
+        for (int r = r0 + w; r < r1; r += 4) mm_put4<TY>(P + r * ldp + n, s, (int)min((long long)4, ldp - n));
     }
     if (!part && !db) return;
     sums[w][lane] = s;
@@ -1024,4 +1035,16 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
         if (db) mm_put4<TY>(static_cast<T*>(db) + n, s, c);
         else mm_put4<MM_F32>(part + (long long)blockIdx.x * N + n, s, c);
     }
+}
+
+// y [R, Kp] = x [R, K] with zeros behind K: rows of 16-bit values at whole steps of 16 bytes.  A thread copies one step.
+template <int TY>
+__device__ __forceinline__ void mm_pad_body(const void* x, void* y, long long ld, int R, int K, int Kp) {
+    typedef typename mm_type<TY>::t T;
+    const int steps = Kp / 8;
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x, r = i / steps;
+    const int k = (int)(i % steps) * 8;
+    if (r < R)
+        *reinterpret_cast<mh_u4*>(static_cast<T*>(y) + r * Kp + k) =
+            mm_vec<TY>::raw(static_cast<const T*>(x) + r * ld + k, K - k);
 }

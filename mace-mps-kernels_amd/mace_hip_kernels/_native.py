@@ -30,7 +30,7 @@ MH_CONV_FWD, MH_CONV_BWD, MH_CONV_BWD_WY, MH_SC_FWD, MH_SC_BWD, MH_CONV_BWD_R, M
     MH_EDGE_BWD, MH_MLP_BWD_P, MH_LIN_BWD_SUM, MH_MLP_H3T, MH_CONV_BWD_T, \
     MH_GEOM_STRAIN, MH_GEOM_DET, MH_MLP_BWD_W, MH_MM_ROWS, MH_MM_OUTER, MH_MM_SUM, MH_MM_SLOPE, MH_EXPERT_HIST, \
     MH_EXPERT_PLACE, MH_DISPATCH, MH_COMBINE, MH_COMBINE_BWD, MH_NORM_FWD, MH_NORM_BWD, MH_HV_ROWS, \
-    MH_HV_PEAKS, MH_HV_COLUMNS, MH_HV_MM, MH_HV_OUTER = range(100)
+    MH_HV_PEAKS, MH_HV_COLUMNS, MH_HV_MM, MH_HV_OUTER, MH_MM_PAD = range(101)
 MH_WANT_GX, MH_WANT_GWY, MH_CUT_MASKED, MH_CUT_NOZERO = 1, 2, 4, 8
 ABI_VERSION = 49
 
@@ -133,11 +133,12 @@ _SIGS = {
     'mh_neighbour_list_work_size': (ctypes.c_size_t, [_I, _I, ctypes.c_int64]),
     'mh_neighbour_list': (ctypes.c_int, [_P] * 5 + [_I, _I, ctypes.c_double, ctypes.c_int64, ctypes.c_int64]
                           + [_P] * 3 + [_I] + [_P] * 3),
-    'mh_mm_rows': (ctypes.c_int, [_P, _P, _L] + [_P] * 4 + [_L, _P, _P] + [_I] * 4 + [_P]),
+    'mh_mm_rows': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 3 + [_L, _P, _P] + [_I] * 4 + [_P]),
     'mh_mm_outer': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 3 + [_I] * 6 + [_P]),
     'mh_mm_sum': (ctypes.c_int, [_P] * 4 + [_I] * 3 + [_L, _P]),
-    'mh_mm_slope': (ctypes.c_int, [_P, _P, _L] + [_P] * 5 + [_I] * 5 + [_P]),
-    'mh_mm_bwd': (ctypes.c_int, [_P] * 4 + [_L] + [_P] * 3 + [_L] + [_P] * 6 + [_I] * 8 + [_P]),
+    'mh_mm_slope': (ctypes.c_int, [_P, _P, _L, _P, _P, _L] + [_P] * 3 + [_I] * 5 + [_P]),
+    'mh_mm_bwd': (ctypes.c_int, [_P] * 4 + [_L, _P, _P, _L, _P, _L, _P, _P, _L] + [_P] * 4 + [_I] * 8 + [_P]),
+    'mh_mm_pad': (ctypes.c_int, [_P, _P, _L, _P] + [_I] * 3 + [_P]),
     'mh_hv_rows': (ctypes.c_int, [_P, _P, _L, _P, _P, _I, _I, _P]),
     'mh_hv_columns': (ctypes.c_int, [_P, _P, _L] + [_P] * 3 + [_I] * 6 + [_P]),
     'mh_hv_mm': (ctypes.c_int, [_P] * 6 + [_L] + [_P] * 5 + [_I] * 4 + [_P]),

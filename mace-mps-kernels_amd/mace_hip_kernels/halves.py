@@ -105,7 +105,7 @@ def product(x, ld, weight, bias, res, ldr, act, slope, offsets, groups, out):
 def input_gradient(p, ldp, weight, offsets, groups, out):
     """out [R, K] = p weight per group, p [R, N], weight [groups, N, K]."""
     R, N = p.shape
-    K = out.shape[1]
+    K = out.shape[-1]
     ph, pp = split_rows(p, ldp, R, N)
     wh, wp = split_columns(weight, K, groups * N, K, groups)
     P = _native.ptr

@@ -14,6 +14,7 @@ halves, ``halves``); 16-bit operands run as they are; every sum is float32 and r
 workgroups are added in a fixed order, so results are bitwise repeatable.  The reference has no such layers.
 """
 import functools
+import math
 
 import torch
 
@@ -24,12 +25,18 @@ ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
 # Tiles: waves (rows x columns), 16 x 16 fragments per wave (rows x columns).  Operands of float32 and of unaligned 16-bit
 # tensors pass through registers (SLOW, also k per LDS buffer and buffers: float32 keeps three bf16 planes and two
-# accumulators); aligned 16-bit ones go straight to LDS (FAST).
+# accumulators, and its 128 x 128 tile measured slower everywhere, 20,000 x 128 x 512 forward 38 against 28 us); 16-bit ones
+# of whole 16-byte steps go straight to LDS (FAST, also k per buffer).
 SLOW = {
-    'slow128': {4: (2, 2, 4, 4, 32, 1), 2: (2, 2, 4, 4, 64, 2)},
+    'slow128': {2: (2, 2, 4, 4, 64, 2)},
     'slow64': {4: (2, 2, 2, 2, 32, 1), 2: (2, 2, 2, 2, 64, 2)},
 }
 FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 2, 4, 4, 64), 'fast64': (2, 2, 2, 2, 64)}
+# What the choices between them go by, as measured: workgroups on a compute unit at once, and the device's rate in 1e12
+# operations a second with all of those and with one each (bfloat16 at 16,384 x 1,024 x 4,096: 157, 176 and 234 us forward with
+# 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11; float32 135 of its own)
+SPEED = {'fast256': (1, 1000, 1000), 'fast128': (2, 820, 640), 'fast64': (4, 600, 250), 'slow128': (2, 650, 400),
+         'slow64': (4, 510, 250)}
 # few rows (forward): 16-row fragments, and the waves that share the contraction
 FEW = {'few16': (1, 4), 'few32': (2, 4), 'few64': (4, 4)}
 CUS = 256                # compute units of an MI355X
@@ -51,7 +58,7 @@ def tile_shape(tile, dtype):
 
 def tiles(dtype):
     """The tiles of a type for all three products, largest first."""
-    return [*(FAST if dtype.itemsize == 2 else ()), *SLOW]
+    return [*(FAST if dtype.itemsize == 2 else ()), *(t for t in SLOW if dtype.itemsize in SLOW[t])]
 
 
 def source(dtype, mode, tile=None, act=0):
@@ -63,12 +70,15 @@ def source(dtype, mode, tile=None, act=0):
         L += ['extern "C" __global__ __launch_bounds__(1024) void mm_sum(const float* part, void* out, const int* off, int R, '
               'int E, int L, int lg, long long n) {', f'  mm_sum_body<{ty}>(part, out, off, R, E, L, lg, n);', '}',
               'extern "C" __global__ __launch_bounds__(256) void mm_slope(const void* g, const void* slope, void* P, '
-              'float* part, void* db, const int* off, long long ldg, int R, int N, int E, int L) {',
-              f'  mm_slope_body<{ty}>(g, slope, P, part, db, off, ldg, R, N, E, L);', '}']
+              'float* part, void* db, const int* off, long long ldg, long long ldp, int R, int N, int E, int L) {',
+              f'  mm_slope_body<{ty}>(g, slope, P, part, db, off, ldg, ldp, R, N, E, L);', '}']
+        if dtype.itemsize == 2:
+            L += ['extern "C" __global__ __launch_bounds__(256) void mm_pad(const void* x, void* y, long long ld, int R, int K, '
+                  'int Kp) {', f'  mm_pad_body<{ty}>(x, y, ld, R, K, Kp);', '}']
         return '\n'.join(L) + '\n'
-    args = 'A, B, C, bias, res, slope, off, lda, ldr, R, N, K, E'
-    tail = ('const void* bias, const void* res, void* slope, const int* off, long long lda, long long ldr, int R, int N, '
-            'int K, int E) {')
+    args = 'A, B, C, bias, res, slope, off, lda, ldb, ldr, R, N, K, E'
+    tail = ('const void* bias, const void* res, void* slope, const int* off, long long lda, long long ldb, long long ldr, '
+            'int R, int N, int K, int E) {')
     if tile in FEW:
         tm, waves = FEW[tile]
         L += [f'extern "C" __global__ __launch_bounds__({64 * waves}) void mm_{mode}({_PTRS}{tail}',
@@ -98,7 +108,10 @@ def module(device, dtype, mode, tile=None, act=0):
         code = _native.compile_source(source(dtype, mode, tile, act))
         with torch.cuda.device(device):
             if mode == 'sum':
-                m = _native.Module(code, {_native.MH_MM_SUM: ('mm_sum', 1024, 1), _native.MH_MM_SLOPE: ('mm_slope', 256, 1)})
+                kinds = {_native.MH_MM_SUM: ('mm_sum', 1024, 1), _native.MH_MM_SLOPE: ('mm_slope', 256, 1)}
+                if dtype.itemsize == 2:
+                    kinds[_native.MH_MM_PAD] = ('mm_pad', 256, 1)
+                m = _native.Module(code, kinds)
             else:
                 waves = FEW[tile][1] if tile in FEW else _tile(tile, dtype)[0] * _tile(tile, dtype)[1]
                 kind = _native.MH_MM_OUTER if mode == 'dw' else _native.MH_MM_ROWS
@@ -119,19 +132,33 @@ def rows_of(t, width):
     return t, t.stride(0)
 
 
-def _aligned(t, ld):
-    """Whether the rows of a 16-bit tensor start at multiples of 16 bytes, with a tile's offsets within 2^31 bytes."""
-    return ld % 8 == 0 and t.data_ptr() % 16 == 0 and ld < 2 ** 21
+def _aligned(t, ld, width):
+    """Whether rows of a 16-bit tensor are whole steps of 16 bytes, with a tile's offsets within 2^31 bytes."""
+    return width % 8 == 0 and ld % 8 == 0 and t.data_ptr() % 16 == 0 and ld < 2 ** 21
 
 
-def _choose_tile(rows, cols, dtype, groups, fast):
-    """The largest tile of which there are enough to give every compute unit one, else the smallest."""
-    names = list(FAST) if fast else list(SLOW)
-    for tile in names[:-1]:
+def _up8(n):
+    return -(-n // 8) * 8
+
+
+def _seconds(tile, dtype, tiles, depth):
+    """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` each."""
+    bm, bn = tile_shape(tile, dtype)
+    at_once, full, alone = (3, 140, 60) if dtype == torch.float32 else SPEED[tile]
+    share = tiles / CUS
+    work = 2e-12 * bm * bn * depth * CUS
+    if at_once == 1:
+        return max(1, math.ceil(share)) * (work / full + 3e-6)
+    return max(work / alone, share * work / full) + 2e-6 * max(1.0, share / at_once)
+
+
+def _choose_tile(rows, cols, depth, dtype, groups, fast):
+    """The tile that is fastest by _seconds.  Groups end in part of a tile: half a tile each on average."""
+    def tiles(tile):
         bm, bn = tile_shape(tile, dtype)
-        if (-(-rows // bm) + groups - 1) * -(-cols // bn) >= CUS:
-            return tile
-    return names[-1]
+        return (-(-rows // bm) + (min(groups, rows) - 1) // 2) * -(-cols // bn)
+    names = FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]
+    return min(names, key=lambda t: _seconds(t, dtype, tiles(t), depth))
 
 
 def _few_tile(rows, groups):
@@ -140,59 +167,104 @@ def _few_tile(rows, groups):
     return next((t for t, (fragments, _) in FEW.items() if per <= 16 * fragments), None)
 
 
-def _outer_tile(M, N, dtype, fast):
-    """The largest tile that both sides of a weight fill: splits over rows make up for few tiles."""
-    names = list(FAST) if fast else list(SLOW)
-    return next((t for t in names if min(M, N) >= tile_shape(t, dtype)[0]), names[-1])
+def _outer_plan(R, M, N, groups, grouped, dtype, fast):
+    """(tile, L, slots) of a sum over R rows: whole groups (L 0), or pieces of L rows in ``slots`` slots whose parts are
+    written and read once more; the fastest by _seconds and those bytes."""
+    best = None
+    for tile in FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]:
+        bm, bn = tile_shape(tile, dtype)
+        tiles = -(-M // bm) * -(-N // bn)
+        # the longest group is what the unsplit form waits for: half as long again as the mean one
+        t = _seconds(tile, dtype, tiles * groups, R / groups * (1.5 if grouped and groups > 1 else 1.0))
+        best = min(best or (t, tile, 0, groups), (t, tile, 0, groups))
+        for pieces in (2, 4, 8, 16, 32, 64):
+            L = -(-max(256, -(-R // pieces)) // 64) * 64
+            if L >= R:
+                break
+            slots = -(-R // L) + (groups if grouped else 0)
+            filled = -(-R // L) + (groups - 1) // 2
+            t = _seconds(tile, dtype, tiles * filled, L) + filled * M * N * 8 / 4.5e12 + 5e-6
+            if slots <= 65535 and slots * M * N <= 2 ** 28:
+                best = min(best, (t, tile, L, slots))
+    return best[1:]
 
 
-def _pieces(R, groups, per, tiles, step):
-    """(L, slots) of a sum over R rows split over workgroups: about two workgroups per compute unit in all, each at
-    least 256 rows; L 0 where the groups' tiles fill the device by themselves."""
+def _halves_pieces(R, groups, grouped, tiles):
+    """(L, slots) of a weight gradient by halves: two workgroups per compute unit, each of 256 rows at least."""
     if tiles * groups >= CUS or R <= 256:
         return 0, groups
-    want = max(1, 2 * CUS // tiles)
-    L = max(256, -(-R // want))
-    L = -(-L // step) * step
-    return L, -(-R // L) + (groups if per else 0)
+    L = max(256, -(-R // max(1, 2 * CUS // tiles)))
+    L = -(-L // 64) * 64
+    return L, -(-R // L) + (groups if grouped else 0)
+
+
+def _padding_pays(flops, slow, moved, copies):
+    """Whether copies of ``moved`` bytes (read and written) to whole steps of 16 bytes are worth a fast tile, for a product
+    that runs at ``slow`` 1e12 operations a second through registers (forward about 600, dx 470, dW 240) and at 850 else."""
+    return flops * (1 / slow - 1 / 850) * 1e-12 > 1.2 * (moved / 4.5e12 + 5e-6 * copies)
+
+
+def _pad(t, ld, rows, width):
+    """(rows copied to whole steps of 16 bytes with zeros behind them, their distance)."""
+    to = _up8(width)
+    y = torch.empty((rows, to), device=t.device, dtype=t.dtype)
+    _native.launch('mm_pad', _native.load().mh_mm_pad, module(t.device, t.dtype, 'sum').handle, t.data_ptr(), ld, y.data_ptr(),
+                   rows, width, to, _native.stream_of(t))
+    return y, to
 
 
 # What a call's sizes lead to, kept by the sizes: modules are looked up and shapes chosen once per size, not per call.
 @functools.lru_cache(maxsize=4096)
-def _rows_plan(device, dtype, mode, R, n, K, groups, act, aligned):
-    """The module of a product over rows; None: by halves."""
-    if dtype == torch.float32 and mode == 'fwd' and halves.pays(R, n, K, groups, mode):
-        return None
-    fast = dtype.itemsize == 2 and aligned and K % 8 == 0 and (mode == 'fwd' or n % 8 == 0)
-    tile = (_few_tile(R, groups) if mode == 'fwd' else None) or _choose_tile(R, n, dtype, groups, fast)
-    return module(device, dtype, mode, tile, act)
+def _fwd_plan(device, dtype, R, n, K, groups, act, x_ok, w_ok):
+    """(module, None: by halves; whether x and the weight are copied first)."""
+    if dtype == torch.float32 and halves.pays(R, n, K, groups, 'fwd'):
+        return None, False, False
+    few = _few_tile(R, groups)
+    if few:
+        return module(device, dtype, 'fwd', few, act), False, False
+    fast = pad = dtype.itemsize == 2
+    if fast and not (x_ok and w_ok):
+        fast = pad = _padding_pays(2.0 * R * n * K, 600, 4 * K * (R * (not x_ok) + groups * n * (not w_ok)),
+                                   2 - x_ok - w_ok)
+    return (module(device, dtype, 'fwd', _choose_tile(R, n, K, dtype, groups, fast), act), pad and not x_ok,
+            pad and not w_ok)
 
 
 @functools.lru_cache(maxsize=4096)
-def _bwd_plan(device, dtype, R, N, K, groups, grouped, g_aligned, w_aligned, x_aligned, want_x, want_w, want_b):
+def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok, want_x, want_w, want_b):
     """(modules of the sums, of dx and of dW; rows per piece and pieces of db; of dW; floats of scratch; whether dx and dW go
-    by halves)."""
-    hx, hw = (want and dtype == torch.float32 and R > 0 and N > 0 and K > 0 and halves.pays(R, N, K, groups, mode)
+    by halves; whether g, the weight and x are copied to whole steps first)."""
+    some = R > 0 and N > 0 and K > 0
+    hx, hw = (want and some and dtype == torch.float32 and halves.pays(R, N, K, groups, mode)
               for want, mode in ((want_x, 'dx'), (want_w, 'dw')))
-    want_x = want_x and not hx
-    rows = _rows_plan(device, dtype, 'dx', R, K, N, groups, 0, g_aligned and w_aligned) if want_x and R and K else None
     # db: pieces of rows for about eight workgroups per compute unit (two / four / eight / sixteen: 100 / 100 / 69 / 73 us at
     # 16,384 x 4,096 bfloat16, 84 / 55 / 41 / 48 at 2,048 in eight groups); few rows are one piece that needs no second sum
     Ls = R if R <= 64 and not grouped else min(256, max(16, -(-R * -(-N // 256) // (8 * CUS) // 4) * 4))
     Ls = max(1, Ls)
     slots = max(1, -(-R // Ls)) + (groups if grouped else 0)
     scratch = slots * N if want_b and (grouped or slots > 1) else 0
-    outer, Lo, slots_o = None, 0, groups
+    p_ok = made_p or g_ok
+    fast_x = fast_w = dtype.itemsize == 2 and some
+    if fast_x:
+        flops = 2.0 * R * N * K
+        if not (p_ok and w_ok):
+            fast_x = want_x and _padding_pays(flops, 470, 4 * (R * N * (not p_ok) + groups * N * K * (not w_ok)),
+                                              2 - p_ok - w_ok)
+        if not (p_ok and x_ok):
+            fast_w = want_w and _padding_pays(flops, 240, 4 * R * (N * (not p_ok) + K * (not x_ok)), 2 - p_ok - x_ok)
+    rows = outer = None
+    if want_x and R and K and not hx:
+        rows = module(device, dtype, 'dx', _choose_tile(R, K, N, dtype, groups, fast_x))
+    Lo, slots_o = 0, groups
     if hw:
-        Lo, slots_o = _pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE), 64)
-        scratch = max(scratch, slots_o * N * K if Lo else 0)
+        Lo, slots_o = _halves_pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE))
     elif want_w and N and K:
-        tile = _outer_tile(N, K, dtype, dtype.itemsize == 2 and g_aligned and x_aligned and N % 8 == 0 and K % 8 == 0)
+        tile, Lo, slots_o = _outer_plan(R, N, K, groups, grouped, dtype, fast_w)
         outer = module(device, dtype, 'dw', tile)
-        bm, bn = tile_shape(tile, dtype)
-        Lo, slots_o = _pieces(R, groups, grouped, -(-N // bm) * -(-K // bn), 64)
-        scratch = max(scratch, slots_o * N * K if Lo else 0)
-    return module(device, dtype, 'sum'), rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw
+    scratch = max(scratch, slots_o * N * K if Lo else 0)
+    pads = ((want_x and fast_x or want_w and fast_w) and not p_ok, want_x and fast_x and not w_ok,
+            want_w and fast_w and not x_ok)
+    return module(device, dtype, 'sum'), rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw, pads
 
 
 def _product(x, ld, weight, bias, res, act, offsets, groups, keep):
@@ -203,43 +275,53 @@ def _product(x, ld, weight, bias, res, act, offsets, groups, keep):
     out = torch.empty((R, n), device=dev, dtype=dt)
     slope = torch.empty((R, n), device=dev, dtype=torch.float32 if dt == torch.float32 else torch.uint16) if keep else None
     if R and n:
-        m = _rows_plan(dev, dt, 'fwd', R, n, K, groups, act, _aligned(x, ld) and weight.data_ptr() % 16 == 0)
+        m, pad_x, pad_w = _fwd_plan(dev, dt, R, n, K, groups, act, _aligned(x, ld, K), _aligned(weight, K, K))
         P = _native.ptr
         r, ldr = (None, 0) if res is None else rows_of(res, n)
         if m is None:
             halves.product(x, ld, weight, bias, r, ldr, act, slope, offsets, groups, out)
             return out, slope
-        _native.launch('mm_fwd', _native.load().mh_mm_rows, m.handle, P(x), ld, P(weight), P(out), P(bias), P(r), ldr,
-                       P(slope), P(offsets), R, n, K, groups, _native.stream_of(x))
+        ldw = K
+        if pad_x:
+            x, ld = _pad(x, ld, R, K)
+        if pad_w:
+            weight, ldw = _pad(weight, K, groups * n, K)
+        _native.launch('mm_fwd', _native.load().mh_mm_rows, m.handle, P(x), ld, P(weight), max(1, ldw), P(out), P(bias), P(r),
+                       ldr, P(slope), P(offsets), R, n, K, groups, _native.stream_of(x))
     return out, slope
 
 
 def _backward(g, ldg, slope, weight, x, ldx, offsets, groups, need):
-    """(dx, dW, db) of g [R, N], each where ``need`` says so (weight or x NULL where what they are for is not)."""
+    """(dx, dW, db) of g [R, N], each where ``need`` says so (weight or x None where what they are for is not)."""
     R, N = g.shape
     K = (x if weight is None else weight).shape[-1] if weight is not None or x is not None else 0
     want_x, want_w, want_b = need
     dev, dt, P = g.device, g.dtype, _native.ptr
-    if slope is not None and not (want_x or want_w):
-        want_p = want_b                                  # db alone still needs the product
-    else:
-        want_p = slope is not None
-    g_aligned = want_p or _aligned(g, ldg)
-    sums, rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw = _bwd_plan(
-        dev, dt, R, N, K, groups, offsets is not None, N % 8 == 0 if want_p else g_aligned,
-        weight is not None and weight.data_ptr() % 16 == 0, x is not None and _aligned(x, ldx), want_x, want_w, want_b)
-    p = torch.empty((R, N), device=dev, dtype=dt) if want_p else None
+    made = slope is not None
+    sums, rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw, (pad_g, pad_w, pad_x) = _bwd_plan(
+        dev, dt, R, N, K, groups, offsets is not None, made, made or _aligned(g, ldg, N),
+        weight is not None and _aligned(weight, K, K), x is not None and _aligned(x, ldx, K), want_x, want_w, want_b)
+    p, ldp, ldw = None, 0, max(1, K)
+    if made:
+        ldp = _up8(N) if dt != torch.float32 else N
+        p = torch.empty((R, ldp), device=dev, dtype=dt)
+    elif pad_g:
+        g, ldg = _pad(g, ldg, R, N)
+    if pad_w:
+        weight, ldw = _pad(weight, K, groups * N, K)
+    if pad_x:
+        x, ldx = _pad(x, ldx, R, K)
     dx = torch.empty((R, K), device=dev, dtype=dt) if want_x else None
     dw = torch.empty((groups, N, K), device=dev, dtype=dt) if want_w else None
     db = torch.empty((groups, N), device=dev, dtype=dt) if want_b else None
     part = torch.empty(scratch, device=dev, dtype=torch.float32) if scratch else None
-    if want_p or want_b or rows is not None or outer is not None:
+    if made or want_b or rows is not None or outer is not None:
         _native.launch('mm_bwd', _native.load().mh_mm_bwd, sums.handle, None if rows is None else rows.handle,
-                   None if outer is None else outer.handle, P(g), ldg, P(slope) if want_p else None, P(weight), P(x), ldx,
-                   P(offsets), P(p), P(dx) if rows is not None else None, P(dw) if outer is not None else None, P(db), P(part),
-                   R, N, K, groups, Ls, slots, Lo, slots_o, _native.stream_of(g))
+                       None if outer is None else outer.handle, P(g), ldg, P(slope), P(weight), ldw, P(x), ldx, P(offsets),
+                       P(p), ldp, P(dx) if rows is not None else None, P(dw) if outer is not None else None, P(db), P(part), R,
+                       N, K, groups, Ls, slots, Lo, slots_o, _native.stream_of(g))
     if hx or hw:
-        if want_p:
+        if made:
             g, ldg = p, N
         if hx:
             halves.input_gradient(g, ldg, weight, offsets, groups, dx)

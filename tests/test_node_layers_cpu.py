@@ -30,22 +30,24 @@ def test_c_entry_points_refuse_bad_arguments():
     one = torch.zeros(64)
     p = one.data_ptr()
     cases = [
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, -1, 4, 8, 1, None), 'bad sizes'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 2, None), 'bad sizes'),
-        (lambda: lib.mh_mm_rows(None, None, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'NULL'),
-        (lambda: lib.mh_mm_rows(None, p, 7, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'overlap'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, p, 3, None, None, 2, 4, 8, 1, None), 'overlap'),
-        (lambda: lib.mh_mm_rows(None, p, 8, p, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'not bound'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, 8, p, None, None, 0, None, None, -1, 4, 8, 1, None), 'bad sizes'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, 8, p, None, None, 0, None, None, 2, 4, 8, 2, None), 'bad sizes'),
+        (lambda: lib.mh_mm_rows(None, None, 8, p, 8, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'NULL'),
+        (lambda: lib.mh_mm_rows(None, p, 7, p, 8, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'overlap'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, 8, p, None, p, 3, None, None, 2, 4, 8, 1, None), 'overlap'),
+        (lambda: lib.mh_mm_rows(None, p, 8, p, 8, p, None, None, 0, None, None, 2, 4, 8, 1, None), 'not bound'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, None, None, None, 2, 4, 4, 1, 0, 1, None), 'NULL'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, p, None, None, 2, 4, 4, 1, 16, 1, None), 'NULL'),
         (lambda: lib.mh_mm_outer(None, p, 4, p, 4, p, p, None, 2, 4, 4, 1, 16, 0, None), 'pieces'),
         (lambda: lib.mh_mm_outer(None, p, 3, p, 4, p, p, None, 2, 4, 4, 1, 0, 1, None), 'overlap'),
         (lambda: lib.mh_mm_sum(None, p, p, None, 4, 1, 0, 8, None), 'bad sizes'),
         (lambda: lib.mh_mm_sum(None, None, p, None, 4, 1, 4, 8, None), 'NULL'),
-        (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, None, None, 2, 4, 1, 4, 1, None), 'NULL'),
-        (lambda: lib.mh_mm_slope(None, p, 4, None, None, None, p, None, 2, 4, 1, 1, 2, None), 'one slot'),
-        (lambda: lib.mh_mm_bwd(None, None, None, p, 4, p, p, p, 4, None, None, p, p, p, p, 2, 4, 4, 1, 4, 1, 0, 1, None),
+        (lambda: lib.mh_mm_slope(None, p, 4, None, None, 0, None, None, None, 2, 4, 1, 4, 1, None), 'NULL'),
+        (lambda: lib.mh_mm_slope(None, p, 4, None, None, 0, None, p, None, 2, 4, 1, 1, 2, None), 'one slot'),
+        (lambda: lib.mh_mm_bwd(None, None, None, p, 4, p, p, 4, p, 4, None, None, 0, p, p, p, p, 2, 4, 4, 1, 4, 1, 0, 1, None),
          'goes with slope'),
+        (lambda: lib.mh_mm_slope(None, p, 4, None, p, 3, None, None, None, 2, 4, 1, 4, 1, None), 'padded'),
+        (lambda: lib.mh_mm_pad(None, p, 4, p, 2, 4, 12, None), 'bad sizes'),
         (lambda: lib.mh_hv_rows(None, p, 3, p, p, 2, 4, None), 'overlap'),
         (lambda: lib.mh_hv_columns(None, p, 4, p, p, None, 6, 4, 4, 2, 4, 4, None), 'bad sizes'),
         (lambda: lib.mh_hv_mm(None, p, p, p, None, None, 0, None, None, p, None, None, 2, 4, 4, 1, None), 'NULL'),
@@ -71,15 +73,18 @@ def test_pieces_cover_all_rows_with_enough_slots():
     """Every sum over rows that is split has slots for all its pieces, however the rows fall into groups."""
     rng = random.Random(0)
     for _ in range(400):
-        groups, tiles = rng.choice([1, 2, 7, 64, 300]), rng.choice([1, 3, 20, 200, 4000])
+        groups, M, N = rng.choice([1, 2, 7, 64, 300]), rng.choice([1, 40, 512, 4096]), rng.choice([8, 100, 1024, 2048])
         R = rng.choice([0, 1, 255, 257, 3000, 20000, 10 ** 6])
         cuts = sorted(rng.randint(0, R) for _ in range(groups - 1))
         sizes = [b - a for a, b in zip([0] + cuts, cuts + [R])]
-        L, slots = matmul._pieces(R, groups, groups > 1, tiles, 64)
-        if L == 0:
-            assert slots == groups
-        else:
-            assert L % 64 == 0 and sum(-(-s // L) for s in sizes) <= slots <= 65535
+        dt, fast = rng.choice([(torch.float32, False), (torch.bfloat16, True), (torch.float16, False)])
+        tile, *plan = matmul._outer_plan(R, M, N, groups, groups > 1, dt, fast)
+        assert (tile in matmul.FAST) == fast and tile in matmul.tiles(dt)
+        for L, slots in (plan, matmul._halves_pieces(R, groups, groups > 1, -(-M // 128) * -(-N // 128))):
+            if L == 0:
+                assert slots == groups
+            else:
+                assert L % 64 == 0 and sum(-(-s // L) for s in sizes) <= slots <= 65535
 
 
 def test_norm_shapes_hold_a_row():

@@ -126,11 +126,11 @@ def test_dense_over_many_tiles_and_split_sums(T, K, N, dt):
 def by_halves(monkeypatch):
     """Float32 products by halves whatever their size."""
     monkeypatch.setattr(halves, 'pays', lambda *a: True)
-    matmul._rows_plan.cache_clear()
+    matmul._fwd_plan.cache_clear()
     matmul._bwd_plan.cache_clear()
     yield
     monkeypatch.undo()
-    matmul._rows_plan.cache_clear()
+    matmul._fwd_plan.cache_clear()
     matmul._bwd_plan.cache_clear()
 
 
@@ -211,9 +211,9 @@ def test_odd_values_by_halves(by_halves):
     _odd_values('halves')
 
 
-@pytest.mark.parametrize('T,K,N', [(300, 200, 264), (1, 8, 8), (513, 64, 72), (260, 328, 520)])
+@pytest.mark.parametrize('T,K,N', [(300, 200, 264), (1, 8, 8), (513, 64, 72), (260, 328, 520), (301, 203, 131), (140, 1, 7)])
 @pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
-def test_every_tile_on_aligned_shapes(T, K, N, dt, monkeypatch):
+def test_every_tile(T, K, N, dt, monkeypatch):
     """Each tile in all three products, one and three groups with a tail, whatever the sizes would have chosen."""
     d = dev()
     rng = np.random.default_rng(T)
@@ -223,10 +223,13 @@ def test_every_tile_on_aligned_shapes(T, K, N, dt, monkeypatch):
     one = dense_case(x, w[0], b[0], 'silu', None, g, dt)
     three = [dense_case(x[i:j], w[e], b[e], 'silu', None, g[i:j], dt) for e, (i, j) in enumerate(zip([0] + cuts[:2], cuts))]
     def choose(tile):
-        monkeypatch.setattr(matmul, '_choose_tile', lambda *a: 'slow64' if tile in matmul.FEW else tile)
-        monkeypatch.setattr(matmul, '_outer_tile', lambda *a: 'slow64' if tile in matmul.FEW else tile)
+        main = 'slow64' if tile in matmul.FEW else tile
+        fast = main in matmul.FAST                       # copies to whole steps of 16 bytes where a shape needs them
+        monkeypatch.setattr(matmul, '_choose_tile', lambda *a: main)
+        monkeypatch.setattr(matmul, '_outer_plan', lambda R, M, N, groups, grouped, *a: (main, 128, -(-R // 128) + 3 * grouped))
         monkeypatch.setattr(matmul, '_few_tile', lambda *a: tile if tile in matmul.FEW else None)
-        matmul._rows_plan.cache_clear()
+        monkeypatch.setattr(matmul, '_padding_pays', lambda *a: fast)
+        matmul._fwd_plan.cache_clear()
         matmul._bwd_plan.cache_clear()
 
     for tile in [*matmul.tiles(dt), *matmul.FEW]:
@@ -246,7 +249,7 @@ def test_every_tile_on_aligned_shapes(T, K, N, dt, monkeypatch):
             for name, t in zip(('y', 'dx', 'dw', 'db'), (y[i], grads[0][i], grads[1][e], grads[2][e])):
                 near(f'{name} of {e}', t, *want[name])
     monkeypatch.undo()
-    matmul._rows_plan.cache_clear()
+    matmul._fwd_plan.cache_clear()
     matmul._bwd_plan.cache_clear()
 
 
