@@ -251,7 +251,7 @@ __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const uns
     if (L) {
         if (!mm_slot(off, E, R, L, blockIdx.y, e, r0, r1)) return;
     } else if (off) {
-        e = blockIdx.y;
+        e = mm_by_length(off, E, blockIdx.y);
         r0 = min(max(off[e], 0), R);
         r1 = min(max(off[e + 1], r0), R);
     }

@@ -258,6 +258,20 @@ __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int 
     return false;
 }
 
+// The group that is k-th by length, longest first (up to 64 groups; more are taken as they come): workgroups start in the order
+// of their index, and a long group that starts last is what all others wait for.  Every lane of a wave calls.
+__device__ __forceinline__ int mm_by_length(const int* __restrict__ off, int E, int k) {
+    if (E > MH_WAVE) return k;
+    const int lane = threadIdx.x & (MH_WAVE - 1);
+    const int n = lane < E ? off[lane + 1] - off[lane] : 0;
+    int rank = 0;
+    for (int g = 0; g < E; ++g) {
+        const int m = mh_bcast(n, g);
+        rank += m > n || (m == n && g < lane) ? 1 : 0;
+    }
+    return __ffsll((unsigned long long)__ballot(lane < E && rank == k)) - 1;
+}
+
 // ------------------------------------------------------------------------------------------------ operand tiles
 // A tile of ROWS x BK values of an operand in LDS: octets of eight values along k, 16 bytes each (one plane for the 16-bit
 // types, three for the parts of float32), octet o of row r at r OPR + (o ^ swizzle(r)).  The swizzle gives 16 rows that
@@ -752,6 +766,64 @@ __device__ __forceinline__ void mm_store_tile(const tile_t& t, long long r0, int
     }
 }
 
+// The same for a whole-column tile of 16-bit results whose rows start at multiples of 16 bytes: a wave turns sixteen of its
+// rows at a time in LDS, so that a store writes whole 128-byte lines of eight rows where the lanes' own eight bytes lie in
+// 32-byte pieces of sixteen.
+template <int TY, int ACT, typename tile_t>
+__device__ __forceinline__ void mm_store_lines(const tile_t& t, mh_u4* lds, long long r0, int rows, int n0, int N,
+                                               const unsigned short* bias, const unsigned short* res, long long ldr,
+                                               unsigned short* slope, unsigned short* C) {
+    constexpr int FM = tile_t::ROWS, FN = tile_t::COLS, W = 16 * FN, LD = W + 8, PER = 64 / (W / 8);
+    static_assert(tile_t::THREADS / 64 * 2 * 16 * LD * 2 <= tile_t::LDS * 16, "the waves' places fit the tile's buffers");
+    const int lane = threadIdx.x & 63, i16 = lane & 15, q = lane >> 4;
+    unsigned short* y = reinterpret_cast<unsigned short*>(lds) + (threadIdx.x >> 6) * 2 * 16 * LD;
+    unsigned short* d = y + 16 * LD;
+    mh_f4 bv[FN];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) bv[j] = bias ? mm_get4<TY>(bias + n0 + tile_t::column(j)) : mh_f4{0.f, 0.f, 0.f, 0.f};
+    const int first = tile_t::row(0) - i16, left = n0 + tile_t::column(0) - 4 * q;      // the wave's corner
+    __syncthreads();                                     // every wave is done with the tile's buffers
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+        const int m = min(tile_t::row(i), rows - 1);
+        mh_f4 rv[FN];
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+            rv[j] = res ? mm_get4<TY>(res + (r0 + m) * ldr + n0 + tile_t::column(j)) : mh_f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+            mh_f4 v = t.value(i, j) + bv[j];
+            unsigned c[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                float s;
+                v[k] = mm_activate<TY, ACT>(v[k], s);
+                if (ACT != MM_NONE && slope) c[k] = mm_slope_code(s);
+            }
+            const int at = i16 * LD + 16 * j + 4 * q;
+            v += rv[j];
+            *reinterpret_cast<mh_u2*>(y + at) = mh_u2{mm_round<TY>(v.x) | (unsigned)mm_round<TY>(v.y) << 16,
+                                                      mm_round<TY>(v.z) | (unsigned)mm_round<TY>(v.w) << 16};
+            if (ACT != MM_NONE && slope)
+                *reinterpret_cast<mh_u2*>(d + at) = mh_u2{c[0] | c[1] << 16, c[2] | c[3] << 16};
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int s = 0; s < 16; s += PER) {
+            const int r = s + lane / (W / 8), c = lane % (W / 8) * 8, m = first + 16 * i + r;
+            if (m < rows) {
+                const long long at = (r0 + m) * N + left + c;
+                *reinterpret_cast<mh_u4*>(C + at) = *reinterpret_cast<const mh_u4*>(y + r * LD + c);
+                if (ACT != MM_NONE && slope)
+                    *reinterpret_cast<mh_u4*>(slope + at) = *reinterpret_cast<const mh_u4*>(d + r * LD + c);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
 // Forward and input gradient: R rows of A [R, K] in groups, B the group's weights ([N, K], or [K, N] where BS), the
 // epilogue v = sums + bias[e]; slope = act'(v); C = act(v) + res.  Rows of no group are written as zeros.
 template <int TY, bool BS, int ACT, typename tile_t>
@@ -781,6 +853,12 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
     t.run(lds, A, lda, rows, B, ldb, min(mm_wide<tile_t, BS>(N) - n0, tile_t::BN), 0, K);
     const T* bias = bias_ ? static_cast<const T*>(bias_) + (long long)e * N : nullptr;
     const T* res = static_cast<const T*>(res_);
+    if constexpr (TY != MM_F32) {
+        if (n0 + tile_t::BN <= N && N % 8 == 0) {
+            mm_store_lines<TY, ACT>(t, lds, r0, rows, n0, N, bias, res, ldr, static_cast<T*>(slope_), static_cast<T*>(C_));
+            return;
+        }
+    }
     if (n0 + tile_t::BN <= N)
         mm_store_tile<TY, ACT, true>(t, r0, rows, n0, N, bias, res, ldr, slope_, static_cast<T*>(C_));
     else
@@ -902,7 +980,7 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
     if (L) {
         if (!mm_slot(off, E, R, L, blockIdx.y, e, r0, r1)) return;
     } else if (off) {
-        e = blockIdx.y;
+        e = mm_by_length(off, E, blockIdx.y);
         r0 = min(max(off[e], 0), R);
         r1 = min(max(off[e + 1], r0), R);
     }

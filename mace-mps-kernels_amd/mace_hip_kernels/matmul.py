@@ -23,20 +23,25 @@ from . import _native, halves
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
-# Tiles: waves (rows x columns), 16 x 16 fragments per wave (rows x columns).  Operands of float32 and of unaligned 16-bit
-# tensors pass through registers (SLOW, also k per LDS buffer and buffers: float32 keeps three bf16 planes and two
-# accumulators, and its 128 x 128 tile measured slower everywhere, 20,000 x 128 x 512 forward 38 against 28 us); 16-bit ones
-# of whole 16-byte steps go straight to LDS (FAST, also k per buffer).
+# Tiles: waves (rows x columns), 16 x 16 fragments per wave (rows x columns), k per LDS buffer.  Operands of float32 and of
+# unaligned 16-bit tensors pass through registers (SLOW, also the buffers: float32 keeps three bf16 planes and two
+# accumulators; two buffers, 32 k and a 128 x 128 tile of it all measured slower), 16-bit ones of whole 16-byte steps go
+# straight to LDS (FAST).
 SLOW = {
     'slow128': {2: (2, 2, 4, 4, 64, 2)},
-    'slow64': {4: (2, 2, 2, 2, 32, 1), 2: (2, 2, 2, 2, 64, 2)},
+    'slow64': {4: (2, 2, 2, 2, 64, 1), 2: (2, 2, 2, 2, 64, 2)},
+    'slow32': {4: (2, 2, 1, 1, 64, 1)},
 }
 FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 2, 4, 4, 64), 'fast64': (2, 2, 2, 2, 64)}
 # What the choices between them go by, as measured: workgroups on a compute unit at once, and the device's rate in 1e12
-# operations a second with all of those and with one each (bfloat16 at 16,384 x 1,024 x 4,096: 157, 176 and 234 us forward with
-# 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11; float32 135 of its own)
-SPEED = {'fast256': (1, 1000, 1000), 'fast128': (2, 820, 640), 'fast64': (4, 600, 250), 'slow128': (2, 650, 400),
-         'slow64': (4, 510, 250)}
+# operations a second with all of those and with one each.  bfloat16 at 16,384 x 1,024 x 4,096: 157, 176 and 234 us forward
+# with 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11.  float32 with 64 and 32: at
+# 20,000 x 128 x 512 36 and 46, at 2,533 x 512 x 128 21 and 13, at 700 x 1,000 x 900 30 and 23.
+SPEED = {
+    2: {'fast256': (1, 1000, 1000), 'fast128': (2, 820, 640), 'fast64': (4, 600, 250), 'slow128': (2, 650, 400),
+        'slow64': (4, 510, 250)},
+    4: {'slow64': (3, 140, 63), 'slow32': (6, 105, 33)},
+}
 # few rows (forward): 16-row fragments, and the waves that share the contraction
 FEW = {'few16': (1, 4), 'few32': (2, 4), 'few64': (4, 4)}
 CUS = 256                # compute units of an MI355X
@@ -141,15 +146,15 @@ def _up8(n):
     return -(-n // 8) * 8
 
 
-def _seconds(tile, dtype, tiles, depth):
-    """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` each."""
+def _seconds(tile, dtype, tiles, depth, longest=0):
+    """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` on average, ``longest`` at most."""
     bm, bn = tile_shape(tile, dtype)
-    at_once, full, alone = (3, 140, 60) if dtype == torch.float32 else SPEED[tile]
+    at_once, full, alone = SPEED[dtype.itemsize][tile]
     share = tiles / CUS
-    work = 2e-12 * bm * bn * depth * CUS
+    work, most = (2e-12 * bm * bn * k * CUS for k in (depth, max(depth, longest)))
     if at_once == 1:
-        return max(1, math.ceil(share)) * (work / full + 3e-6)
-    return max(work / alone, share * work / full) + 2e-6 * max(1.0, share / at_once)
+        return max(max(1, math.ceil(share)) * (work / full + 3e-6), most / full)
+    return max(most / alone, share * work / full) + 2e-6 * max(1.0, share / at_once)
 
 
 def _choose_tile(rows, cols, depth, dtype, groups, fast):
@@ -174,8 +179,8 @@ def _outer_plan(R, M, N, groups, grouped, dtype, fast):
     for tile in FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]:
         bm, bn = tile_shape(tile, dtype)
         tiles = -(-M // bm) * -(-N // bn)
-        # the longest group is what the unsplit form waits for: half as long again as the mean one
-        t = _seconds(tile, dtype, tiles * groups, R / groups * (1.5 if grouped and groups > 1 else 1.0))
+        # the longest group is what the unsplit form waits for: of few groups, taken as two and a half times the mean one
+        t = _seconds(tile, dtype, tiles * groups, R / groups, R / groups * (2.5 if 1 < groups <= 64 else 1.0))
         best = min(best or (t, tile, 0, groups), (t, tile, 0, groups))
         for pieces in (2, 4, 8, 16, 32, 64):
             L = -(-max(256, -(-R // pieces)) // 64) * 64
