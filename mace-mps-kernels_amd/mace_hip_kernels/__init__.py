@@ -18,6 +18,10 @@ Everything else stays on the original e3nn / PyTorch path.  The backward pass is
 ``patch_model(model, double_backward=True)`` makes every drop-in differentiable once more (force-loss gradients,
 Hessian-vector products).  The graph itself can be built on the GPU (``neighbour_list``).
 
+The drop-ins hold their weights as constants.  Layers to be trained next to a patched model, with gradients to their
+weights, in float32, bfloat16 and float16: ``dense``, ``expert_dense``, ``expert_order``, ``dispatch``, ``combine``,
+``block_norm``, and modules of them (``NodeFeedForward``, ``NodeHead``).
+
 The kernels are generated per layer with the layer's coefficients as literals, compiled by hipRTC through
 ``libmace_hip.so`` (C ABI in include/mace_hip.h) and launched on torch's current HIP stream.  If that library cannot
 be loaded, ``patch_model`` raises: there is no CPU or eager fallback.
@@ -42,6 +46,7 @@ from . import geometry as _geometry
 from .conv import check_graphs
 from .matmul import dense, expert_dense
 from .experts import ExpertOrder, combine, dispatch, expert_order
+from .feedforward import NodeFeedForward, NodeHead, node_features
 from .neighbours import NeighbourList, neighbour_list, update_batch
 from .norms import block_norm
 
@@ -50,7 +55,8 @@ __all__ = ['patch_model', 'unpatch_model', 'HipConvTP', 'HipSymmetricContraction
            'HipNodeLinear', 'HipRadialMLP', 'HipRadialEmbedding', 'conv_supported', 'sc_supported', 'sh_supported', 'lin_supported',
            'mlp_supported', 'emb_supported', 'HipReshapeIrreps', 'reshape_supported', 'HipReadout',
            'readout_supported', 'neighbour_list', 'update_batch', 'NeighbourList', 'check_graphs', 'dense', 'expert_dense',
-           'ExpertOrder', 'expert_order', 'dispatch', 'combine', 'block_norm']
+           'ExpertOrder', 'expert_order', 'dispatch', 'combine', 'block_norm',
+           'NodeFeedForward', 'NodeHead', 'node_features']
 
 _LINEAR_CLASSES = ('Linear', 'FullyConnectedTensorProduct')
 
