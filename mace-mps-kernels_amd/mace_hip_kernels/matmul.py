@@ -33,14 +33,15 @@ SLOW = {
     'slow32': {4: (2, 2, 1, 1, 64, 1)},
 }
 FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 2, 4, 4, 64), 'fast64': (2, 2, 2, 2, 64)}
-# What the choices between them go by, as measured: workgroups on a compute unit at once, and the device's rate in 1e12
-# operations a second with all of those and with one each.  bfloat16 at 16,384 x 1,024 x 4,096: 157, 176 and 234 us forward
-# with 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11.  float32 with 64 and 32: at
-# 20,000 x 128 x 512 36 and 46, at 2,533 x 512 x 128 21 and 13, at 700 x 1,000 x 900 30 and 23.
+# What the choices between them go by, as measured: workgroups on a compute unit at once, the device's rate in 1e12
+# operations a second with all of those and with one each, and what a round of workgroups costs besides (us, filling the first
+# tile, storing the last).  bfloat16 at 8,192 x 8,192 x 8,192 859 us with 256 and 982 with 128; at 16,384 x 1,024 x 4,096 149,
+# 163 and 234 with 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11.  float32 with
+# 64 and 32: at 20,000 x 128 x 512 36 and 46, at 2,533 x 512 x 128 21 and 13, at 700 x 1,000 x 900 30 and 23.
 SPEED = {
-    2: {'fast256': (1, 1000, 1000), 'fast128': (2, 820, 640), 'fast64': (4, 600, 250), 'slow128': (2, 650, 400),
-        'slow64': (4, 510, 250)},
-    4: {'slow64': (3, 140, 63), 'slow32': (6, 105, 33)},
+    2: {'fast256': (1, 1280, 1280, 10), 'fast128': (2, 1120, 780, 5), 'fast64': (4, 740, 350, 3),
+        'slow128': (2, 800, 480, 5), 'slow64': (4, 620, 300, 3)},
+    4: {'slow64': (3, 150, 70, 3), 'slow32': (6, 110, 38, 2)},
 }
 # few rows (forward): 16-row fragments, and the waves that share the contraction
 FEW = {'few16': (1, 4), 'few32': (2, 4), 'few64': (4, 4)}
@@ -149,12 +150,12 @@ def _up8(n):
 def _seconds(tile, dtype, tiles, depth, longest=0):
     """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` on average, ``longest`` at most."""
     bm, bn = tile_shape(tile, dtype)
-    at_once, full, alone = SPEED[dtype.itemsize][tile]
+    at_once, full, alone, ramp = SPEED[dtype.itemsize][tile]
     share = tiles / CUS
     work, most = (2e-12 * bm * bn * k * CUS for k in (depth, max(depth, longest)))
-    if at_once == 1:
-        return max(max(1, math.ceil(share)) * (work / full + 3e-6), most / full)
-    return max(most / alone, share * work / full) + 2e-6 * max(1.0, share / at_once)
+    if at_once == 1:                                     # whole rounds
+        return max(max(1, math.ceil(share)) * (work / full + ramp * 1e-6), most / full)
+    return max(most / alone, share * work / full) + max(1.0, share / at_once) * ramp * 1e-6
 
 
 def _choose_tile(rows, cols, depth, dtype, groups, fast):

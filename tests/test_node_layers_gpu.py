@@ -352,6 +352,93 @@ def test_expert_dense_and_its_gradients(sizes, K, N, tail, dt):
         near(f'db of {e}', grads[2][e], *want['db'])
 
 
+@pytest.mark.parametrize('dt', [F32, BF16], ids=['f32', 'bf16'])
+def test_each_gradient_alone(dt):
+    """Every subset of inputs with gradients gives the gradients that all together give."""
+    d = dev()
+    rng = np.random.default_rng(31)
+    T, K, N, E = 90, 40, 48, 3
+    x, w, b, r = rand(rng, T, K, dt=dt), rand(rng, E, N, K, dt=dt), rand(rng, E, N, dt=dt), rand(rng, T, N, dt=dt)
+    g = rand(rng, T, N, dt=dt).to(d)
+    off = torch.tensor([0, 20, 20, 85], dtype=torch.int32, device=d)
+    for act in (None, 'silu'):
+        print(f'[case] gradients alone {act} {dt}', flush=True)
+
+        def run(mask):
+            ts = [t.to(d).requires_grad_(m) for t, m in zip((x, w, b, r), mask)]
+            outs = [mhk.expert_dense(ts[0], ts[1], off, ts[2], act, ts[3]),
+                    mhk.dense(ts[0], ts[1][0], ts[2][0], act, ts[3])]
+            ins = [t for t, m in zip(ts, mask) if m]
+            return [torch.autograd.grad(y, ins, g) for y in outs]
+
+        full = run((True,) * 4)
+        for m in range(1, 15):
+            mask = [bool(m >> i & 1) for i in range(4)]
+            for got, want in zip(run(mask), full):
+                for a, bb in zip(got, [t for t, q in zip(want, mask) if q]):
+                    assert torch.equal(a, bb), (act, mask)
+    o = mhk.expert_order(torch.randint(-1, 4, (T, 2), device=d), 4)
+    y, wt, res = rand(rng, 2 * T, N, dt=dt), rand(rng, T, 2), rand(rng, T, N, dt=dt)
+
+    def mix(mask):
+        ts = [t.to(d).requires_grad_(m) for t, m in zip((y, wt, res), mask)]
+        return torch.autograd.grad(mhk.combine(*ts[:2], o, ts[2]), [t for t, m in zip(ts, mask) if m], g)
+
+    full = mix((True,) * 3)
+    for m in range(1, 7):
+        mask = [bool(m >> i & 1) for i in range(3)]
+        for a, bb in zip(mix(mask), [t for t, q in zip(full, mask) if q]):
+            assert torch.equal(a, bb), mask
+
+
+@pytest.mark.parametrize('E', [64, 65, 200, 1000])
+def test_expert_dense_over_many_groups(E):
+    d = dev()
+    print(f'[case] expert_dense of {E} groups', flush=True)
+    rng = np.random.default_rng(E)
+    sizes = rng.integers(0, 9, E) * (rng.random(E) < 0.7)
+    sizes[E // 2] = 150
+    off = torch.tensor(np.concatenate([[0], np.cumsum(sizes)]), dtype=torch.int32)
+    n, K, N = int(off[-1]), 24, 40
+    x, w, g = rand(rng, n + 5, K, dt=BF16), rand(rng, E, N, K, dt=BF16), rand(rng, n + 5, N, dt=BF16)
+    lx, lw = x.to(d).requires_grad_(), w.to(d).requires_grad_()
+    y = mhk.expert_dense(lx, lw, off.to(d), activation='relu')
+    dx, dw = torch.autograd.grad(y, (lx, lw), g.to(d))
+    for e in (0, 1, E // 2, E - 2, E - 1):
+        i = slice(int(off[e]), int(off[e + 1]))
+        want = dense_case(x[i], w[e], None, 'relu', None, g[i], BF16)
+        for name, t in (('y', y[i]), ('dx', dx[i]), ('dw', dw[e])):
+            near(f'{name} of {e}', t, *want[name])
+    assert (y[n:] == 0).all() and (dx[n:] == 0).all()
+
+
+def test_tensors_past_32_bit_offsets():
+    """Results and operands of more than 2^31 values: the rows behind that are as right as the first."""
+    d = dev()
+    print('[case] more than 2^31 values', flush=True)
+    T, K, N = 1_050_000, 16, 2056
+    assert T * N > 2 ** 31
+    g = torch.Generator(device=d).manual_seed(1)
+    x = torch.randn(T, K, generator=g, device=d).bfloat16().requires_grad_()
+    w, b = torch.randn(N, K, generator=g, device=d).bfloat16(), torch.randn(N, generator=g, device=d).bfloat16()
+    y = mhk.dense(x, w, b, 'silu')
+    gy = torch.ones(1, 1, device=d, dtype=BF16).expand(T, N)
+    dx, = torch.autograd.grad(y, x, gy)
+    for i in (slice(0, 40), slice(T - 40, T)):
+        want = dense_case(x.detach()[i].cpu(), w.cpu(), b.cpu(), 'silu', None, torch.ones(40, N, dtype=BF16), BF16)
+        near('y', y[i], *want['y'])
+        near('dx', dx[i], *want['dx'])
+    h, n = mhk.block_norm(y, y, scale=b)
+    want = norm_case(y[-40:].cpu(), y[-40:].cpu(), None, b.cpu(), None, None, None, None, 'rms', 1e-6)
+    near('h', h[-40:], want['h'], 1e-5 * 64 + U[BF16] * want['h'].abs())
+    del h, n
+    e = torch.arange(T, device=d)[:, None] % 7
+    o = mhk.expert_order(e, 7)
+    xs = mhk.dispatch(y.detach(), o)
+    assert torch.equal(xs[o.place[-3:, 0].long()], y[-3:])
+    assert torch.equal(mhk.combine(xs, None, o)[-3:], y[-3:])
+
+
 def test_expert_dense_with_offsets_out_of_range_stays_inside():
     """Contents of the offsets never lead out of the tensors: the call ends, and rows inside its groups are theirs."""
     d = dev()
