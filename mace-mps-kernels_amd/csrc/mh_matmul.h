@@ -815,8 +815,9 @@ __device__ __forceinline__ void mm_store_lines(const tile_t& t, mh_u4* lds, long
             if (m < rows) {
                 const long long at = (r0 + m) * N + left + c;
                 *reinterpret_cast<mh_u4*>(C + at) = *reinterpret_cast<const mh_u4*>(y + r * LD + c);
-                if (ACT != MM_NONE && slope)
-                    *reinterpret_cast<mh_u4*>(slope + at) = *reinterpret_cast<const mh_u4*>(d + r * LD + c);
+                if (ACT != MM_NONE && slope)             // not read before the backward: past the caches
+                    __builtin_nontemporal_store(*reinterpret_cast<const mh_u4*>(d + r * LD + c),
+                                                reinterpret_cast<mh_u4*>(slope + at));
             }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
