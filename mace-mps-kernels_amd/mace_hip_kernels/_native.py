@@ -179,6 +179,27 @@ def load():
     return _lib
 
 
+_layers = None
+PLAN_FORWARD, PLAN_BACKWARD, PLAN_ROUTE, PLAN_NORM = range(4)        # _layers.so's kinds of plan: dense layers, routing, norms
+PLANNERS = [None] * 4
+
+
+def layers():
+    """The trainable layers' host side, ``_layers.so`` (csrc/mh_layers.cpp), loaded once."""
+    global _layers
+    if _layers is None:
+        load()
+        try:
+            from . import _layers as module
+        except ImportError as e:
+            raise RuntimeError(f'mace_hip_kernels: _layers.so is missing or stale ({e}); build it with '
+                               '__graft_entry__.build()') from e
+        module.set_planner(lambda kind, *key: PLANNERS[kind](*key))
+        module.set_timed(launch if timing.active is not None else None)
+        _layers = module
+    return _layers
+
+
 def check(rc, what=''):
     if rc != 0:
         msg = load().mh_last_error().decode(errors='replace')
@@ -278,12 +299,16 @@ class timing:
 
     def __enter__(self):
         timing.active = self
+        if _layers is not None:
+            _layers.set_timed(launch)
         self._was = load().mh_launch_log(1)
         launch_log_take()
         return self
 
     def __exit__(self, *exc):
         timing.active = None
+        if _layers is not None:
+            _layers.set_timed(None)
         load().mh_launch_log(self._was)
 
     def summary(self):

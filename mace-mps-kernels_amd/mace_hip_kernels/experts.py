@@ -13,10 +13,9 @@ results, so all of it is bitwise repeatable.  The reference has no counterpart (
 import torch
 
 from . import _native
-from .matmul import DOUBLE_BACKWARD, TYPES, check_like, check_rows, rows_of
+from .matmul import TYPES, DTYPES, planner, refused, check_like, check_rows, handle
 
 MAX_EXPERTS = 1024
-SHARE = 4096             # assignments per workgroup of the sort
 
 
 class ExpertOrder:
@@ -64,105 +63,32 @@ def module(device, dtype=None):
     return m
 
 
-def _lanes(C, dtype):
-    """log2 of the lanes that share a row: one 16-byte access each, a wave at most."""
+@planner(_native.PLAN_ROUTE)
+def _plan(device, dtype, C, *_):
+    """[module, log2 of the lanes that share a row: one 16-byte access each, a wave at most]; the sort's for no type."""
+    device = torch.device('cuda', device)
+    if dtype < 0:
+        return [handle(module(device)), 0]
+    dtype = DTYPES[dtype]
     vectors = -(-C * dtype.itemsize // 16)
-    return min(6, max(0, (vectors - 1).bit_length()))
+    return [handle(module(device, dtype)), min(6, max(0, (vectors - 1).bit_length()))]
 
 
 def expert_order(experts, n_experts):
     """The places of assignments ``experts`` [T, k] (int32 or int64 on the GPU) in a stable sort by expert; values outside
     [0, n_experts) are dropped (a router marks what exceeds an expert's capacity with -1).  n_experts up to 1024."""
-    if not torch.is_tensor(experts) or experts.dtype not in (torch.int32, torch.int64):
-        raise TypeError('experts must be an int32 or int64 tensor')
-    if not experts.is_cuda:
-        raise TypeError(f'mace_hip_kernels: experts must be a GPU tensor, got one on {experts.device}')
-    if experts.dim() != 2 or experts.shape[1] < 1:
-        raise ValueError(f'experts must be [T, k] with k >= 1, got {list(experts.shape)}')
-    if not 1 <= n_experts <= MAX_EXPERTS:
-        raise ValueError(f'n_experts must be between 1 and {MAX_EXPERTS}, got {n_experts}')
-    A = experts.numel()
-    if A >= 2 ** 31 - 2 ** 21:
-        raise ValueError(f'too many assignments for one launch: {A}')
-    e = experts.contiguous()
-    blocks = max(1, min(512, -(-A // SHARE)))
-    buf = torch.empty(n_experts + 1 + 2 * A + (blocks * (n_experts + 1) if blocks > 1 else 0), dtype=torch.int32,
-                      device=e.device)
-    offsets, rows = buf[:n_experts + 1], buf[n_experts + 1:n_experts + 1 + A]
-    place, hist = buf[n_experts + 1 + A:n_experts + 1 + 2 * A], buf[n_experts + 1 + 2 * A:]
-    P = _native.ptr
-    _native.launch('expert_order', _native.load().mh_expert_order, module(e.device).handle, P(e),
-                   int(e.dtype == torch.int64), A, n_experts, P(hist) if blocks > 1 else None, blocks, P(offsets), P(rows),
-                   P(place), _native.stream_of(e))
-    return ExpertOrder(offsets, rows, place.view(experts.shape), n_experts)
-
-
-def _spread(x, order):
-    """x [T, C] to its places [T k, C]."""
-    T, k = order.place.shape
-    C = x.shape[-1]
-    x2, ld = rows_of(x, C)
-    y = torch.empty(T * k, C, device=x.device, dtype=x.dtype)
-    P = _native.ptr
-    if T and C:
-        _native.launch('ex_dispatch', _native.load().mh_dispatch, module(x.device, x.dtype).handle, P(x2), ld, P(order.place),
-                       P(order.offsets), P(y), T, k, C, order.n_experts, _lanes(C, x.dtype), _native.stream_of(x2))
-    return y
-
-
-def _gather(y, w, order, res):
-    """res + sum_j w y[place] [T, C]."""
-    T, k = order.place.shape
-    C = y.shape[-1]
-    out = torch.empty(T, C, device=y.device, dtype=y.dtype)
-    P = _native.ptr
-    if T and C:
-        y2 = y.contiguous()
-        r, ldr = (None, 0) if res is None else rows_of(res, C)
-        _native.launch('ex_combine', _native.load().mh_combine, module(y.device, y.dtype).handle, P(y2), P(w), P(order.place),
-                       P(r), ldr, P(out), T, k, C, _lanes(C, y.dtype), _native.stream_of(y2))
-    return out
-
-
-class _DispatchFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, order):
-        ctx.order = order
-        return _spread(x, order)
-
-    @staticmethod
-    def backward(ctx, g):
-        if torch.is_grad_enabled():
-            raise RuntimeError(DOUBLE_BACKWARD)
-        return _gather(g, None, ctx.order, None), None
-
-
-class _CombineFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, y, w, res, order):
-        ctx.order = order
-        w2 = None if w is None else w.contiguous()
-        ctx.save_for_backward(y if w is not None and ctx.needs_input_grad[1] else None, w2)
-        return _gather(y, w2, order, res)
-
-    @staticmethod
-    def backward(ctx, g):
-        if torch.is_grad_enabled():
-            raise RuntimeError(DOUBLE_BACKWARD)
-        y, w = ctx.saved_tensors
-        order = ctx.order
-        T, k = order.place.shape
-        C = g.shape[-1]
-        g2, ldg = rows_of(g, C)
-        dy = torch.empty(T * k, C, device=g.device, dtype=g.dtype) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(T, k, device=g.device, dtype=torch.float32) if ctx.needs_input_grad[1] else None
-        P = _native.ptr
-        if T and (dw is not None or (C and dy is not None)):
-            y2 = None if dw is None else y.contiguous()
-            _native.launch('ex_combine_bwd', _native.load().mh_combine_bwd, module(g.device, g.dtype).handle, P(g2), ldg, P(y2),
-                           P(w), P(order.place), P(order.offsets), P(dy), P(dw), T, k, C, order.n_experts,
-                           _lanes(C, g.dtype), _native.stream_of(g2))
-        return dy, dw, g if ctx.needs_input_grad[2] else None, None
+    out = _native.layers().expert_order(experts, n_experts)
+    if out is None:
+        if not torch.is_tensor(experts) or experts.dtype not in (torch.int32, torch.int64):
+            raise TypeError('experts must be an int32 or int64 tensor')
+        if not experts.is_cuda:
+            raise TypeError(f'mace_hip_kernels: experts must be a GPU tensor, got one on {experts.device}')
+        if experts.dim() != 2 or experts.shape[1] < 1:
+            raise ValueError(f'experts must be [T, k] with k >= 1, got {list(experts.shape)}')
+        if not 1 <= n_experts <= MAX_EXPERTS:
+            raise ValueError(f'n_experts must be between 1 and {MAX_EXPERTS}, got {n_experts}')
+        raise ValueError(f'too many assignments for one launch: {experts.numel()}')
+    return ExpertOrder(*out, n_experts)
 
 
 def _check_order(order, device):
@@ -175,33 +101,38 @@ def _check_order(order, device):
 def dispatch(x, order):
     """The rows of x [T, C] at their places [T k, C] (x[t] at place[t, j] for every kept j); the places behind the last kept
     one are zero rows.  Backward: dx[t] = sum over the kept j of the gradient at place[t, j]."""
-    check_rows('x', x)
-    _check_order(order, x.device)
-    if x.dim() != 2 or x.shape[0] != order.place.shape[0]:
-        raise ValueError(f'x must be [{order.place.shape[0]}, C], got {list(x.shape)}')
-    if torch.is_grad_enabled() and x.requires_grad:
-        return _DispatchFn.apply(x, order)
-    return _spread(x, order)
+    y = _native.layers().dispatch(x, order.place, order.offsets) if isinstance(order, ExpertOrder) else None
+    if y is None:
+        check_rows('x', x)
+        _check_order(order, x.device)
+        if x.dim() != 2 or x.shape[0] != order.place.shape[0]:
+            raise ValueError(f'x must be [{order.place.shape[0]}, C], got {list(x.shape)}')
+        raise refused('dispatch')
+    return y
 
 
 def combine(y, weights, order, residual=None):
     """residual[t] + sum over the kept j of weights[t, j] y[place[t, j]] for rows y [T k, C] in expert order; weights [T, k]
     float32 or of y's type (None: 1), residual [T, C].  Dropped assignments are not read, whatever their weight.  A node
     without any kept one comes out as its residual (or zeros).  Backward to all three (dropped weights get 0)."""
-    check_rows('y', y)
-    _check_order(order, y.device)
-    T, k = order.place.shape
-    if y.dim() != 2 or y.shape[0] != T * k:
-        raise ValueError(f'y must be [{T * k}, C], got {list(y.shape)}')
-    if weights is not None:
-        if not torch.is_tensor(weights) or weights.dtype not in (torch.float32, y.dtype) or weights.device != y.device:
-            raise TypeError(f'weights must be float32 or {y.dtype} on {y.device}')
-        if weights.shape != (T, k):
-            raise ValueError(f'weights must be [{T}, {k}], got {list(weights.shape)}')
-        weights = weights.float()
-    if residual is not None:
-        check_like('residual', residual, y, (T, y.shape[1]))
-    if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return _CombineFn.apply(y, weights, residual, order)
-    return _gather(y, None if weights is None else weights.contiguous(), order, residual)
+    out = None
+    if isinstance(order, ExpertOrder):
+        out = _native.layers().combine(y, weights, residual, order.place, order.offsets)
+    if out is None:
+        check_rows('y', y)
+        _check_order(order, y.device)
+        T, k = order.place.shape
+        if y.dim() != 2 or y.shape[0] != T * k:
+            raise ValueError(f'y must be [{T * k}, C], got {list(y.shape)}')
+        if weights is not None:
+            if not torch.is_tensor(weights) or weights.dtype not in (torch.float32, y.dtype) or weights.device != y.device:
+                raise TypeError(f'weights must be float32 or {y.dtype} on {y.device}')
+            if weights.shape != (T, k):
+                raise ValueError(f'weights must be [{T}, {k}], got {list(weights.shape)}')
+            weights = weights.float()
+        if residual is not None:
+            check_like('residual', residual, y, (T, y.shape[1]))
+        out = _native.layers().combine(y, weights, residual, order.place, order.offsets)
+        if out is None:
+            raise refused('combine')
+    return out

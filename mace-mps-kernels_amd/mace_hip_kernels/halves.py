@@ -60,65 +60,3 @@ def module(device, mode, act=0):
                                          _native.MH_HV_COLUMNS: ('hv_columns', 256, 1)})
         kind = _native.MH_HV_OUTER if mode == 'dw' else _native.MH_HV_MM
         return _native.Module(code, {kind: (f'hv_{mode}', 64 * TILE[0] * TILE[1], SIDE, SIDE)})
-
-
-def _up(n, to):
-    return -(-n // to) * to
-
-
-def split_rows(x, ld, R, K):
-    """(halves, peaks) of R rows of K values."""
-    y = torch.empty(R * 2 * _up(K, 32), device=x.device, dtype=torch.uint16)
-    peak = torch.empty(R, device=x.device, dtype=torch.int32)
-    P = _native.ptr
-    _native.launch('hv_rows', _native.load().mh_hv_rows, module(x.device, 'split').handle, P(x), ld, P(y), P(peak), R, K,
-                   _native.stream_of(x))
-    return y, peak
-
-
-def split_columns(x, ld, R, C, groups, offsets=None):
-    """(halves, peaks and marks [2, groups, C]) of the columns of R rows, scaled per group of rows: by offsets, else equal
-    groups."""
-    y = torch.empty(R * 2 * _up(C, 8), device=x.device, dtype=torch.uint16)
-    peak = torch.zeros(2, groups, C, device=x.device, dtype=torch.int32)
-    G = R // groups if offsets is None else 0
-    # pieces of rows for about eight workgroups per compute unit
-    L = min(256, max(16, _up(-(-R * -(-C // 256) // 2048), 4)))
-    slots = groups * -(-G // L) if offsets is None else -(-R // L) + groups
-    P = _native.ptr
-    _native.launch('hv_columns', _native.load().mh_hv_columns, module(x.device, 'split').handle, P(x), ld, P(y), P(peak),
-                   P(offsets), R, C, groups, G, L, slots, _native.stream_of(x))
-    return y, peak
-
-
-def product(x, ld, weight, bias, res, ldr, act, slope, offsets, groups, out):
-    """out [R, n] = act(x weight^T + bias) + res (slope: act' there where given)."""
-    R, K = x.shape
-    n = out.shape[1]
-    xh, xp = split_rows(x, ld, R, K)
-    wh, wp = split_rows(weight, K, groups * n, K)
-    P = _native.ptr
-    _native.launch('hv_fwd', _native.load().mh_hv_mm, module(x.device, 'fwd', act).handle, P(xh), P(wh), P(out), P(bias),
-                   P(res), ldr, P(slope), P(offsets), P(xp), P(wp), None, R, n, K, groups, _native.stream_of(x))
-
-
-def input_gradient(p, ldp, weight, offsets, groups, out):
-    """out [R, K] = p weight per group, p [R, N], weight [groups, N, K]."""
-    R, N = p.shape
-    K = out.shape[-1]
-    ph, pp = split_rows(p, ldp, R, N)
-    wh, wp = split_columns(weight, K, groups * N, K, groups)
-    P = _native.ptr
-    _native.launch('hv_dx', _native.load().mh_hv_mm, module(p.device, 'dx').handle, P(ph), P(wh), P(out), None, None, 0,
-                   None, P(offsets), P(pp), P(wp[0]), P(wp[1]), R, K, N, groups, _native.stream_of(p))
-
-
-def weight_gradient(p, ldp, x, ldx, offsets, groups, out, part, L, slots):
-    """out [groups, N, K] (or its parts, where L) = p^T x per group, p [R, N], x [R, K]."""
-    R, N = p.shape
-    K = x.shape[1]
-    ph, pp = split_columns(p, ldp, R, N, groups, offsets)
-    xh, xp = split_columns(x, ldx, R, K, groups, offsets)
-    P = _native.ptr
-    _native.launch('hv_dw', _native.load().mh_hv_outer, module(p.device, 'dw').handle, P(ph), P(xh), P(out), P(part),
-                   P(offsets), P(pp[0]), P(pp[1]), P(xp[0]), P(xp[1]), R, N, K, groups, L, slots, _native.stream_of(p))

@@ -13,7 +13,6 @@ float32 accuracy (operands split into three bf16 parts, six partial products; la
 halves, ``halves``); 16-bit operands run as they are; every sum is float32 and rounded once.  The backward keeps act'(a) of the forward, not a itself.  Sums over rows that are split over
 workgroups are added in a fixed order, so results are bitwise repeatable.  The reference has no such layers.
 """
-import functools
 import math
 
 import torch
@@ -21,6 +20,7 @@ import torch
 from . import _native, halves
 
 TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+DTYPES = {v: k for k, v in TYPES.items()}
 ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
 # Tiles: waves (rows x columns), 16 x 16 fragments per wave (rows x columns), k per LDS buffer.  Operands of float32 and of
@@ -126,27 +126,6 @@ def module(device, dtype, mode, tile=None, act=0):
     return m
 
 
-def rows_of(t, width):
-    """``t`` [..., width] as rows [R, width] whose elements are contiguous (copied only where they are not), and the
-    distance between rows."""
-    if t.dim() != 2:
-        t = t.reshape(-1, width) if width else t.reshape(t.shape[:-1].numel(), 0)
-    if t.shape[0] <= 1 or width == 0:
-        return t.contiguous(), width
-    if (width > 1 and t.stride(1) != 1) or t.stride(0) < width:
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-def _aligned(t, ld, width):
-    """Whether rows of a 16-bit tensor are whole steps of 16 bytes, with a tile's offsets within 2^31 bytes."""
-    return width % 8 == 0 and ld % 8 == 0 and t.data_ptr() % 16 == 0 and ld < 2 ** 21
-
-
-def _up8(n):
-    return -(-n // 8) * 8
-
-
 def _seconds(tile, dtype, tiles, depth, longest=0):
     """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` on average, ``longest`` at most."""
     bm, bn = tile_shape(tile, dtype)
@@ -210,36 +189,47 @@ def _padding_pays(flops, slow, moved, copies):
     return flops * (1 / slow - 1 / 850) * 1e-12 > 1.2 * (moved / 4.5e12 + 5e-6 * copies)
 
 
-def _pad(t, ld, rows, width):
-    """(rows copied to whole steps of 16 bytes with zeros behind them, their distance)."""
-    to = _up8(width)
-    y = torch.empty((rows, to), device=t.device, dtype=t.dtype)
-    _native.launch('mm_pad', _native.load().mh_mm_pad, module(t.device, t.dtype, 'sum').handle, t.data_ptr(), ld, y.data_ptr(),
-                   rows, width, to, _native.stream_of(t))
-    return y, to
+def handle(m):
+    """A module's handle as a number (0: none), for plans."""
+    return 0 if m is None else m.handle.value
 
 
-# What a call's sizes lead to, kept by the sizes: modules are looked up and shapes chosen once per size, not per call.
-@functools.lru_cache(maxsize=4096)
-def _fwd_plan(device, dtype, R, n, K, groups, act, x_ok, w_ok):
-    """(module, None: by halves; whether x and the weight are copied first)."""
+def planner(kind):
+    """Makes a function ``_layers.so``'s planner of a kind.  It keeps the numbers by the arguments; ``cache_clear()`` has it ask
+    again."""
+    def register(fn):
+        _native.PLANNERS[kind] = fn
+        fn.cache_clear = lambda: _native.layers().clear_plans()
+        return fn
+    return register
+
+
+@planner(_native.PLAN_FORWARD)
+def _fwd_plan(device, dtype, R, n, K, groups, act, x_ok, w_ok, *_):
+    """[module, whether by halves, modules of the halves and of the copies, whether x and the weight are copied first to whole
+    steps of 16 bytes]; x_ok, w_ok: whether they come in such."""
+    device, dtype = torch.device('cuda', device), DTYPES[dtype]
     if dtype == torch.float32 and halves.pays(R, n, K, groups, 'fwd'):
-        return None, False, False
+        return [handle(halves.module(device, 'fwd', act)), 1, handle(halves.module(device, 'split')), 0, 0, 0]
     few = _few_tile(R, groups)
     if few:
-        return module(device, dtype, 'fwd', few, act), False, False
+        return [handle(module(device, dtype, 'fwd', few, act)), 0, 0, 0, 0, 0]
     fast = pad = dtype.itemsize == 2
     if fast and not (x_ok and w_ok):
         fast = pad = _padding_pays(2.0 * R * n * K, 600, 4 * K * (R * (not x_ok) + groups * n * (not w_ok)),
                                    2 - x_ok - w_ok)
-    return (module(device, dtype, 'fwd', _choose_tile(R, n, K, dtype, groups, fast), act), pad and not x_ok,
-            pad and not w_ok)
+    pads = [pad and not x_ok, pad and not w_ok]
+    return [handle(module(device, dtype, 'fwd', _choose_tile(R, n, K, dtype, groups, fast), act)), 0, 0,
+            handle(module(device, dtype, 'sum') if any(pads) else None), *map(int, pads)]
 
 
-@functools.lru_cache(maxsize=4096)
-def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok, want_x, want_w, want_b):
-    """(modules of the sums, of dx and of dW; rows per piece and pieces of db; of dW; floats of scratch; whether dx and dW go
-    by halves; whether g, the weight and x are copied to whole steps first)."""
+@planner(_native.PLAN_BACKWARD)
+def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok, need, *_):
+    """[modules of the sums, of dx, of dW, of halves; rows per piece and pieces of db; of dW; floats of scratch; whether dx and
+    dW go by halves; whether g, the weight and x are copied to whole steps first].  need: bits of dx, dW, db; made_p: with an
+    activation, whose product g act'(a) comes in whole steps."""
+    device, dtype = torch.device('cuda', device), DTYPES[dtype]
+    want_x, want_w, want_b = (bool(need >> i & 1) for i in range(3))
     some = R > 0 and N > 0 and K > 0
     hx, hw = (want and some and dtype == torch.float32 and halves.pays(R, N, K, groups, mode)
               for want, mode in ((want_x, 'dx'), (want_w, 'dw')))
@@ -259,10 +249,13 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok,
         if not (p_ok and x_ok):
             fast_w = want_w and _padding_pays(flops, 240, 4 * R * (N * (not p_ok) + K * (not x_ok)), 2 - p_ok - x_ok)
     rows = outer = None
-    if want_x and R and K and not hx:
+    if hx:
+        rows = halves.module(device, 'dx')
+    elif want_x and R and K:
         rows = module(device, dtype, 'dx', _choose_tile(R, K, N, dtype, groups, fast_x))
     Lo, slots_o = 0, groups
     if hw:
+        outer = halves.module(device, 'dw')
         Lo, slots_o = _halves_pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE))
     elif want_w and N and K:
         tile, Lo, slots_o = _outer_plan(R, N, K, groups, grouped, dtype, fast_w)
@@ -270,109 +263,9 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok,
     scratch = max(scratch, slots_o * N * K if Lo else 0)
     pads = ((want_x and fast_x or want_w and fast_w) and not p_ok, want_x and fast_x and not w_ok,
             want_w and fast_w and not x_ok)
-    return module(device, dtype, 'sum'), rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw, pads
-
-
-def _product(x, ld, weight, bias, res, act, offsets, groups, keep):
-    """(out [R, n], act' of it or None) of rows x [R, K] and weight [.., n, K]."""
-    R, K = x.shape
-    n = weight.shape[-2]
-    dev, dt = x.device, x.dtype
-    out = torch.empty((R, n), device=dev, dtype=dt)
-    slope = torch.empty((R, n), device=dev, dtype=torch.float32 if dt == torch.float32 else torch.uint16) if keep else None
-    if R and n:
-        m, pad_x, pad_w = _fwd_plan(dev, dt, R, n, K, groups, act, _aligned(x, ld, K), _aligned(weight, K, K))
-        P = _native.ptr
-        r, ldr = (None, 0) if res is None else rows_of(res, n)
-        if m is None:
-            halves.product(x, ld, weight, bias, r, ldr, act, slope, offsets, groups, out)
-            return out, slope
-        ldw = K
-        if pad_x:
-            x, ld = _pad(x, ld, R, K)
-        if pad_w:
-            weight, ldw = _pad(weight, K, groups * n, K)
-        _native.launch('mm_fwd', _native.load().mh_mm_rows, m.handle, P(x), ld, P(weight), max(1, ldw), P(out), P(bias), P(r),
-                       ldr, P(slope), P(offsets), R, n, K, groups, _native.stream_of(x))
-    return out, slope
-
-
-def _backward(g, ldg, slope, weight, x, ldx, offsets, groups, need):
-    """(dx, dW, db) of g [R, N], each where ``need`` says so (weight or x None where what they are for is not)."""
-    R, N = g.shape
-    K = (x if weight is None else weight).shape[-1] if weight is not None or x is not None else 0
-    want_x, want_w, want_b = need
-    dev, dt, P = g.device, g.dtype, _native.ptr
-    made = slope is not None
-    sums, rows, outer, Ls, slots, Lo, slots_o, scratch, hx, hw, (pad_g, pad_w, pad_x) = _bwd_plan(
-        dev, dt, R, N, K, groups, offsets is not None, made, made or _aligned(g, ldg, N),
-        weight is not None and _aligned(weight, K, K), x is not None and _aligned(x, ldx, K), want_x, want_w, want_b)
-    p, ldp, ldw = None, 0, max(1, K)
-    if made:
-        ldp = _up8(N) if dt != torch.float32 else N
-        p = torch.empty((R, ldp), device=dev, dtype=dt)
-    elif pad_g:
-        g, ldg = _pad(g, ldg, R, N)
-    if pad_w:
-        weight, ldw = _pad(weight, K, groups * N, K)
-    if pad_x:
-        x, ldx = _pad(x, ldx, R, K)
-    dx = torch.empty((R, K), device=dev, dtype=dt) if want_x else None
-    dw = torch.empty((groups, N, K), device=dev, dtype=dt) if want_w else None
-    db = torch.empty((groups, N), device=dev, dtype=dt) if want_b else None
-    part = torch.empty(scratch, device=dev, dtype=torch.float32) if scratch else None
-    if made or want_b or rows is not None or outer is not None:
-        _native.launch('mm_bwd', _native.load().mh_mm_bwd, sums.handle, None if rows is None else rows.handle,
-                       None if outer is None else outer.handle, P(g), ldg, P(slope), P(weight), ldw, P(x), ldx, P(offsets),
-                       P(p), ldp, P(dx) if rows is not None else None, P(dw) if outer is not None else None, P(db), P(part), R,
-                       N, K, groups, Ls, slots, Lo, slots_o, _native.stream_of(g))
-    if hx or hw:
-        if made:
-            g, ldg = p, N
-        if hx:
-            halves.input_gradient(g, ldg, weight, offsets, groups, dx)
-        if hw:
-            halves.weight_gradient(g, ldg, x, ldx, offsets, groups, dw, part, Lo, slots_o)
-            if Lo:
-                _native.launch('mm_sum', _native.load().mh_mm_sum, sums.handle, P(part), P(dw), P(offsets), R, groups, Lo,
-                               N * K, _native.stream_of(g))
-    return dx, dw, db
-
-
-DOUBLE_BACKWARD = ('mace_hip_kernels: double backward (create_graph=True) is not available for the trainable node layers '
-                   '(dense, expert_dense, dispatch, combine, block_norm)')
-
-
-class _DenseFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, res, act, offsets):
-        need = ctx.needs_input_grad
-        K = weight.shape[-1]
-        groups = weight.shape[0] if offsets is not None else 1
-        x2, ld = rows_of(x, K)
-        weight = weight.contiguous()
-        out, slope = _product(x2, ld, weight, None if bias is None else bias.contiguous(), res, act, offsets, groups,
-                              act != 0 and (need[0] or need[1] or need[2]))
-        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, slope, offsets)
-        ctx.sizes = x.shape, weight.shape, None if bias is None else bias.shape
-        return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])
-
-    @staticmethod
-    def backward(ctx, g):
-        if torch.is_grad_enabled():          # only true under create_graph=True
-            raise RuntimeError(DOUBLE_BACKWARD)
-        x, weight, slope, offsets = ctx.saved_tensors
-        xs, ws, bs = ctx.sizes
-        need = ctx.needs_input_grad
-        dx = dw = db = None
-        if need[0] or need[1] or need[2]:
-            g2, ldg = rows_of(g, ws[-2])
-            x2, ldx = (None, 0) if x is None else rows_of(x, ws[-1])
-            dx, dw, db = _backward(g2, ldg, slope, weight, x2, ldx, offsets, ws[0] if offsets is not None else 1, need[:3])
-            dx = None if dx is None else dx.view(xs)
-            dw = None if dw is None else dw.view(ws)
-            db = None if db is None else db.view(bs)
-        return dx, dw, db, g if need[3] else None, None, None
+    return [handle(module(device, dtype, 'sum')), handle(rows), handle(outer),
+            handle(halves.module(device, 'split') if hx or hw else None), Ls, slots, Lo, slots_o, scratch, int(hx), int(hw),
+            *map(int, pads)]
 
 
 def check_like(name, t, x, shape=None):
@@ -397,7 +290,7 @@ def check_rows(name, x):
         raise ValueError(f'{name} is too large for one launch: {list(x.shape)}')
 
 
-def _checked(x, weight, bias, activation, residual, lead):
+def _check(x, weight, bias, activation, residual, lead):
     check_rows('x', x)
     check_like('weight', weight, x)
     if weight.dim() != 2 + len(lead) or weight.shape[-1] != x.shape[-1]:
@@ -409,17 +302,10 @@ def _checked(x, weight, bias, activation, residual, lead):
         check_like('residual', residual, x, (*x.shape[:-1], n))
     if activation not in ACTIVATIONS:
         raise ValueError(f'activation must be one of {list(ACTIVATIONS)}, got {activation!r}')
-    return ACTIVATIONS[activation]
 
 
-def _run(x, weight, bias, residual, act, offsets):
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        return _DenseFn.apply(x, weight, bias, residual, act, offsets)
-    x2, ld = rows_of(x, weight.shape[-1])
-    out, _ = _product(x2, ld, weight.contiguous(), None if bias is None else bias.contiguous(), residual, act, offsets,
-                      weight.shape[0] if offsets is not None else 1, False)
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], out.shape[1])
+def refused(name):
+    return RuntimeError(f'mace_hip_kernels: {name} did not take its arguments')
 
 
 def dense(x, weight, bias=None, activation=None, residual=None):
@@ -427,7 +313,11 @@ def dense(x, weight, bias=None, activation=None, residual=None):
     (float32, bfloat16 or float16) on one GPU; activation None, 'relu', 'silu' or 'gelu' (by erf).  Sums are float32, the
     result is rounded once.  Infinite and NaN values act as in a float32 sum.  x and residual may be rows of a wider
     tensor (any distance between rows); other strides are copied.  First-order backward to all four tensors."""
-    return _run(x, weight, bias, residual, _checked(x, weight, bias, activation, residual, ()), None)
+    y = _native.layers().dense(x, weight, bias, residual, ACTIVATIONS.get(activation, -1), None)
+    if y is None:
+        _check(x, weight, bias, activation, residual, ())
+        raise refused('dense')
+    return y
 
 
 def expert_dense(x, weight, offsets, bias=None, activation=None, residual=None):
@@ -435,12 +325,17 @@ def expert_dense(x, weight, offsets, bias=None, activation=None, residual=None):
     [E, N, K], bias [E, N], offsets [E + 1] int32 on the GPU, not decreasing, as ``expert_order`` gives them).  Empty groups
     are fine (their weights' gradients are zero); rows of no group come out as zeros and get zero gradients.  The offsets
     are not read back: contents outside [0, R] give wrong rows, no error."""
-    act = _checked(x, weight, bias, activation, residual, ('E',))
-    if x.dim() != 2:
-        raise ValueError(f'x must be rows [R, K], got {list(x.shape)}')
-    E = weight.shape[0]
-    if not torch.is_tensor(offsets) or offsets.dtype != torch.int32 or offsets.device != x.device:
-        raise TypeError(f'offsets must be an int32 tensor on {x.device}')
-    if E < 1 or tuple(offsets.shape) != (E + 1,):
-        raise ValueError(f'offsets must be [{E + 1}] for {E} weights (at least one), got {list(offsets.shape)}')
-    return _run(x, weight, bias, residual, act, offsets.contiguous())
+    y = None
+    if torch.is_tensor(offsets):
+        y = _native.layers().dense(x, weight, bias, residual, ACTIVATIONS.get(activation, -1), offsets)
+    if y is None:
+        _check(x, weight, bias, activation, residual, ('E',))
+        if x.dim() != 2:
+            raise ValueError(f'x must be rows [R, K], got {list(x.shape)}')
+        E = weight.shape[0]
+        if not torch.is_tensor(offsets) or offsets.dtype != torch.int32 or offsets.device != x.device:
+            raise TypeError(f'offsets must be an int32 tensor on {x.device}')
+        if E < 1 or tuple(offsets.shape) != (E + 1,):
+            raise ValueError(f'offsets must be [{E + 1}] for {E} weights (at least one), got {list(offsets.shape)}')
+        raise refused('expert_dense')
+    return y

@@ -12,9 +12,10 @@ tensor once and gives the gradients of all of them; its sums over rows are added
 import torch
 
 from . import _native
-from .matmul import CUS, DOUBLE_BACKWARD, TYPES, check_like, check_rows, module as mm_module
+from .matmul import CUS, TYPES, DTYPES, planner, refused, check_like, check_rows, handle, module as mm_module
 
 MAX_CHANNELS = 8192
+KINDS = {'rms': 0, 'layer': 1}
 
 
 def shape(C, dtype):
@@ -68,60 +69,16 @@ def module(device, dtype, tpr, nv, layer, branch, gate):
     return m
 
 
-def _forward(x, y, gate, scale, wp, wn, eps, layer, gmode, keep):
-    C = x.shape[-1]
-    T = x.numel() // C if C else 0
-    n = torch.empty_like(x)
-    h = x if y is None else torch.empty_like(x)
-    stats = torch.empty(T, 4, device=x.device, dtype=torch.float32) if keep else None
-    if T:
-        tpr, nv = shape(C, x.dtype)
-        P = _native.ptr
-        _native.launch('nm_fwd', _native.load().mh_norm_fwd,
-                       module(x.device, x.dtype, tpr, nv, layer, y is not None, gmode).handle, P(x), P(y), P(gate), P(scale),
-                       P(wp), P(wn), None if y is None else P(h), P(n), P(stats), T, C, eps, _native.stream_of(x))
-    return h, n, stats
+@planner(_native.PLAN_NORM)
+def _plan(device, dtype, T, C, layer, branch, gate, *_):
+    """[module, module of the sums, workgroups of the backward]."""
+    device, dtype = torch.device('cuda', device), DTYPES[dtype]
+    tpr, nv = shape(C, dtype)
+    return [handle(module(device, dtype, tpr, nv, bool(layer), bool(branch), gate)), handle(mm_module(device, dtype, 'sum')),
+            _backward_blocks(T, tpr)]
 
 
-class _BlockNormFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, y, gate, scale, wp, wn, eps, layer, gmode):
-        h, n, stats = _forward(x, y, gate, scale, wp, wn, eps, layer, gmode, True)
-        ctx.save_for_backward(x, y, gate, scale, wp, wn, stats)
-        ctx.args = layer, gmode
-        ctx.set_materialize_grads(False)
-        return n if y is None else (h, n)
-
-    @staticmethod
-    def backward(ctx, *grads):
-        if torch.is_grad_enabled():          # only true under create_graph=True
-            raise RuntimeError(DOUBLE_BACKWARD)
-        x, y, gate, scale, wp, wn, stats = ctx.saved_tensors
-        layer, gmode = ctx.args
-        need = ctx.needs_input_grad
-        gh, gn = (None, grads[0]) if y is None else grads
-        if gh is None and gn is None:
-            return (None,) * 9
-        gh, gn = (None if g is None else g.contiguous() for g in (gh, gn))
-        C = x.shape[-1]
-        T = x.numel() // C if C else 0
-        dev, dt, P, lib = x.device, x.dtype, _native.ptr, _native.load()
-        dx, dy, dgate = (torch.empty_like(t) if w else None for t, w in zip((x, y, gate), need[:3]))
-        dsum = torch.empty((3, C), device=dev, dtype=dt) if any(need[3:6]) else None
-        tpr, nv = shape(C, dt)
-        blocks = _backward_blocks(T, tpr)
-        part = None if dsum is None else torch.empty((blocks, 3, C), device=dev, dtype=torch.float32)
-        _native.launch('nm_bwd', lib.mh_norm_bwd, module(dev, dt, tpr, nv, layer, y is not None, gmode).handle,
-                       mm_module(dev, dt, 'sum').handle, P(gh), P(gn), P(x), P(y), P(gate), P(scale), P(wp), P(wn), P(stats),
-                       P(dx), P(dy), P(dgate), P(part), P(dsum), T, C, blocks, _native.stream_of(x))
-        return (dx, dy, dgate, *(dsum[i] if w else None for i, w in enumerate(need[3:6])), None, None, None)
-
-
-def block_norm(x, y=None, gate=None, scale=None, post_weight=None, pre_weight=None, eps=1e-6, kind='rms'):
-    """(h, n): h = x + scale gate norm(y) post_weight and n = norm(h) pre_weight, per row of x [..., C] (y None: h is x and
-    gate, scale and post_weight must be None).  y [..., C]; gate [..., C] or [..., 1]; the weights [C], each 1 where None;
-    all of one type (float32, bfloat16 or float16).  kind 'rms' or 'layer' (the mean subtracted first).  n is formed from h
-    before h is rounded to the type.  C up to 8192.  First-order backward to every tensor given."""
+def _check(x, y, gate, scale, post_weight, pre_weight, eps, kind):
     check_rows('x', x)
     C = x.shape[-1]
     if not 1 <= C <= MAX_CHANNELS:
@@ -130,24 +87,27 @@ def block_norm(x, y=None, gate=None, scale=None, post_weight=None, pre_weight=No
         raise ValueError(f"kind must be 'rms' or 'layer', got {kind!r}")
     if not eps >= 0:
         raise ValueError(f'eps must not be negative, got {eps}')
-    gmode = 0
     if y is None:
         if gate is not None or scale is not None or post_weight is not None:
             raise ValueError('gate, scale and post_weight belong to a branch y')
     else:
         check_like('y', y, x, x.shape)
     if gate is not None:
-        # [..., 1] is one value a row, also where there is one channel
         check_like('gate', gate, x)
         if gate.shape[:-1] != x.shape[:-1] or gate.dim() != x.dim() or gate.shape[-1] not in (1, C):
             raise ValueError(f'gate must be {[*x.shape[:-1], C]} or {[*x.shape[:-1], 1]}, got {list(gate.shape)}')
-        gmode = 1 if gate.shape[-1] == 1 else 2
     for name, w in (('scale', scale), ('post_weight', post_weight), ('pre_weight', pre_weight)):
         if w is not None:
             check_like(name, w, x, (C,))
-    ts = [None if t is None else t.contiguous() for t in (x, y, gate, scale, post_weight, pre_weight)]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
-        out = _BlockNormFn.apply(*ts, float(eps), kind == 'layer', gmode)
-        return (x, out) if y is None else out
-    h, n, _ = _forward(*ts, float(eps), kind == 'layer', gmode, False)
-    return (x if y is None else h), n
+
+
+def block_norm(x, y=None, gate=None, scale=None, post_weight=None, pre_weight=None, eps=1e-6, kind='rms'):
+    """(h, n): h = x + scale gate norm(y) post_weight and n = norm(h) pre_weight, per row of x [..., C] (y None: h is x and
+    gate, scale and post_weight must be None).  y [..., C]; gate [..., C] or [..., 1]; the weights [C], each 1 where None;
+    all of one type (float32, bfloat16 or float16).  kind 'rms' or 'layer' (the mean subtracted first).  n is formed from h
+    before h is rounded to the type.  C up to 8192.  First-order backward to every tensor given."""
+    out = _native.layers().block_norm(x, y, gate, scale, post_weight, pre_weight, eps, KINDS.get(kind, -1))
+    if out is None:
+        _check(x, y, gate, scale, post_weight, pre_weight, eps, kind)
+        raise refused('block_norm')
+    return out

@@ -11,7 +11,7 @@ import pytest
 import torch
 
 import mace_hip_kernels as mhk
-from mace_hip_kernels import halves, matmul, norms
+from mace_hip_kernels import _native, halves, matmul, norms
 
 pytestmark = pytest.mark.gpu
 
@@ -766,3 +766,43 @@ def test_refusals_on_the_gpu():
         with pytest.raises(kind, match=text):
             call()
     assert set(matmul.TYPES) == {F32, BF16, F16}
+
+
+@pytest.mark.parametrize('dt', [F32, BF16], ids=['f32', 'bf16'])
+def test_gradients_at_odd_places(dt):
+    """A gradient in rows of a wider tensor, off the steps of 16 bytes that its width promises, against the same copied."""
+    d = dev()
+    rng = np.random.default_rng(77)
+    x, w, b = (rand(rng, *s, dt=dt).to(d).requires_grad_() for s in ((300, 64), (72, 64), (72,)))
+    wide = rand(rng, 300, 83, dt=dt).to(d)
+    for act in (None, 'silu'):
+        y = mhk.dense(x, w, b, act)
+        for g in (wide[:, 3:75], wide[:, :72]):
+            print(f'[case] gradient at odd places {dt} {act}', flush=True)
+            a = torch.autograd.grad(y, (x, w, b), g, retain_graph=True)
+            c = torch.autograd.grad(y, (x, w, b), g.contiguous(), retain_graph=True)
+            for name, s, t in zip(('dx', 'dw', 'db'), a, c):
+                r = (s.double() - t.double()).norm() / t.double().norm()
+                assert r <= 8 * {F32: 2 ** -24, BF16: 2 ** -8}[dt], (name, act, float(r))
+
+
+def test_launches_are_timed_in_both_directions():
+    d = dev()
+    x, w = torch.randn(40, 32, device=d, requires_grad=True), torch.randn(24, 32, device=d, requires_grad=True)
+    with _native.timing() as tm:
+        mhk.block_norm(mhk.dense(x, w))[1].sum().backward()
+    seen = tm.summary()
+    assert {'mm_fwd', 'nm_fwd', 'nm_bwd', 'mm_bwd'} <= set(seen), seen
+    assert 'mm_fwd' in tm.symbols['mm_fwd'] and 'mm_dx' in tm.symbols['mm_bwd'], tm.symbols
+    n = len(tm.records)
+    mhk.dense(x, w).sum().backward()
+    assert len(tm.records) == n
+
+
+def test_a_tensor_that_changed_its_shape_is_refused():
+    d = dev()
+    x, w = torch.randn(40, 32, device=d, requires_grad=True), torch.randn(24, 32, device=d, requires_grad=True)
+    y = mhk.dense(x, w)
+    x.data = torch.randn(8, 32, device=d)
+    with pytest.raises(RuntimeError, match='changed its shape|Expected'):
+        y.sum().backward()
