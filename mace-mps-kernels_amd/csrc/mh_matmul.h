@@ -400,16 +400,17 @@ __device__ __forceinline__ mh_f4 mm_mfma(mh_u4 a, mh_u4 b, mh_f4 c) {
 
 // The sums of one workgroup's tile over k in [kbeg, kend): WM x WN waves, each FM x FN fragments of 16 x 16.  B's fragment
 // is the instruction's first operand, so that a lane ends with four consecutive n (4 (lane / 16) + j) of one m
-// (lane % 16) and stores them at once.  BUFS LDS buffers; the loads of the next tile are in flight during a tile's
-// products.
-template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK, int BUFS>
+// (lane % 16) and stores them at once.  The next tile's loads to registers are in flight during a tile's products; one buffer of
+// LDS, because a second one costs workgroups their place (bfloat16, 64 x 64, dw of 8,001 x 1,023 x 2,049 in pieces: 145 us
+// with one, 208 with two).
+template <int TY, bool AS, bool BS, int WM, int WN, int FM, int FN, int BK>
 struct mm_tile {
     typedef typename mm_type<TY>::t T;
     static constexpr int THREADS = 64 * WM * WN, BM = 16 * FM * WM, BN = 16 * FN * WN, OPR = BK / 8, ROWS = FM, COLS = FN;
     static constexpr bool WHOLE_STEPS = false;
     static constexpr int PLANES = TY == MM_F32 ? 3 : 1;
     static constexpr int TA = PLANES * BM * OPR, TB = PLANES * BN * OPR;      // octets of a buffer
-    static constexpr int LDS = BUFS * (TA + TB);
+    static constexpr int LDS = TA + TB;
     mh_f4 acc[FM][FN];
     mh_f4 low[TY == MM_F32 ? FM : 1][TY == MM_F32 ? FN : 1];                 // the products below hi hi
 
@@ -460,21 +461,19 @@ struct mm_tile {
         la.load(kbeg, kend);
         lb.load(kbeg, kend);
         la.store(lds);
-        lb.store(lds + BUFS * TA);
+        lb.store(lds + TA);
         __syncthreads();
-        int cur = 0;
         for (int k = kbeg; k < kend; k += BK) {
             const bool more = k + BK < kend;
             if (more) {
                 la.load(k + BK, kend);
                 lb.load(k + BK, kend);
             }
-            products(lds + cur * TA, lds + BUFS * TA + cur * TB);
+            products(lds, lds + TA);
             if (!more) break;
-            if (BUFS == 1) __syncthreads();             // one buffer: every wave has read it
-            else cur ^= 1;
-            la.store(lds + cur * TA);
-            lb.store(lds + BUFS * TA + cur * TB);
+            __syncthreads();                            // every wave has read the tile
+            la.store(lds);
+            lb.store(lds + TA);
             __syncthreads();
         }
     }
@@ -531,6 +530,13 @@ __device__ __forceinline__ void mm_read_turned(const unsigned (&at)[2], mh_u2 (&
         : "=&v"(lo[0]), "=&v"(lo[1]), "=&v"(hi[0]), "=&v"(hi[1])
         : "v"(at[0]), "v"(at[1]), "n"(STEP)
         : "memory");
+}
+template <int STEP>
+__device__ __forceinline__ void mm_read_turned(const unsigned (&at)[1], mh_u2 (&lo)[1], mh_u2 (&hi)[1]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
+                 : "=&v"(lo[0]), "=&v"(hi[0])
+                 : "v"(at[0]), "n"(STEP)
+                 : "memory");
 }
 
 template <bool STRIDED, int ROWS, int BK, int THREADS, bool HALVES>

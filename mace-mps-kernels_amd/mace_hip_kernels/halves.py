@@ -11,21 +11,20 @@ import torch
 from . import _native
 
 # waves (rows x columns), 16 x 16 fragments per wave (rows x columns): 128 x 128 a workgroup, two of them on a compute unit
-# (256 x 256 with eight waves measured 167 us where these take 117, at 20,000 x 1,024 x 1,024)
-TILE = 2, 2, 4, 4
+# (with four waves 171 us where these take 166, at 20,000 x 1,024 x 1,024 with the halves' making; 256 x 256 about 220)
+TILE = 2, 4, 4, 2
 SIDE = 128
 
 
-def pays(rows, n, K, groups, mode):
-    """Whether a product of [rows, K] and [groups, n, K] is faster by halves: by its operations at the rate of either path,
-    the bytes of the halves (read and written once by rows, read twice by columns), the launches, and a margin of three tenths.  Measured (us,
-    direct / halves): 20,000 x 1,024 x 1,024 forward 312 / 163, dx 335 / 162, dw 403 / 247; 8,192 x 512 x 2,048 119 / 72, 138 /
-    97, 176 / 130; 2,533 x 512 x 512 forward 10 / 29; 20,000 x 128 x 512 28 / 39, 32 / 46, 40 / 78."""
-    flops = 2.0 * rows * n * K
+def pays(rows, n, K, groups, mode, product, direct):
+    """Whether a product of [rows, K] and [groups, n, K] that takes ``direct`` seconds is faster by halves: by the seconds of
+    the ``product`` of halves itself, the bytes of the halves (read and written once by rows, read twice by columns), the
+    launches, and a margin of a tenth for what these leave out.  Measured (us, direct / halves): 20,000 x 1,024 x 1,024 forward
+    268 / 166, dx 269 / 168, dw 290 / 247; 4,096 x 1,024 x 1,024 52 / 49, 60 / 46, 73 / 82; 8,192 x 512 x 2,048 107 / 72, 113 /
+    91, 126 / 132; 5,000 x 512 x 512 26 / 36, 28 / 28, 41 / 58; 20,000 x 128 x 512 forward 30 / 40."""
     moved = {'fwd': 8 * (rows * K + groups * n * K), 'dx': 8 * rows * n + 12 * groups * n * K,
              'dw': 12 * rows * (n + K)}[mode]
-    direct = flops / (104e12 if mode == 'dw' else 135e12)
-    return 1.3 * (flops / 370e12 + moved / 4.5e12 + (15e-6 if mode == 'dw' else 8e-6)) < direct
+    return 1.1 * (product + moved / 4.5e12 + (15e-6 if mode == 'dw' else 8e-6)) < direct
 
 
 def source(mode, act=0):

@@ -24,24 +24,34 @@ DTYPES = {v: k for k, v in TYPES.items()}
 ACTIVATIONS = {None: 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
 # Tiles: waves (rows x columns), 16 x 16 fragments per wave (rows x columns), k per LDS buffer.  Operands of float32 and of
-# unaligned 16-bit tensors pass through registers (SLOW, also the buffers: float32 keeps three bf16 planes and two
-# accumulators; two buffers, 32 k and a 128 x 128 tile of it all measured slower), 16-bit ones of whole 16-byte steps go
-# straight to LDS (FAST).
+# unaligned 16-bit tensors pass through registers (SLOW), 16-bit ones of whole 16-byte steps go straight to LDS (FAST).
+# Eight waves that share a tile rather than four measured (us): float32 64 x 64 at 1,999 x 515 x 1,021 21 / 27, at 4,096 x 1,024 x
+# 1,024 61 / 72, 128 x 128 there 52 (four: 79); bfloat16 128 x 128 at 16,384 x 1,024 x 2,048 94 / 100, at 1,024 x 1,024 x 1,024
+# 13.8 / 15.7, but 64 x 64 there 8.8 / 8.5.
 SLOW = {
-    'slow128': {2: (2, 2, 4, 4, 64, 2)},
-    'slow64': {4: (2, 2, 2, 2, 64, 1), 2: (2, 2, 2, 2, 64, 2)},
-    'slow32': {4: (2, 2, 1, 1, 64, 1)},
+    'slow128': {4: (2, 4, 4, 2, 64), 2: (2, 4, 4, 2, 64)},
+    'slow64': {4: (4, 2, 1, 2, 64), 2: (2, 2, 2, 2, 64)},
+    'slow32': {4: (2, 2, 1, 1, 64)},
 }
-FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 2, 4, 4, 64), 'fast64': (2, 2, 2, 2, 64)}
-# What the choices between them go by, as measured: workgroups on a compute unit at once, the device's rate in 1e12
-# operations a second with all of those and with one each, and what a round of workgroups costs besides (us, filling the first
-# tile, storing the last).  bfloat16 at 8,192 x 8,192 x 8,192 859 us with 256 and 982 with 128; at 16,384 x 1,024 x 4,096 149,
-# 163 and 234 with 256, 128 and 64; at 8,192 x 2,048 x 512 58, 27 and 28; at 1,024 x 1,024 x 1,024 32, 15 and 11.  float32 with
-# 64 and 32: at 20,000 x 128 x 512 36 and 46, at 2,533 x 512 x 128 21 and 13, at 700 x 1,000 x 900 30 and 23.
+FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 4, 4, 2, 64), 'fast64': (2, 2, 2, 2, 64), 'deep64': (2, 2, 2, 2, 128)}
+# What the choices between them go by, as measured: workgroups on a compute unit at once; what a round of workgroups costs
+# besides the products (us, filling the first tile, storing the last); and for each product the device's rate in 1e12
+# operations a second with all of those and with one each.  In us: bfloat16 at 8,192 x 8,192 x 8,192 859 with 256 and 982 with
+# 128; at 16,384 x 1,024 x 4,096 149, 163 and 234 with 256, 128 and 64; at 8,192 x 2,048 x 512 57, 27 and 28; at 600 x 2,048 x
+# 1,024 22, 17.6 and 13.3 with 128, 64 and deep64, which at 16,384 x 1,024 x 2,048 takes 155 to 64's 124; unaligned at 8,001 x
+# 1,023 x 2,049 87 and 106 with 128 and 64, at 4,001 x 513 x 257 15 and 10.  float32 with 128, 64 and 32: at 20,000 x 1,024 x
+# 1,024 268, 314 and 400, at 20,000 x 128 x 512 32, 30 and 40, at 2,533 x 512 x 128 28, 10.9 and 9.4.
 SPEED = {
-    2: {'fast256': (1, 1280, 1280, 10), 'fast128': (2, 1120, 780, 5), 'fast64': (4, 740, 350, 3),
-        'slow128': (2, 800, 480, 5), 'slow64': (4, 620, 300, 3)},
-    4: {'slow64': (3, 150, 70, 3), 'slow32': (6, 110, 38, 2)},
+    2: {'fast256': (1, 10, {'fwd': (1280, 1280), 'dx': (1280, 1280), 'dw': (1280, 1280)}),
+        'fast128': (2, 4, {'fwd': (1190, 820), 'dx': (1190, 820), 'dw': (1000, 700)}),
+        'fast64': (4, 3, {'fwd': (740, 320), 'dx': (740, 320), 'dw': (690, 230)}),
+        'deep64': (2, 3, {'fwd': (650, 420), 'dx': (650, 420), 'dw': (650, 310)}),
+        'slow128': (2, 5, {'fwd': (620, 500), 'dx': (500, 330), 'dw': (470, 320)}),
+        'slow64': (4, 3, {'fwd': (380, 220), 'dx': (350, 140), 'dw': (340, 100)})},
+    4: {'slow128': (1, 5, {'fwd': (181, 181), 'dx': (156, 156), 'dw': (172, 172)}),
+        'slow64': (3, 3, {'fwd': (150, 125), 'dx': (140, 115), 'dw': (125, 85)}),
+        'slow32': (6, 2, {'fwd': (85, 38), 'dx': (85, 38), 'dw': (85, 33)}),
+        'halves': (2, 5, {'fwd': (370, 300), 'dx': (370, 300), 'dw': (370, 300)})},
 }
 # few rows (forward): 16-row fragments, and the waves that share the contraction
 FEW = {'few16': (1, 4), 'few32': (2, 4), 'few64': (4, 4)}
@@ -56,6 +66,8 @@ def _tile(tile, dtype):
 
 def tile_shape(tile, dtype):
     """(rows, columns) of a tile."""
+    if tile == 'halves':
+        return halves.SIDE, halves.SIDE
     if tile in FEW:
         return 16 * FEW[tile][0], 16
     wm, wn, fm, fn = _tile(tile, dtype)[:4]
@@ -126,41 +138,65 @@ def module(device, dtype, mode, tile=None, act=0):
     return m
 
 
-def _seconds(tile, dtype, tiles, depth, longest=0):
+def _seconds(tile, dtype, mode, tiles, depth, longest=0):
     """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` on average, ``longest`` at most."""
     bm, bn = tile_shape(tile, dtype)
-    at_once, full, alone, ramp = SPEED[dtype.itemsize][tile]
-    share = tiles / CUS
+    at_once, ramp, rates = SPEED[dtype.itemsize][tile]
+    full, alone = rates[mode]
+    share = math.ceil(tiles / CUS)                       # of the compute units with most
     work, most = (2e-12 * bm * bn * k * CUS for k in (depth, max(depth, longest)))
     if at_once == 1:                                     # whole rounds
-        return max(max(1, math.ceil(share)) * (work / full + ramp * 1e-6), most / full)
+        return max(max(1, share) * (work / full + ramp * 1e-6), most / full)
     return max(most / alone, share * work / full) + max(1.0, share / at_once) * ramp * 1e-6
 
 
-def _choose_tile(rows, cols, depth, dtype, groups, fast):
-    """The tile that is fastest by _seconds.  Groups end in part of a tile: half a tile each on average."""
-    def tiles(tile):
-        bm, bn = tile_shape(tile, dtype)
-        return (-(-rows // bm) + (min(groups, rows) - 1) // 2) * -(-cols // bn)
-    names = FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]
-    return min(names, key=lambda t: _seconds(t, dtype, tiles(t), depth))
+def _names(dtype, fast):
+    return FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]
 
 
-def _few_tile(rows, groups):
-    """The tile for few rows per group, or None."""
+def _tiles(tile, rows, cols, dtype, groups):
+    """Workgroups of a product of rows in groups.  Groups end in part of a tile: half a tile each on average."""
+    bm, bn = tile_shape(tile, dtype)
+    return max(-(-rows // bm) + (groups - 1) // 2, min(groups, rows)) * -(-cols // bn)
+
+
+def _rows_plan(rows, cols, depth, dtype, groups, fast, mode):
+    """(seconds, tile) of the fastest tile by _seconds, and at least the time of reading the weights."""
+    t, tile = min((_seconds(t, dtype, mode, _tiles(t, rows, cols, dtype, groups), depth), t) for t in _names(dtype, fast))
+    return max(t, min(groups, rows) * cols * depth * dtype.itemsize / 4.5e12 + 3e-6), tile
+
+
+def _choose_tile(rows, cols, depth, dtype, groups, fast, mode):
+    return _rows_plan(rows, cols, depth, dtype, groups, fast, mode)[1]
+
+
+def _few_tile(rows, groups, n, K, dtype, aligned):
+    """The tile for few rows per group (64 at most on average), or None where a tile of rows is faster.  Measured (us, few / a
+    tile) with 1, 16 and 64 rows in each group: bfloat16, one group of 4,096 x 1,024 4.2 / 7.6, 4.8 / 7.6, 8.0 / 7.8; 64 of them
+    105 / 118, 161 / 125, 355 / 166; 16 of 2,546 x 773 29 / 22, 41 / 28, 97 / 38; float32, 64 of 1,024 x 1,024 54 / 56, 69 / 75,
+    164 / 139."""
     per = -(-rows // groups)
-    return next((t for t, (fragments, _) in FEW.items() if per <= 16 * fragments), None)
+    tile = next((t for t, (fragments, _) in FEW.items() if per <= 16 * fragments), None)
+    if tile is None:
+        return None
+    # a workgroup's time on its compute unit, in us: a start, and its steps along K, dearer with more rows; sixteen columns each
+    step = (0.0013 + 0.00005 * per) * (1 if aligned else 1.7) if dtype.itemsize == 2 else 0.0025 + 0.00009 * per
+    share = min(groups, rows) * -(-n // 16) / CUS
+    few = 3e-6 + max(1.0, share) * (0.3 + step * K) * 1e-6
+    # 2 us: what staging a tile costs before the first product; in float32 _seconds is a fifth short for groups of few rows
+    other = _rows_plan(rows, n, K, dtype, groups, dtype.itemsize == 2 and aligned, 'fwd')[0]
+    return tile if few < other * (1.0 if dtype.itemsize == 2 else 1.2) + 2e-6 else None
 
 
-def _outer_plan(R, M, N, groups, grouped, dtype, fast):
-    """(tile, L, slots) of a sum over R rows: whole groups (L 0), or pieces of L rows in ``slots`` slots whose parts are
+def _outer_best(R, M, N, groups, grouped, dtype, fast):
+    """(seconds, tile, L, slots) of a sum over R rows: whole groups (L 0), or pieces of L rows in ``slots`` slots whose parts are
     written and read once more; the fastest by _seconds and those bytes."""
     best = None
-    for tile in FAST if fast else [t for t in SLOW if dtype.itemsize in SLOW[t]]:
+    for tile in _names(dtype, fast):
         bm, bn = tile_shape(tile, dtype)
         tiles = -(-M // bm) * -(-N // bn)
         # the longest group is what the unsplit form waits for: of few groups, taken as two and a half times the mean one
-        t = _seconds(tile, dtype, tiles * groups, R / groups, R / groups * (2.5 if 1 < groups <= 64 else 1.0))
+        t = _seconds(tile, dtype, 'dw', tiles * groups, R / groups, R / groups * (2.5 if 1 < groups <= 64 else 1.0))
         best = min(best or (t, tile, 0, groups), (t, tile, 0, groups))
         for pieces in (2, 4, 8, 16, 32, 64):
             L = -(-max(256, -(-R // pieces)) // 64) * 64
@@ -168,10 +204,14 @@ def _outer_plan(R, M, N, groups, grouped, dtype, fast):
                 break
             slots = -(-R // L) + (groups if grouped else 0)
             filled = -(-R // L) + (groups - 1) // 2
-            t = _seconds(tile, dtype, tiles * filled, L) + filled * M * N * 8 / 4.5e12 + 5e-6
+            t = _seconds(tile, dtype, 'dw', tiles * filled, L) + filled * M * N * 8 / 4.5e12 + 5e-6
             if slots <= 65535 and slots * M * N <= 2 ** 28:
                 best = min(best, (t, tile, L, slots))
-    return best[1:]
+    return best
+
+
+def _outer_plan(*args):
+    return _outer_best(*args)[1:]
 
 
 def _halves_pieces(R, groups, grouped, tiles):
@@ -183,10 +223,26 @@ def _halves_pieces(R, groups, grouped, tiles):
     return L, -(-R // L) + (groups if grouped else 0)
 
 
-def _padding_pays(flops, slow, moved, copies):
-    """Whether copies of ``moved`` bytes (read and written) to whole steps of 16 bytes are worth a fast tile, for a product
-    that runs at ``slow`` 1e12 operations a second through registers (forward about 600, dx 470, dW 240) and at 850 else."""
-    return flops * (1 / slow - 1 / 850) * 1e-12 > 1.2 * (moved / 4.5e12 + 5e-6 * copies)
+def _by_halves(R, N, K, groups, grouped, mode):
+    """Whether a float32 product goes by halves."""
+    f32 = torch.float32
+    if mode == 'dw':
+        L, slots = _halves_pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE))
+        tiles = -(-N // halves.SIDE) * -(-K // halves.SIDE) * slots
+        product = _seconds('halves', f32, mode, tiles, L or R / groups) + (slots * N * K * 8 / 4.5e12 if L else 0.0)
+        direct = _outer_best(R, N, K, groups, grouped, f32, False)[0]
+    else:
+        cols, depth = (N, K) if mode == 'fwd' else (K, N)
+        stored = 4 * R * cols / 4.5e12
+        product = _seconds('halves', f32, mode, _tiles('halves', R, cols, f32, groups), depth) + stored
+        direct = _rows_plan(R, cols, depth, f32, groups, False, mode)[0] + stored
+    return halves.pays(R, N, K, groups, mode, product, direct)
+
+
+def _padding_pays(slow, fast, moved, copies):
+    """Whether copies of ``moved`` bytes (read and written) to whole steps of 16 bytes are worth a fast tile: ``slow`` and
+    ``fast``, the seconds of the best tile of either kind."""
+    return slow - fast > 1.2 * (moved / 4.5e12 + 5e-6 * copies)
 
 
 def handle(m):
@@ -209,17 +265,17 @@ def _fwd_plan(device, dtype, R, n, K, groups, act, x_ok, w_ok, *_):
     """[module, whether by halves, modules of the halves and of the copies, whether x and the weight are copied first to whole
     steps of 16 bytes]; x_ok, w_ok: whether they come in such."""
     device, dtype = torch.device('cuda', device), DTYPES[dtype]
-    if dtype == torch.float32 and halves.pays(R, n, K, groups, 'fwd'):
+    if dtype == torch.float32 and R > 0 and _by_halves(R, n, K, groups, False, 'fwd'):
         return [handle(halves.module(device, 'fwd', act)), 1, handle(halves.module(device, 'split')), 0, 0, 0]
-    few = _few_tile(R, groups)
+    few = _few_tile(R, groups, n, K, dtype, bool(x_ok and w_ok))
     if few:
         return [handle(module(device, dtype, 'fwd', few, act)), 0, 0, 0, 0, 0]
     fast = pad = dtype.itemsize == 2
     if fast and not (x_ok and w_ok):
-        fast = pad = _padding_pays(2.0 * R * n * K, 600, 4 * K * (R * (not x_ok) + groups * n * (not w_ok)),
-                                   2 - x_ok - w_ok)
+        slow, quick = (_rows_plan(R, n, K, dtype, groups, q, 'fwd')[0] for q in (False, True))
+        fast = pad = _padding_pays(slow, quick, 4 * K * (R * (not x_ok) + groups * n * (not w_ok)), 2 - x_ok - w_ok)
     pads = [pad and not x_ok, pad and not w_ok]
-    return [handle(module(device, dtype, 'fwd', _choose_tile(R, n, K, dtype, groups, fast), act)), 0, 0,
+    return [handle(module(device, dtype, 'fwd', _choose_tile(R, n, K, dtype, groups, fast, 'fwd'), act)), 0, 0,
             handle(module(device, dtype, 'sum') if any(pads) else None), *map(int, pads)]
 
 
@@ -231,7 +287,7 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok,
     device, dtype = torch.device('cuda', device), DTYPES[dtype]
     want_x, want_w, want_b = (bool(need >> i & 1) for i in range(3))
     some = R > 0 and N > 0 and K > 0
-    hx, hw = (want and some and dtype == torch.float32 and halves.pays(R, N, K, groups, mode)
+    hx, hw = (want and some and dtype == torch.float32 and _by_halves(R, N, K, groups, grouped, mode)
               for want, mode in ((want_x, 'dx'), (want_w, 'dw')))
     # db: pieces of rows for about eight workgroups per compute unit (two / four / eight / sixteen: 100 / 100 / 69 / 73 us at
     # 16,384 x 4,096 bfloat16, 84 / 55 / 41 / 48 at 2,048 in eight groups); few rows are one piece that needs no second sum
@@ -242,17 +298,17 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok,
     p_ok = made_p or g_ok
     fast_x = fast_w = dtype.itemsize == 2 and some
     if fast_x:
-        flops = 2.0 * R * N * K
         if not (p_ok and w_ok):
-            fast_x = want_x and _padding_pays(flops, 470, 4 * (R * N * (not p_ok) + groups * N * K * (not w_ok)),
-                                              2 - p_ok - w_ok)
+            fast_x = want_x and _padding_pays(*(_rows_plan(R, K, N, dtype, groups, q, 'dx')[0] for q in (False, True)),
+                                              4 * (R * N * (not p_ok) + groups * N * K * (not w_ok)), 2 - p_ok - w_ok)
         if not (p_ok and x_ok):
-            fast_w = want_w and _padding_pays(flops, 240, 4 * R * (N * (not p_ok) + K * (not x_ok)), 2 - p_ok - x_ok)
+            fast_w = want_w and _padding_pays(*(_outer_best(R, N, K, groups, grouped, dtype, q)[0] for q in (False, True)),
+                                              4 * R * (N * (not p_ok) + K * (not x_ok)), 2 - p_ok - x_ok)
     rows = outer = None
     if hx:
         rows = halves.module(device, 'dx')
     elif want_x and R and K:
-        rows = module(device, dtype, 'dx', _choose_tile(R, K, N, dtype, groups, fast_x))
+        rows = module(device, dtype, 'dx', _choose_tile(R, K, N, dtype, groups, fast_x, 'dx'))
     Lo, slots_o = 0, groups
     if hw:
         outer = halves.module(device, 'dw')
