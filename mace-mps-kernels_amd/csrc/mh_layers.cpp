@@ -380,6 +380,14 @@ PlanPtr route_plan(const Tensor& t, int64_t C) {
     return plan(Key{{ROUTE, t.device().index(), type_of(t), C}}, R_SIZE);
 }
 
+// a tensor of its own on part of `buf`'s memory (a view by the dispatcher costs 0.8 us, of a call of 6)
+Tensor part_of(const Tensor& buf, int64_t first, c10::IntArrayRef shape) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(buf.storage()), buf.key_set(), buf.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(first);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(shape);
+    return t;
+}
+
 py::object expert_order(py::handle e_, int64_t E) {
     Tensor e;
     if (!tensor(e_, &e) || !e.is_cuda() || (e.scalar_type() != at::kInt && e.scalar_type() != at::kLong) || e.dim() != 2 ||
@@ -396,7 +404,7 @@ py::object expert_order(py::handle e_, int64_t E) {
         return mh_expert_order(p->module(R_MODULE), ptr(e), e.scalar_type() == at::kLong, A, E,
                                blocks > 1 ? d + E + 1 + 2 * A : nullptr, blocks, d, d + E + 1, d + E + 1 + A, stream_of(e));
     });
-    return py::make_tuple(buf.narrow(0, 0, E + 1), buf.narrow(0, E + 1, A), buf.narrow(0, E + 1 + A, A).view(e.sizes()));
+    return py::make_tuple(part_of(buf, 0, {E + 1}), part_of(buf, E + 1, {A}), part_of(buf, E + 1 + A, e.sizes()));
 }
 
 // x [T, C] to its places [T k, C]
