@@ -1099,11 +1099,10 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
             if (slope_) {
                 mh_u4 d = {0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int j = 0; j < 3; ++j)
-                    if (j < c) {
-                        if constexpr (TY == MM_F32) d[j] = static_cast<const unsigned*>(slope_)[at + j];
-                        else d[j / 2] |= (unsigned)static_cast<const unsigned short*>(slope_)[at + j] << (16 * (j & 1));
-                    }
+                for (int j = 0; j < 4; ++j) {            // behind the row: v is zero there, and the slope too
+                    if constexpr (TY == MM_F32) d[j] = j < c ? static_cast<const unsigned*>(slope_)[at + j] : 0u;
+                    else d[j / 2] |= (j < c ? static_cast<const unsigned short*>(slope_)[at + j] : 16384u) << (16 * (j & 1));
+                }
                 v = times(v, d);
             }
             if (P) mm_put4<TY>(P + r * ldp + n, v, (int)min((long long)4, ldp - n));

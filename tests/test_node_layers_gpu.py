@@ -806,3 +806,21 @@ def test_a_tensor_that_changed_its_shape_is_refused():
     x.data = torch.randn(8, 32, device=d)
     with pytest.raises(RuntimeError, match='changed its shape|Expected'):
         y.sum().backward()
+
+
+@pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('N', [64, 51])
+def test_slopes_of_nan_stay_in_their_rows(N, dt):
+    """A NaN input makes its own row's output and gradient NaN, the others keep the values they have without it."""
+    d = dev()
+    rng = np.random.default_rng(N)
+    x, w, g = rand(rng, 70, 40, dt=dt).to(d), rand(rng, N, 40, dt=dt).to(d), rand(rng, 70, N, dt=dt).to(d)
+    bad = x.clone()
+    bad[3, 7] = float('nan')
+    for act in ('silu', 'gelu'):
+        print(f'[case] NaN slopes {dt} N={N} {act}', flush=True)
+        (y, dx), (z, dz) = ((o, torch.autograd.grad(o, i, g)[0]) for i in (x.clone().requires_grad_(), bad.clone().requires_grad_())
+                            for o in (mhk.dense(i, w, None, act),))
+        keep = torch.arange(70, device=d) != 3
+        assert z[3].isnan().all() and dz[3].isnan().all(), act
+        assert torch.equal(y[keep], z[keep]) and torch.equal(dx[keep], dz[keep]) and dx.isfinite().all(), act
