@@ -10,8 +10,10 @@
 // A row's values stay in registers between the sums that they need (one read of each input), all sums are float32.
 #pragma once
 
-// A row of up to TPR NV V values, thread l holding vectors l, l + TPR, ...; TPR 64: a wave (four rows a workgroup), more: the
-// workgroup.
+// A row of up to TPR NV V values, thread l holding vectors l, l + TPR, ...; TPR up to 64: a part of a wave (256 / TPR rows a
+// workgroup), more: the workgroup.
+__device__ constexpr int nm_waves(int tpr) { return tpr > MH_WAVE ? tpr / MH_WAVE : 1; }
+__device__ constexpr int nm_rows(int tpr) { return tpr > MH_WAVE ? 1 : 256 / tpr; }
 template <int TY, int TPR, int NV>
 struct nm_row {
     typedef typename mm_type<TY>::t T;
@@ -52,9 +54,9 @@ struct nm_row {
 // The row's sums of a and b, to every thread of it.  `slot` alternates between two LDS places from call to call, so one
 // barrier per call is enough.
 template <int TPR>
-__device__ __forceinline__ void nm_sum2(float& a, float& b, float (*ws)[2][TPR / MH_WAVE], int slot) {
+__device__ __forceinline__ void nm_sum2(float& a, float& b, float (*ws)[2][nm_waves(TPR)], int slot) {
 #pragma unroll
-    for (int d = 1; d < MH_WAVE; d <<= 1) {
+    for (int d = 1; d < (TPR < MH_WAVE ? TPR : MH_WAVE); d <<= 1) {
         a += __shfl_xor(a, d, MH_WAVE);
         b += __shfl_xor(b, d, MH_WAVE);
     }
@@ -76,7 +78,7 @@ __device__ __forceinline__ void nm_sum2(float& a, float& b, float (*ws)[2][TPR /
 
 // mean and 1 / sqrt(var + eps) of a row held in registers; the variance from the differences to the mean
 template <int TY, int TPR, int NV, bool LAYER>
-__device__ __forceinline__ void nm_stats(const nm_row<TY, TPR, NV>& y, int C, int l, float eps, float (*ws)[2][TPR / MH_WAVE], int& slot,
+__device__ __forceinline__ void nm_stats(const nm_row<TY, TPR, NV>& y, int C, int l, float eps, float (*ws)[2][nm_waves(TPR)], int& slot,
                                          float& mean, float& rstd) {
     typedef nm_row<TY, TPR, NV> row;
     float s = 0.f, z = 0.f;
@@ -104,11 +106,11 @@ __device__ __forceinline__ void nm_fwd_body(const void* x_, const void* y_, cons
                                             float eps) {
     typedef nm_row<TY, TPR, NV> row;
     typedef typename mm_type<TY>::t S;
-    __shared__ float ws[2][2][TPR / MH_WAVE];
-    constexpr int PER = TPR > MH_WAVE ? 1 : 4;           // rows of a workgroup
+    __shared__ float ws[2][2][nm_waves(TPR)];
+    constexpr int PER = nm_rows(TPR);                     // rows of a workgroup
     const int l = threadIdx.x % TPR;
     const long long t = (long long)blockIdx.x * PER + threadIdx.x / TPR;
-    if (t >= T) return;                                  // a whole wave or a whole workgroup
+    if (t >= T) return;                                  // all threads of a row
     int slot = 0;
     row h, w;
     float my = 0.f, ry = 0.f, mh, rh;
@@ -172,8 +174,8 @@ __device__ __forceinline__ void nm_bwd_body(const void* gh_, const void* gn_, co
     typedef nm_row<TY, TPR, NV> row;
     typedef nm_raw<TY, TPR, NV> raw;
     typedef typename mm_type<TY>::t S;
-    __shared__ float ws[2][2][TPR / MH_WAVE];
-    constexpr int PER = TPR > MH_WAVE ? 1 : 4;           // rows of a workgroup
+    __shared__ float ws[2][2][nm_waves(TPR)];
+    constexpr int PER = nm_rows(TPR);                     // rows of a workgroup
     const int l = threadIdx.x % TPR, groups = gridDim.x * PER;
     const int me = blockIdx.x * PER + threadIdx.x / TPR;
     int slot = 0;
@@ -282,14 +284,9 @@ __device__ __forceinline__ void nm_bwd_body(const void* gh_, const void* gn_, co
         }
     }
     if (!part) return;
-    row s, o;
-    if (Y) {
-        s = rs.row();
-        o = rp.row();
-    }
     float* p = part + (long long)blockIdx.x * 3 * C;
     if constexpr (PER > 1) {
-        // a workgroup's row groups add up in LDS, in their order
+        // a workgroup's rows add up in LDS, in their order
         __shared__ float sums[2][PER][TPR * NV * row::V];
         const int g = threadIdx.x / TPR;
         row::each(C, l, [&](int i, int j) {
@@ -298,15 +295,25 @@ __device__ __forceinline__ void nm_bwd_body(const void* gh_, const void* gn_, co
             sums[1][g][c] = an.r[i].v[j];
         });
         __syncthreads();
-        if (g) return;
-        row::each(C, l, [&](int i, int j) {
-            const int c = (l + i * TPR) * row::V + j;
-#pragma unroll
+        for (int c = threadIdx.x; c < C; c += 256) {
+            float z = sums[0][0][c], v = sums[1][0][c];
+#pragma unroll 4
             for (int k = 1; k < PER; ++k) {
-                az.r[i].v[j] += sums[0][k][c];
-                an.r[i].v[j] += sums[1][k][c];
+                z += sums[0][k][c];
+                v += sums[1][k][c];
             }
-        });
+            if (Y) {
+                p[c] = wp_ ? z * mm_get<TY>(static_cast<const S*>(wp_) + c) : z;
+                p[C + c] = scale_ ? z * mm_get<TY>(static_cast<const S*>(scale_) + c) : z;
+            }
+            p[2 * C + c] = v;
+        }
+        return;
+    }
+    row s, o;
+    if (Y) {
+        s = rs.row();
+        o = rp.row();
     }
     row::each(C, l, [&](int i, int j) {
         const int c = (l + i * TPR) * row::V + j;

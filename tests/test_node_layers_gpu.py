@@ -824,3 +824,12 @@ def test_slopes_of_nan_stay_in_their_rows(N, dt):
         keep = torch.arange(70, device=d) != 3
         assert z[3].isnan().all() and dz[3].isnan().all(), act
         assert torch.equal(y[keep], z[keep]) and torch.equal(dx[keep], dz[keep]) and dx.isfinite().all(), act
+
+
+@pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+@pytest.mark.parametrize('kind', ['rms', 'layer'])
+@pytest.mark.parametrize('T,C,gate', [(1, 2, 'row'), (65, 16, 'full'), (130, 33, None), (77, 100, 'row'), (1000, 130, 'full'),
+                                      (200, 255, 'row'), (2100, 257, None)])
+def test_block_norm_of_narrow_rows(T, C, gate, kind, dt):
+    """Rows that several to a wave are taken: T that fills no workgroup, C on both sides of each split."""
+    test_block_norm_and_its_gradients(T, C, gate, kind, dt)
