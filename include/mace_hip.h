@@ -726,9 +726,9 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * part [slots, M, N]; mh_mm_sum then adds them: out[e, i] = sum of part[s, i] over e's pieces in order, i < n.  With
  * L = 0 part may be NULL.  Bind MH_MM_OUTER as MH_MM_ROWS, MH_MM_SUM with 1024 threads.
  *
- * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1; zeros from N to ldp <= N + 8) for rows g [R, N], and the sums of p's columns before
- * rounding: over each piece of L rows into part [slots, N], or with one slot of all rows into db [N] (both NULL: none).
- * Rows of no group are left alone.  Bind MH_MM_SLOPE with 256 threads.
+ * mh_mm_slope: p = g act' (p NULL: not stored; slope NULL: act' = 1; zeros from N to ldp <= N + 8) for rows g [R, N], and the
+ * sums of p's columns before rounding: over each piece of L rows into part [slots, N], or with one slot of all rows into db [N]
+ * (both NULL: none).  Rows of no group are left alone.  Bind MH_MM_SLOPE with 256 threads.
  *
  * mh_mm_bwd: the backward of mh_mm_rows 'fwd' in one call, from g [R, N]: p = g act' (scratch [R, N]; NULL with slope NULL),
  * db, dx = p W_e and dW = p^T x per group, each left out where its pointer is NULL.  sums, rows, outer: modules of
@@ -760,9 +760,11 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * mh_norm_fwd: u = norm(y), h = x + scale gate u wp, n = norm(h) wn per row of C; gate, scale, wp, wn NULL: 1 (gate's shape is
  * compiled in); modules without a branch take y, h NULL.  stats [T, 4] float32 (NULL: none) for mh_norm_bwd, which gives dx,
  * dy, dgate and dw [3, C] = the gradients of scale, wp and wn (each may be NULL) from gh and gn (NULL: 0); part [blocks, 3, C]
- * is scratch for the workgroups' sums and sums a module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD as norms.module does. */
+ * is scratch for the workgroups' sums and sums a module of matmul.source 'sum', both for dw.  Bind MH_NORM_FWD and MH_NORM_BWD
+ * as norms.module does. */
 int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, const void* bias,
-               const void* res, int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E, void* stream);
+               const void* res, int64_t ldr, void* slope, const int32_t* offsets, int32_t R, int32_t N, int32_t K, int32_t E,
+               void* stream);
 int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t ldb, void* C, float* part,
                 const int32_t* offsets, int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
 int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,

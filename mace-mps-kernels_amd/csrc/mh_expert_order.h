@@ -27,7 +27,9 @@ extern "C" __global__ __launch_bounds__(1024) void expert_hist(const void* __res
 
 // The places, block b for its `per` assignments (a multiple of EX_CHUNK): where each expert's run starts for this block
 // follows from the blocks' histograms (nb of them; one block counts for itself), then chunks of 1024 are ranked: within a
-// wave by the lanes that hold the same key, found with one ballot per bit of it, across waves by counts in LDS.
+// wave by the lanes that hold the same key, found with one ballot per bit of it, across waves by counts in LDS.  Bound by
+// latency, not by its 12 bytes an assignment: 160 of them 3.7 us in one workgroup, 131,072 with 128 experts 13.6 us in 32 (and
+// 4.9 for their histograms), a chunk of 1,024 about 2.4 us.
 extern "C" __global__ __launch_bounds__(1024) void expert_place(const void* __restrict__ experts, int wide, int A, int E, int per,
                                                                  const int* __restrict__ hist, int* __restrict__ offsets,
                                                                  int* __restrict__ rows, int* __restrict__ place) {

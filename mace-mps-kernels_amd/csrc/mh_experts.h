@@ -16,7 +16,8 @@ __device__ __forceinline__ void ex_zero_tail(typename mm_type<TY>::t* y, const i
 }
 
 // y[place[t, j]] = x[t]: each row of x read once, written to its places past the caches (here and below: a training step's
-// four passes over 32,768 nodes of four rows of 1,024 bfloat16 values took 350 us with ordinary stores, 276 with these)
+// four passes over 32,768 nodes of four rows of 1,024 bfloat16 values took 350 us with ordinary stores, 276 with these).  Bound
+// by its bytes: 63 us there, 5.3 TB/s.
 template <int TY>
 __device__ __forceinline__ void ex_dispatch_body(const void* x_, const int* place, const int* offsets, void* y_, long long ldx,
                                                  int T, int k, int C, int E, int lg) {
@@ -82,7 +83,8 @@ __device__ __forceinline__ void ex_combine_body(const void* y_, const float* w, 
 }
 
 // dy[place[t, j]] = w[t, j] g[t] (dy NULL: not wanted) and dw[t, j] = <g[t], y[place[t, j]]>, 0 where dropped (dw NULL: not
-// wanted), four j at a time: a vector of g is loaded once for the four rows of y and dy, which pass by the caches.
+// wanted), four j at a time: a vector of g is loaded once for the four rows of y and dy, which pass by the caches.  Bound by its
+// bytes: 114 us at 32,768 nodes of four rows of 1,024 bfloat16 values, 5.3 TB/s.
 template <int TY>
 __device__ __forceinline__ void ex_combine_bwd_body(const void* g_, const void* y_, const float* w, const int* place,
                                                     const int* offsets, void* dy_, float* dw, long long ldg, int T, int k, int C,

@@ -211,7 +211,8 @@ Tensor dense_forward(DenseArgs a, const Tensor& like, const Tensor& b, const Ten
     void* s = stream_of(like);
     void* sl = slope ? ptr(*slope) : nullptr;
     if (p[F_HALVES]) {
-        const Halves h = halves_of_rows(p.module(F_SPLIT), a.x, a.ld, R, K), c = halves_of_rows(p.module(F_SPLIT), a.w, K, groups * n, K);
+        const Halves h = halves_of_rows(p.module(F_SPLIT), a.x, a.ld, R, K);
+        const Halves c = halves_of_rows(p.module(F_SPLIT), a.w, K, groups * n, K);
         launch("hv_fwd", [&] {
             return mh_hv_mm(p.module(F_MODULE), u16(h.y), u16(c.y), f32(out), f32(b), f32(r), ldr, static_cast<float*>(sl),
                             i32(off), u32(h.peak), u32(c.peak), nullptr, R, n, K, groups, s);
@@ -306,14 +307,16 @@ struct DenseFn : torch::autograd::Function<DenseFn> {
         }
         mh_module* split = p.module(B_SPLIT);
         if (p[B_DX_HALVES]) {
-            const Halves a = halves_of_rows(split, g, ldg, R, N), c = halves_of_columns(split, w, K, groups * N, K, groups, Tensor());
+            const Halves a = halves_of_rows(split, g, ldg, R, N);
+            const Halves c = halves_of_columns(split, w, K, groups * N, K, groups, Tensor());
             launch("hv_dx", [&] {
                 return mh_hv_mm(p.module(B_ROWS), u16(a.y), u16(c.y), f32(dx), nullptr, nullptr, 0, nullptr, i32(off),
                                 u32(a.peak), u32(c.peak), u32(c.peak) + groups * K, R, K, N, groups, s);
             });
         }
         if (p[B_DW_HALVES]) {
-            const Halves a = halves_of_columns(split, g, ldg, R, N, groups, off), c = halves_of_columns(split, x, ldx, R, K, groups, off);
+            const Halves a = halves_of_columns(split, g, ldg, R, N, groups, off);
+            const Halves c = halves_of_columns(split, x, ldx, R, K, groups, off);
             launch("hv_dw", [&] {
                 return mh_hv_outer(p.module(B_OUTER), u16(a.y), u16(c.y), f32(dw), f32(part), i32(off), u32(a.peak),
                                    u32(a.peak) + groups * N, u32(c.peak), u32(c.peak) + groups * K, R, N, K, groups, p[B_LO],

@@ -534,14 +534,6 @@ __device__ __forceinline__ void mm_read_turned(const unsigned (&at)[2], mh_u2 (&
         : "v"(at[0]), "v"(at[1]), "n"(STEP)
         : "memory");
 }
-template <int STEP>
-__device__ __forceinline__ void mm_read_turned(const unsigned (&at)[1], mh_u2 (&lo)[1], mh_u2 (&hi)[1]) {
-    asm volatile("ds_read_b64_tr_b16 %0, %2\n\tds_read_b64_tr_b16 %1, %2 offset:%3\n\ts_waitcnt lgkmcnt(0)"
-                 : "=&v"(lo[0]), "=&v"(hi[0])
-                 : "v"(at[0]), "n"(STEP)
-                 : "memory");
-}
-
 template <bool STRIDED, int ROWS, int BK, int THREADS, bool HALVES>
 struct mm_mover {
     static constexpr int OPR = BK / 8, ITEMS = ROWS * OPR / THREADS;
@@ -877,7 +869,9 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
 // The forward for few rows: a workgroup takes 16 TM rows of a group and 16 columns, its WAVES waves share the contraction and
 // add their sums through LDS in wave order.  Both operands go from memory to the matrix cores' registers: weights are read
 // once and no tile of rows is worth staging.  Bound by the weights' bytes and by latency: a wave keeps four 128-byte
-// pieces of 16 weight rows in flight.  float32 uses v_mfma_f32_16x16x4_f32 (k in the order 4 q + j of four steps).
+// pieces of 16 weight rows in flight.  One row of 1,024 to 4,096 in bfloat16 takes 4.1 us (8.4 MB, 2 TB/s: two trips to memory
+// and a launch), eight rows of different ones of 64 experts of 1,024 to 2,048 9 us, one row of each of 64 groups of 1,024 to
+// 4,096 105 us (5.1 TB/s).  float32 uses v_mfma_f32_16x16x4_f32 (k in the order 4 q + j of four steps).
 template <int TY, int ACT, int TM, int WAVES>
 __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
                                             void* slope_, const int* off, long long lda, long long ldb, long long ldr, int R, int N,
@@ -978,6 +972,8 @@ __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void
 
 // Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  blockIdx.y is
 // the group (L 0: all its rows; none give zeros), or a slot of at most L of its rows whose sums go to part[slot] in float32.
+// Bound as the other products; 16,384 rows of 4,096 by 1,024 in bfloat16 in four pieces take 140 us and 10 for their sum
+// (980 TFLOP/s), eight groups of 2,048 rows of 2,048 by 1,024 whole 75 us.
 template <int TY, typename tile_t>
 __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, void* C_, float* part, const int* off,
                                               long long lda, long long ldb, int R, int M, int N, int E, int L) {
@@ -1013,7 +1009,8 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
 
 // out[e, i] = sum of part[s, i] over the group's slots in a fixed order: what ends a sum that was split over rows.  2^lg waves
 // share a column's slots (wave w takes every 2^lg-th) and are added in wave order, so that few columns of many slots are
-// not one wave's chain of loads; 1024 threads, four columns a lane.
+// not one wave's chain of loads; 1024 threads, four columns a lane.  Bound by its bytes: 4 slots of 4,096 x 1,024 in 10 us, 512
+// slots of 6,144 columns in 5.
 template <int TY>
 __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const int* off, int R, int E, int L, int lg,
                                             long long n) {
@@ -1050,10 +1047,12 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
     if (c > 0) mm_put4<TY>(static_cast<T*>(out_) + (long long)e * n + i, v, c);
 }
 
-// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1), rows ldp >= N apart with zeros behind N, and the sums of its columns in float32, before
-// rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows, rounded into db (both NULL: none).
-// A workgroup takes a slot and 256 columns, 64 threads of four columns each by four rows at a time.  Bound by its bytes; the
-// slope is read for the last time, past the caches: 69 us at 16,384 x 4,096 bfloat16, 5.8 TB/s (81 as an ordinary read).
+// p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1), rows ldp >= N apart with zeros behind N, and the sums of
+// its columns in float32, before rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows,
+// rounded into db (both NULL: none).  For 16-bit types p is rounded once here, as the matrix products take it: the error of a
+// gradient is then that of a product of rounded operands.  A workgroup takes a slot and 256 columns, 64 threads of four
+// columns each by four rows at a time.  Bound by its bytes; the slope is read for the last time, past the caches: 69 us at
+// 16,384 x 4,096 bfloat16, 5.8 TB/s (81 as an ordinary read).
 template <int TY>
 __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, void* db, const int* off,
                                               long long ldg, long long ldp, int R, int N, int E, int L) {
@@ -1123,7 +1122,8 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
     }
 }
 
-// y [R, Kp] = x [R, K] with zeros behind K: rows of 16-bit values at whole steps of 16 bytes.  A thread copies one step.
+// y [R, Kp] = x [R, K] with zeros behind K: rows of 16-bit values at whole steps of 16 bytes.  A thread copies one step;
+// bound by its bytes, about 4.5 TB/s where they are many.
 template <int TY>
 __device__ __forceinline__ void mm_pad_body(const void* x, void* y, long long ld, int R, int K, int Kp) {
     typedef typename mm_type<TY>::t T;

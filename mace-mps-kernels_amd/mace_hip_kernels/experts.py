@@ -7,8 +7,8 @@ stands a layer with weights per expert (``expert_dense`` over ``order.offsets``)
     rows = dispatch(x, order)                             # [T k, C]; rows of no assignment are zero
     y = combine(rows, weights, order, residual=x)         # x[t] + sum over the kept j of weights[t, j] rows[place[t, j]]
 
-No sizes are read back: T k rows whatever the counts, the kept ones first.  Kernels in ``csrc/mh_expert_order.h`` and ``csrc/mh_experts.h``; no atomics on
-results, so all of it is bitwise repeatable.  The reference has no counterpart (its models mix elements by one-hot weights).
+No sizes are read back: T k rows whatever the counts, the kept ones first.  Kernels in ``csrc/mh_expert_order.h`` and
+``csrc/mh_experts.h``; no atomics on results, so all of it is bitwise repeatable.  The reference has no counterpart (its models mix elements by one-hot weights).
 """
 import torch
 

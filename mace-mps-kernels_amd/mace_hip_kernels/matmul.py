@@ -8,9 +8,11 @@ bfloat16 and float16, for any number of rows from none on and any widths.
     h = expert_dense(rows, weights, order.offsets, biases)                # rows [R, K], weights [E, N, K], biases [E, N]
 
 A drop-in of ``patch_model`` holds its weights as constants; these are what a model trains next to it.  The kernels are in
-``csrc/mh_matmul.h``, one hipRTC module per type, product and tile.  A float32 product runs on the bf16 matrix cores at
-float32 accuracy (operands split into three bf16 parts, six partial products; large ones as three products of float16
-halves, ``halves``); 16-bit operands run as they are; every sum is float32 and rounded once.  The backward keeps act'(a) of the forward, not a itself.  Sums over rows that are split over
+``csrc/mh_matmul.h``, one hipRTC module per type, product and tile; here is what chooses between them by sizes, types and
+alignment, and ``csrc/mh_layers.cpp`` runs them.  A float32 product runs on the bf16 matrix cores at float32 accuracy
+(operands split into three bf16 parts, six partial products; large ones as three products of float16 halves, ``halves``);
+16-bit operands run as they are; every sum is float32 and rounded once.  The backward keeps act'(a) of the forward, not a
+itself, and rounds p = g act'(a) to the type before the products that contract it.  Sums over rows that are split over
 workgroups are added in a fixed order, so results are bitwise repeatable.  The reference has no such layers.
 """
 import math
@@ -36,7 +38,7 @@ SLOW = {
 FAST = {'fast256': (2, 4, 8, 4, 64), 'fast128': (2, 4, 4, 2, 64), 'fast64': (2, 2, 2, 2, 64), 'deep64': (2, 2, 2, 2, 128)}
 # What the choices between them go by, as measured: workgroups on a compute unit at once; what a round of workgroups costs
 # besides the products (us, filling the first tile, storing the last); and for each product the device's rate in 1e12
-# operations a second with all of those and with one each.  In us: bfloat16 at 8,192 x 8,192 x 8,192 859 with 256 and 982 with
+# operations a second with all of those and with one each (and its own cost of a round).  In us: bfloat16 at 8,192 x 8,192 x 8,192 859 with 256 and 982 with
 # 128; at 16,384 x 1,024 x 4,096 149, 163 and 234 with 256, 128 and 64; at 8,192 x 2,048 x 512 57, 27 and 28; at 600 x 2,048 x
 # 1,024 22, 17.6 and 13.3 with 128, 64 and deep64, which at 16,384 x 1,024 x 2,048 takes 155 to 64's 124; unaligned at 8,001 x
 # 1,023 x 2,049 87 and 106 with 128 and 64, at 4,001 x 513 x 257 15 and 10.  float32 with 128, 64 and 32: at 20,000 x 1,024 x
@@ -48,8 +50,8 @@ SPEED = {
         'deep64': (2, 3, {'fwd': (650, 420), 'dx': (650, 420), 'dw': (650, 310)}),
         'slow128': (2, 5, {'fwd': (620, 500), 'dx': (500, 330), 'dw': (470, 320)}),
         'slow64': (4, 3, {'fwd': (380, 220), 'dx': (350, 140), 'dw': (340, 100)})},
-    4: {'slow128': (1, 5, {'fwd': (181, 181), 'dx': (156, 156), 'dw': (172, 172)}),
-        'slow64': (3, 3, {'fwd': (150, 125), 'dx': (140, 115), 'dw': (125, 85)}),
+    4: {'slow128': (1, 5, {'fwd': (181, 181), 'dx': (156, 156), 'dw': (155, 155)}),
+        'slow64': (3, 3, {'fwd': (150, 125), 'dx': (140, 115), 'dw': (125, 85, 6)}),
         'slow32': (6, 2, {'fwd': (85, 38), 'dx': (85, 38), 'dw': (85, 33)}),
         'halves': (2, 5, {'fwd': (370, 300), 'dx': (370, 300), 'dw': (370, 300)})},
 }
@@ -142,9 +144,13 @@ def _seconds(tile, dtype, mode, tiles, depth, longest=0):
     """A product's time by SPEED: ``tiles`` workgroups of a contraction of ``depth`` on average, ``longest`` at most."""
     bm, bn = tile_shape(tile, dtype)
     at_once, ramp, rates = SPEED[dtype.itemsize][tile]
-    full, alone = rates[mode]
-    share = math.ceil(tiles / CUS)                       # of the compute units with most
-    work, most = (2e-12 * bm * bn * k * CUS for k in (depth, max(depth, longest)))
+    full, alone, *own = rates[mode]
+    ramp = own[0] if own else ramp
+    share = tiles / CUS
+    if tile != 'halves':
+        share = math.ceil(share)                         # of the compute units with most
+    # whole steps of 64 along k
+    work, most = (2e-12 * bm * bn * 64 * math.ceil(k / 64) * CUS for k in (depth, max(depth, longest)))
     if at_once == 1:                                     # whole rounds
         return max(max(1, share) * (work / full + ramp * 1e-6), most / full)
     return max(most / alone, share * work / full) + max(1.0, share / at_once) * ramp * 1e-6
