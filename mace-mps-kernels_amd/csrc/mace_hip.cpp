@@ -1211,10 +1211,10 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
 // ---------------------------------------------------------------------------------------------- trainable node layers
 namespace {
 
-// Pieces of at most L rows that R rows in E groups can make, with the rows of no group counted as one group more (no more
-// groups have rows than there are rows).
+// Pieces of at most L rows that R rows in E groups can make, with the rows of no group, before the first one and behind the
+// last, counted as two groups more (no more groups have rows than there are rows).
 int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
-    return (R + L - 1) / L + (offsets ? std::min(E, R) + 1 : 0);
+    return (R + L - 1) / L + (offsets ? std::min(E, R) + 2 : 0);
 }
 
 }  // namespace

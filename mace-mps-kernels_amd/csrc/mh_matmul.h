@@ -214,10 +214,11 @@ __device__ __forceinline__ float mm_slope_value(unsigned c) {
 
 // ------------------------------------------------------------------------------------------------ groups of rows
 // Rows [0, R) in E groups, group e from off[e] to off[e + 1]; each group is cut into pieces of L rows, and slot s is the
-// s-th piece.  False past the last one; rows after the last group then follow as pieces with e = -1.  off NULL: one group
-// of all rows.  Offsets are clamped into [0, R] and to the largest before them, so whatever they hold, groups are disjoint,
-// no piece leads out of the tensors, and there are at most R / L + E of them.  Every lane of a wave calls (64 groups at a
-// time are scanned across it); R + L < 2^31.
+// s-th piece.  False past the last one; the rows of no group then follow as pieces with e = -1, those before the first group
+// and those behind the last.  off NULL: one group of all rows.  Offsets are clamped into [0, R] and to the largest before
+// them, so whatever they hold, groups are disjoint, no piece leads out of the tensors, and there are at most R / L + E
+// of them (R / L + E + 2 with those of no group).  Every lane of a wave calls (64 groups at a time are scanned across it);
+// R + L < 2^31.
 __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int R, int L, int s, int& e, int& r0, int& r1) {
     if (!off) {
         e = 0;
@@ -225,8 +226,8 @@ __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int 
         r1 = min(R, r0 + L);
         return r0 < R;
     }
-    const int lane = threadIdx.x & (MH_WAVE - 1);
-    int base = 0, top = min(max(off[0], 0), R);          // pieces and rows before these 64 groups
+    const int lane = threadIdx.x & (MH_WAVE - 1), lead = min(max(off[0], 0), R);
+    int base = 0, top = lead;                            // pieces and rows before these 64 groups
     for (int g0 = 0; g0 < E; g0 += MH_WAVE) {
         int hi = max(top, min(off[min(g0 + lane, E - 1) + 1], R));
 #pragma unroll
@@ -255,9 +256,14 @@ __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int 
         top = mh_bcast(hi, MH_WAVE - 1);
     }
     e = -1;
-    const long long r = top + (long long)(s - base) * L;
-    r0 = (int)min(r, (long long)R);
-    r1 = min(R, r0 + L);
+    const int d = s - base, first = (lead + L - 1) / L;  // pieces before the first group
+    if (d < first) {
+        r0 = d * L;
+        r1 = min(lead, r0 + L);
+    } else {
+        r0 = (int)min(top + (long long)(d - first) * L, (long long)R);
+        r1 = min(R, r0 + L);
+    }
     return false;
 }
 
@@ -842,7 +848,7 @@ __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, voi
     T* C = static_cast<T*>(C_) + (long long)r0 * N + n0;
     tile_t t;
     if (!live) {
-        // a tail of rows without a group
+        // rows without a group
         for (int i = threadIdx.x; i < rows * min(N - n0, tile_t::BN); i += tile_t::THREADS) {
             const int w = min(N - n0, tile_t::BN);
             C[(long long)(i / w) * N + i % w] = 0;

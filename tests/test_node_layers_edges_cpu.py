@@ -1,0 +1,92 @@
+"""
+The index arithmetic of the trainable node layers' kernels on the CPU: their own functions out of the device headers, compiled
+by g++ with the lanes of a wave as one (MH_WAVE 1), over sizes and contents that no GPU test can hold or should be given.
+"""
+import ctypes
+import os
+import random
+import re
+import shutil
+import subprocess
+
+import numpy as np
+import pytest
+
+from mace_hip_kernels import _native
+
+CSRC = os.path.dirname(_native.DEVICE_HEADER)
+SHIM = """
+#include <algorithm>
+#include <cstdint>
+#include <cstring>
+#include <cstdlib>
+#define __device__
+#define __forceinline__ inline
+#define __restrict__
+#define MH_WAVE 1
+using std::max; using std::min;
+struct dim { unsigned x, y, z; };
+static dim threadIdx, blockIdx, blockDim, gridDim;
+static int __shfl_up(int v, int, int) { return v; }
+static int mh_bcast(int v, int) { return v; }
+static unsigned long long __ballot(bool b) { return b; }
+static int __ffsll(unsigned long long v) { return v ? 1 + __builtin_ctzll(v) : 0; }
+"""
+
+
+def function(header, name):
+    """The text of a function of a device header, its template line and qualifiers included."""
+    with open(os.path.join(CSRC, header)) as f:
+        text = f.read()
+    m = re.search(r'^(template <[^\n]*>\n)?[^\n;]*\b' + name + r'\([^;{]*\{', text, re.M)
+    depth, end = 1, m.end()
+    while depth:
+        depth += {'{': 1, '}': -1}.get(text[end], 0)
+        end += 1
+    return text[m.start():end] + '\n'
+
+
+def host_library(src, tmp_path):
+    c, so = tmp_path / 'part.cpp', tmp_path / 'part.so'
+    c.write_text(SHIM + src)
+    subprocess.run(['g++', '-O1', '-std=c++17', '-shared', '-fPIC', '-w', str(c), '-o', str(so)], check=True)
+    return ctypes.CDLL(str(so))
+
+
+needs_gxx = pytest.mark.skipif(shutil.which('g++') is None, reason='needs g++')
+
+
+@needs_gxx
+def test_slots_cover_every_row_once(tmp_path):
+    """Whatever the offsets hold, the pieces that a launch has room for cover every row once: a group's by its own, the rows
+    before, between and behind the groups by pieces of no group."""
+    lib = host_library(function('mh_matmul.h', 'mm_slot') + function('mace_hip.cpp', 'pieces') + """
+extern "C" long long count(const int* off, long long R, long long E, long long L) { return pieces(off, R, E, L); }
+extern "C" int slot(const int* off, int E, int R, int L, int s, int* out) { return mm_slot(off, E, R, L, s, out[0], out[1], out[2]); }
+""", tmp_path)
+    lib.count.restype, lib.count.argtypes = ctypes.c_longlong, [ctypes.c_void_p] + [ctypes.c_longlong] * 3
+    lib.slot.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+    rng = random.Random(3)
+    for n in range(600):
+        R, E, L = rng.choice([1, 12, 100, 700]), rng.choice([1, 2, 3, 9, 130]), rng.choice([1, 16, 64, 256])
+        if n % 4 == 0:                                   # any contents
+            off = [rng.randint(-5, R + 5) for _ in range(E + 1)]
+        else:
+            off = sorted(rng.randint(0, R) for _ in range(E + 1))
+            off[0] = min(off[0], rng.choice([0, R]))
+        top, of = min(max(off[0], 0), R), np.full(R, -1)
+        for e in range(E):
+            hi = max(top, min(off[e + 1], R))
+            of[top:hi], top = e, hi
+        o, out = np.array(off, dtype=np.int32), np.zeros(3, dtype=np.int32)
+        got, live = np.full(R, -2), True
+        for s in range(lib.count(o.ctypes.data, R, E, L)):
+            is_live = bool(lib.slot(o.ctypes.data, E, R, L, s, out.ctypes.data))
+            assert live or not is_live
+            live = is_live
+            e, r0, r1 = (int(v) for v in out)
+            assert 0 <= r0 <= R and r1 <= R and r1 - r0 <= L and (e >= 0) == live
+            if r0 < R:
+                assert (got[r0:r1] == -2).all()
+                got[r0:r1] = e
+        assert (got == of).all(), (off, R, L)

@@ -1,0 +1,85 @@
+"""
+The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row.
+Tolerances as in the layers' other tests, derived beside each.
+"""
+import numpy as np
+import pytest
+import torch
+
+import mace_hip_kernels as mhk
+from mace_hip_kernels import matmul
+from test_node_layers_gpu import BF16, F16, F32, by_halves, dense_case, dev, near, rand  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+TYPES = pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
+
+
+def poison(*shapes, dt):
+    """Leaves NaN in the memory that the next tensors of these shapes get."""
+    for _ in range(3):
+        kept = [torch.full(s, float('nan'), dtype=dt, device='cuda') for s in shapes for _ in range(3)]
+        del kept
+
+
+# ------------------------------------------------------------------------------------------ rows before the first group
+def _behind_leading_rows(dt, lead=290):
+    """expert_dense over offsets that begin at ``lead``: rows before the first group and behind the last are zero, with zero
+    gradients, and the groups are as ever."""
+    d = dev()
+    rng = np.random.default_rng(lead)
+    R, K, N = lead + 410, 64, 72
+    off = [lead, lead, lead + 210, lead + 350]
+    x, w, b, g = rand(rng, R, K, dt=dt), rand(rng, 3, N, K, dt=dt, scale=K ** -0.5), rand(rng, 3, N, dt=dt), rand(rng, R, N, dt=dt)
+    res = rand(rng, R, N, dt=dt)
+    for rows in (slice(0, lead), slice(off[-1], R)):
+        x[rows], g[rows], res[rows] = float('nan'), float('nan'), float('nan')
+    for act in (None, 'silu'):
+        leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+        poison((R, N), (R, K), dt=dt)
+        y = mhk.expert_dense(*leaves[:2], torch.tensor(off, dtype=torch.int32, device=d), leaves[2], act, res.to(d))
+        poison((R, N), (R, K), dt=dt)
+        grads = torch.autograd.grad(y, leaves, g.to(d))
+        for rows in (slice(0, lead), slice(off[-1], R)):
+            assert (y[rows] == 0).all() and (grads[0][rows] == 0).all(), (act, rows)
+        for e, (i, j) in enumerate(zip(off, off[1:])):
+            want = dense_case(x[i:j], w[e], b[e], act, res[i:j], g[i:j], dt)
+            for name, t in zip(('y', 'dx', 'dw', 'db'), (y[i:j], grads[0][i:j], grads[1][e], grads[2][e])):
+                near(f'{name} of {e}', t, *want[name])
+
+
+@TYPES
+def test_rows_before_the_first_group(dt, monkeypatch):
+    for tile in [*matmul.tiles(dt), *matmul.FEW]:
+        print(f'[case] leading rows, tile {tile} {dt}', flush=True)
+        main = 'slow64' if tile in matmul.FEW else tile
+        monkeypatch.setattr(matmul, '_choose_tile', lambda *a: main)
+        monkeypatch.setattr(matmul, '_outer_plan', lambda R, M, N, groups, grouped, *a: (main, 128, -(-R // 128) + 3 * grouped))
+        monkeypatch.setattr(matmul, '_few_tile', lambda *a: tile if tile in matmul.FEW else None)
+        matmul._fwd_plan.cache_clear()
+        try:
+            _behind_leading_rows(dt)
+        finally:
+            monkeypatch.undo()
+            matmul._fwd_plan.cache_clear()
+
+
+def test_rows_before_the_first_group_by_halves(by_halves):  # noqa: F811
+    print('[case] leading rows by halves', flush=True)
+    _behind_leading_rows(F32)
+
+
+@TYPES
+def test_a_slice_of_the_experts(dt):
+    """The offsets and weights of some of the experts give these experts' rows, by the sizes' own choice of kernels."""
+    d = dev()
+    print(f'[case] a slice of the experts {dt}', flush=True)
+    rng = np.random.default_rng(5)
+    T, E, K, N = 60, 6, 40, 24
+    order = mhk.expert_order(torch.tensor(rng.integers(0, E, (T, 2)), device=d), E)
+    x, w = rand(rng, T, K, dt=dt).to(d), rand(rng, E, N, K, dt=dt).to(d)
+    rows = mhk.dispatch(x, order)
+    whole = mhk.expert_dense(rows, w, order.offsets, activation='relu')
+    poison((2 * T, N), dt=dt)
+    part = mhk.expert_dense(rows, w[2:5], order.offsets[2:6], activation='relu')
+    a, z = order.offsets[2].item(), order.offsets[5].item()
+    assert torch.equal(part[a:z], whole[a:z]) and (part[:a] == 0).all() and (part[z:] == 0).all()
