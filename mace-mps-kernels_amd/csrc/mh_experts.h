@@ -4,15 +4,17 @@
 // the places behind offsets[E] belong to no assignment.
 #pragma once
 
-// A thread group of 2^lg lanes per row; rows past the last group are zeroed by every block in turn.
+// A thread group of 2^lg lanes per row; rows past the last group are zeroed by every block in turn.  A row's number and the
+// step to the next take 64 bits: A, up to 2^31, and the number of thread groups add up to more than 32 hold.
 template <int TY>
 __device__ __forceinline__ void ex_zero_tail(typename mm_type<TY>::t* y, const int* offsets, int E, int A, int C, int lg) {
     typedef mm_vec<TY> vec;
     vec z;
     z.zero();
-    const int tpr = 1 << lg, l = threadIdx.x & (tpr - 1), rpb = blockDim.x >> lg;
-    for (int p = min(max(offsets[E], 0), A) + (int)blockIdx.x * rpb + (threadIdx.x >> lg); p < A; p += gridDim.x * rpb)
-        for (int c = l * vec::V; c < C; c += tpr * vec::V) z.put(y + (long long)p * C + c, C - c);
+    const int tpr = 1 << lg, l = threadIdx.x & (tpr - 1);
+    const long long rpb = blockDim.x >> lg;
+    for (long long p = min(max(offsets[E], 0), A) + blockIdx.x * rpb + (threadIdx.x >> lg); p < A; p += gridDim.x * rpb)
+        for (int c = l * vec::V; c < C; c += tpr * vec::V) z.put(y + p * C + c, C - c);
 }
 
 // y[place[t, j]] = x[t]: each row of x read once, written to its places past the caches (here and below: a training step's

@@ -90,3 +90,39 @@ extern "C" int slot(const int* off, int E, int R, int L, int s, int* out) { retu
                 assert (got[r0:r1] == -2).all()
                 got[r0:r1] = e
         assert (got == of).all(), (off, R, L)
+
+
+@needs_gxx
+def test_rows_behind_the_last_group_are_zeroed_near_the_largest_counts(tmp_path):
+    """The rows past the last kept assignment are each zeroed once, and no other place is written, where their number and that
+    of the workgroups' rows together pass 2^31."""
+    lib = host_library("""
+typedef long long ll;
+static ll seen[1 << 16], n;                               // the places written
+template <int TY> struct mm_type { typedef char t; };
+template <int TY> struct mm_vec {
+    static constexpr int V = 8;
+    void zero() {}
+    void put(char* p, int) { if (n < (1 << 16)) seen[n] = (ll)(uintptr_t)p; ++n; }
+};
+""" + function('mh_experts.h', 'ex_zero_tail') + """
+// rows written by thread `t` of block `b` of a launch of T rows by 2^lg lanes each; the first at most 65,536 in `out`
+extern "C" ll tail(int last, int A, int T, int lg, unsigned b, unsigned t, ll* out) {
+    blockDim.x = 256, blockIdx.x = b, threadIdx.x = t, gridDim.x = (T + (256ll >> lg) - 1) / (256 >> lg), n = 0;
+    ex_zero_tail<0>((char*)0, &last, 0, A, 1, lg);
+    memcpy(out, seen, 8 * std::min(n, (ll)1 << 16));
+    return n;
+}
+""", tmp_path)
+    lib.tail.restype = ctypes.c_longlong
+    lib.tail.argtypes = [ctypes.c_int] * 4 + [ctypes.c_uint] * 2 + [ctypes.c_void_p]
+    out = np.zeros(1 << 16, dtype=np.int64)
+    # one value a row: a lane each; T rows of k assignments, of which the first `last` are kept
+    for T, k in ((1_080_000_000, 1), (2 ** 31 - 2 ** 21 - 1, 1), (700_000_000, 3), (500_000_000, 4), (1000, 2)):
+        A, blocks = T * k, -(-T // 256)
+        for last in (0, A // 2, A - 1000, A - 1, A):
+            for b in sorted({0, 1, blocks // 2, blocks - 2, blocks - 1} & set(range(blocks))):
+                for t in (0, 255):
+                    got = lib.tail(last, A, T, 0, b, t, out.ctypes.data)
+                    want = np.arange(last + b * 256 + t, A, blocks * 256)
+                    assert got == len(want) and (out[:got] == want).all(), (T, k, last, b, t)
