@@ -718,8 +718,9 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * res [R, N] and slope may be NULL.  Rows of no group are zero.  act (none, relu, silu, gelu by erf) is compiled in.  slope [R, N]
  * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types uint16 fixed point (steps of 2^-15
  * from -0.5; 0: NaN).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
- * Modules of a tile in matmul.FAST need every address and row distance to be multiples of 16 bytes and rows padded to such,
- * with zeros in operands whose rows are contracted (mh_mm_pad: y [R, Kp] = x [R, K] and zeros, MH_MM_PAD with 256 threads).
+ * Modules of a tile in matmul.FAST (their kernels' names begin with mm_fast_) need every address and row distance to be
+ * multiples of 16 bytes, row distances below 2^21 values (both are checked) and rows padded to whole steps, with zeros in
+ * operands whose rows are contracted (mh_mm_pad: y [R, Kp] = x [R, K] and zeros, MH_MM_PAD with 256 threads).
  *
  * mh_mm_outer: C[e] [M, N] = sum over the group's rows of A[r, :]^T B[r, :] (A [R, M], B [R, N]; an empty group: zeros).
  * L > 0: the groups' rows are cut into pieces of L, `slots` >= the number of pieces, whose float32 sums go to
@@ -744,7 +745,8 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * rows each (R = E G); pieces of L rows, `slots` >= their number.  Rows of no group are not written.
  * mh_hv_mm: mh_mm_rows from halves: A rows with pa [R]; B rows [E N] with pb [E][N] and mb NULL (C = act(A B^T + bias) +
  * res), or columns of E groups of K rows, length N, with pb and mb [E][N] (C = A B).  mh_hv_outer: mh_mm_outer from columns
- * A (pa, ma [E][M]) and B (pb, mb [E][N]).  All buffers 16-byte aligned.  Bind MH_HV_ROWS, MH_HV_PEAKS and MH_HV_COLUMNS with
+ * A (pa, ma [E][M]) and B (pb, mb [E][N]).  All buffers 16-byte aligned; rows of halves, 2 K values, and columns, M and N,
+ * below 2^21 with their padding.  Bind MH_HV_ROWS, MH_HV_PEAKS and MH_HV_COLUMNS with
  * 256 threads, the others as MH_MM_ROWS.
  *
  * mh_expert_order: the A = T k assignments experts [T, k] (int32, or int64 where wide), values outside [0, E) dropped,

@@ -41,6 +41,7 @@ struct Kernel {
     int groups = 1;                // bytes of dynamic LDS, of which `resident` workgroups fit on the device at once
     int lds = 0;
     int64_t resident = 0;
+    bool steps = false;            // takes operands in whole steps of 16 bytes only (its name begins with mm_fast_)
 };
 
 }  // namespace
@@ -148,7 +149,7 @@ extern "C" {
 
 const char* mh_last_error(void) { return g_err.c_str(); }
 
-int mh_version(void) { return 49; }
+int mh_version(void) { return 50; }
 
 int mh_launch_log(int enable) {
     std::lock_guard<std::mutex> lock(g_log_mu);
@@ -261,6 +262,7 @@ int mh_module_bind_grid(mh_module* m, int kind, const char* name, int block_thre
     m->k[kind].block = block_threads;
     m->k[kind].rows_per_block = rows_per_block;
     m->k[kind].grid_y = grid_y;
+    m->k[kind].steps = m->k[kind].name.compare(0, 8, "mm_fast_") == 0;
     m->k[kind].gfn = nullptr;
     m->k[kind].groups = 1;
     return 0;
@@ -1217,6 +1219,14 @@ int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
     return (R + L - 1) / L + (offsets ? std::min(E, R) + 2 : 0);
 }
 
+// Rows that a tile loads straight to LDS lie fewer values apart than this: it holds the byte offsets of up to 256 rows of 16-bit
+// values in 31 bits, and what lies behind is taken as zero.
+constexpr int64_t kStepsLd = int64_t(1) << 21;
+
+bool whole_steps(const void* p, int64_t ld) {
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ld % 8 == 0 && ld < kStepsLd;
+}
+
 }  // namespace
 
 extern "C" {
@@ -1230,6 +1240,8 @@ int mh_mm_rows(mh_module* m, const void* A, int64_t lda, const void* B, int64_t 
     if (!m || !m->k[MH_MM_ROWS].fn) return fail(-1, "mh_mm_rows: kernel slot not bound in this module");
     const Kernel& k = m->k[MH_MM_ROWS];
     if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_mm_rows: too many rows");
+    if (k.steps && K > 0 && !(whole_steps(A, lda) && whole_steps(B, ldb)))
+        return fail(-1, "mh_mm_rows: this module takes rows in whole steps of 16 bytes, fewer than 2^21 values apart");
     const int64_t tiles = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
     void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &lda, &ldb, &ldr, &R, &N, &K, &E};
     return launch_blocks(m, MH_MM_ROWS, tiles, args, stream, "mh_mm_rows");
@@ -1244,6 +1256,8 @@ int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t
     if (L && (slots < 1 || R > 0x7fffffff - L)) return fail(-1, "mh_mm_outer: bad pieces");
     if (!m || !m->k[MH_MM_OUTER].fn) return fail(-1, "mh_mm_outer: kernel slot not bound in this module");
     const Kernel& k = m->k[MH_MM_OUTER];
+    if (k.steps && R > 0 && !(whole_steps(A, lda) && whole_steps(B, ldb)))
+        return fail(-1, "mh_mm_outer: this module takes rows in whole steps of 16 bytes, fewer than 2^21 values apart");
     const int64_t tiles = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
                           ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
     void* args[] = {&A, &B, &C, &part, &offsets, &lda, &ldb, &R, &M, &N, &E, &L};
@@ -1343,7 +1357,9 @@ int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32
 int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const float* bias, const float* res, int64_t ldr,
              float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
              int32_t N, int32_t K, int32_t E, void* stream) {
-    if (R < 0 || N < 0 || K < 1 || K > 0x3fffffff || E < 1 || (E > 1 && !offsets)) return fail(-1, "mh_hv_mm: bad sizes");
+    // a row of halves is 2 K values long, rounded up; a column operand's is N
+    if (R < 0 || N < 0 || K < 1 || 2LL * K > kStepsLd - 64 || (mb && N > kStepsLd - 8) || E < 1 || (E > 1 && !offsets))
+        return fail(-1, "mh_hv_mm: bad sizes");
     if (R == 0 || N == 0) return 0;
     if (!A || !B || !C || !pa || !pb) return fail(-1, "mh_hv_mm: NULL operand");
     if (res && ldr < N) return fail(-1, "mh_hv_mm: rows overlap (ld below the row's length)");
@@ -1358,8 +1374,8 @@ int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const
 int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, float* part, const int32_t* offsets,
                 const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
                 int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
-    if (R < 1 || R > 0x3fffffff || M < 1 || N < 1 || E < 1 || (E > 1 && !offsets) || L < 0 || (L && slots < 1) ||
-        R > 0x7fffffff - L)
+    if (R < 1 || R > 0x3fffffff || M < 1 || N < 1 || M > kStepsLd - 8 || N > kStepsLd - 8 || E < 1 || (E > 1 && !offsets) ||
+        L < 0 || (L && slots < 1) || R > 0x7fffffff - L)
         return fail(-1, "mh_hv_outer: bad sizes");
     if (!A || !B || !pa || !ma || !pb || !mb || (L ? !part : !C)) return fail(-1, "mh_hv_outer: NULL operand");
     if (!m || !m->k[MH_HV_OUTER].fn) return fail(-1, "mh_hv_outer: kernel slot not bound in this module");

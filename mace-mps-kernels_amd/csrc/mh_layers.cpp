@@ -133,9 +133,12 @@ Tensor rows_of(const Tensor& t, int64_t width, int64_t* ld) {
     return r;
 }
 
+const int64_t kMost = (1LL << 31) - 1024;               // rows, and values of one
+const int64_t kSteps = 1 << 21;                         // values between rows that a tile loads straight to LDS (its 31-bit offsets)
+
 // whether rows of a 16-bit tensor are whole steps of 16 bytes, with a tile's offsets within 2^31 bytes
 bool steps(const Tensor& t, int64_t ld, int64_t width) {
-    return width % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld < (1 << 21);
+    return width % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && ld < kSteps;
 }
 
 int64_t up(int64_t n, int64_t to) { return (n + to - 1) / to * to; }
@@ -147,6 +150,7 @@ enum { B_SUMS, B_ROWS, B_OUTER, B_SPLIT, B_LS, B_SLOTS, B_LO, B_SLOTS_O, B_SCRAT
 
 Tensor padded(mh_module* sums, const Tensor& t, int64_t* ld, int64_t rows, int64_t width) {
     const int64_t to = up(width, 8);
+    TORCH_CHECK(rows < kMost && to < kSteps, "mace_hip_kernels: rows that no tile takes were to be copied for one");
     Tensor y = at::empty({rows, to}, t.options());
     launch("mm_pad", [&] { return mh_mm_pad(sums, ptr(t), *ld, ptr(y), rows, width, to, stream_of(t)); });
     *ld = to;
@@ -339,7 +343,6 @@ bool tensor(py::handle h, Tensor* t) {
 }
 bool maybe(py::handle h, Tensor* t) { return h.is_none() || tensor(h, t); }
 bool alike(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.device() == x.device(); }
-const int64_t kMost = (1LL << 31) - 1024;
 // rows of features that the kernels take
 bool fits(const Tensor& x) {
     return x.is_cuda() && type_of(x) >= 0 && x.dim() >= 1 && x.size(-1) < kMost &&

@@ -32,7 +32,7 @@ MH_CONV_FWD, MH_CONV_BWD, MH_CONV_BWD_WY, MH_SC_FWD, MH_SC_BWD, MH_CONV_BWD_R, M
     MH_EXPERT_PLACE, MH_DISPATCH, MH_COMBINE, MH_COMBINE_BWD, MH_NORM_FWD, MH_NORM_BWD, MH_HV_ROWS, \
     MH_HV_PEAKS, MH_HV_COLUMNS, MH_HV_MM, MH_HV_OUTER, MH_MM_PAD = range(101)
 MH_WANT_GX, MH_WANT_GWY, MH_CUT_MASKED, MH_CUT_NOZERO = 1, 2, 4, 8
-ABI_VERSION = 49
+ABI_VERSION = 50
 
 # hipcc/hipRTC options for every generated layer: gfx950 code, -O3, and packed-FP32 instructions disabled.
 ARCH = os.environ.get('MACE_HIP_ARCH', 'gfx950')

@@ -58,6 +58,8 @@ SPEED = {
 # few rows (forward): 16-row fragments, and the waves that share the contraction
 FEW = {'few16': (1, 4), 'few32': (2, 4), 'few64': (4, 4)}
 CUS = 256                # compute units of an MI355X
+# Rows that a tile may load straight to LDS lie fewer than this many values apart: it holds their byte offsets in 31 bits
+LD_MAX = 2 ** 21
 
 _PTRS = 'const void* A, const void* B, void* C, '
 
@@ -79,6 +81,11 @@ def tile_shape(tile, dtype):
 def tiles(dtype):
     """The tiles of a type for all three products, largest first."""
     return [*(FAST if dtype.itemsize == 2 else ()), *(t for t in SLOW if dtype.itemsize in SLOW[t])]
+
+
+def symbol(mode, tile):
+    """The kernel of a product's module: ``mm_fast_`` where the library is to hold operands to what FAST tiles take."""
+    return f'mm_{"fast_" if tile in FAST else ""}{mode}'
 
 
 def source(dtype, mode, tile=None, act=0):
@@ -108,7 +115,7 @@ def source(dtype, mode, tile=None, act=0):
     b = lambda v: 'true' if v else 'false'  # noqa: E731
     L += [f'typedef mm_{"fast_" if tile in FAST else ""}tile<{ty}, {b(mode == "dw")}, {b(mode != "fwd")}, '
           f'{", ".join(map(str, shape))}> tile_t;']
-    head = f'extern "C" __global__ __launch_bounds__({64 * shape[0] * shape[1]}) void mm_{mode}({_PTRS}'
+    head = f'extern "C" __global__ __launch_bounds__({64 * shape[0] * shape[1]}) void {symbol(mode, tile)}({_PTRS}'
     if mode == 'dw':
         L += [head + 'float* part, const int* off, long long lda, long long ldb, int R, int M, int N, int E, int L) {',
               f'  mm_outer_body<{ty}, tile_t>(A, B, C, part, off, lda, ldb, R, M, N, E, L);', '}']
@@ -135,7 +142,7 @@ def module(device, dtype, mode, tile=None, act=0):
             else:
                 waves = FEW[tile][1] if tile in FEW else _tile(tile, dtype)[0] * _tile(tile, dtype)[1]
                 kind = _native.MH_MM_OUTER if mode == 'dw' else _native.MH_MM_ROWS
-                m = _native.Module(code, {kind: (f'mm_{mode}', 64 * waves, *tile_shape(tile, dtype))})
+                m = _native.Module(code, {kind: (symbol(mode, tile), 64 * waves, *tile_shape(tile, dtype))})
         _MODULES[key] = m
     return m
 
@@ -232,6 +239,8 @@ def _halves_pieces(R, groups, grouped, tiles):
 def _by_halves(R, N, K, groups, grouped, mode):
     """Whether a float32 product goes by halves."""
     f32 = torch.float32
+    if 2 * max(N, K) > LD_MAX - 64 or groups * N >= 2 ** 31:
+        return False
     if mode == 'dw':
         L, slots = _halves_pieces(R, groups, grouped, -(-N // halves.SIDE) * -(-K // halves.SIDE))
         tiles = -(-N // halves.SIDE) * -(-K // halves.SIDE) * slots
@@ -276,7 +285,7 @@ def _fwd_plan(device, dtype, R, n, K, groups, act, x_ok, w_ok, *_):
     few = _few_tile(R, groups, n, K, dtype, bool(x_ok and w_ok))
     if few:
         return [handle(module(device, dtype, 'fwd', few, act)), 0, 0, 0, 0, 0]
-    fast = pad = dtype.itemsize == 2
+    fast = pad = dtype.itemsize == 2 and K <= LD_MAX - 8 and groups * n < 2 ** 31
     if fast and not (x_ok and w_ok):
         slow, quick = (_rows_plan(R, n, K, dtype, groups, q, 'fwd')[0] for q in (False, True))
         fast = pad = _padding_pays(slow, quick, 4 * K * (R * (not x_ok) + groups * n * (not w_ok)), 2 - x_ok - w_ok)
@@ -302,7 +311,7 @@ def _bwd_plan(device, dtype, R, N, K, groups, grouped, made_p, g_ok, w_ok, x_ok,
     slots = max(1, -(-R // Ls)) + (groups if grouped else 0)
     scratch = slots * N if want_b and (grouped or slots > 1) else 0
     p_ok = made_p or g_ok
-    fast_x = fast_w = dtype.itemsize == 2 and some
+    fast_x = fast_w = dtype.itemsize == 2 and some and max(N, K) <= LD_MAX - 8 and groups * N < 2 ** 31
     if fast_x:
         if not (p_ok and w_ok):
             fast_x = want_x and _padding_pays(*(_rows_plan(R, K, N, dtype, groups, q, 'dx')[0] for q in (False, True)),

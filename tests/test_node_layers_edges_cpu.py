@@ -1,8 +1,10 @@
 """
-The index arithmetic of the trainable node layers' kernels on the CPU: their own functions out of the device headers, compiled
-by g++ with the lanes of a wave as one (MH_WAVE 1), over sizes and contents that no GPU test can hold or should be given.
+The index arithmetic of the trainable node layers on the CPU, over sizes and contents that no GPU test can hold or should be
+given: the kernels' own functions out of the device headers, compiled by g++ with the lanes of a wave as one (MH_WAVE 1), and
+the choices of tiles.
 """
 import ctypes
+import itertools
 import os
 import random
 import re
@@ -11,8 +13,9 @@ import subprocess
 
 import numpy as np
 import pytest
+import torch
 
-from mace_hip_kernels import _native
+from mace_hip_kernels import _native, halves, matmul
 
 CSRC = os.path.dirname(_native.DEVICE_HEADER)
 SHIM = """
@@ -126,3 +129,50 @@ extern "C" ll tail(int last, int A, int T, int lg, unsigned b, unsigned t, ll* o
                     got = lib.tail(last, A, T, 0, b, t, out.ctypes.data)
                     want = np.arange(last + b * 256 + t, A, blocks * 256)
                     assert got == len(want) and (out[:got] == want).all(), (T, k, last, b, t)
+
+
+def test_wide_rows_take_tiles_with_64_bit_offsets(monkeypatch):
+    """Rows that are as far apart as a tile straight to LDS cannot address, after copies to whole steps, as the product g act'(a)
+    or as halves, go through registers instead; just below the limit they need not."""
+    # a row's byte offset in the largest of those tiles, its steps included
+    assert max(max(matmul.tile_shape(t, torch.bfloat16)) for t in matmul.FAST) * 2 * matmul.LD_MAX <= 2 ** 30
+    chosen = []
+    monkeypatch.setattr(matmul, 'module', lambda device, dtype, mode, tile=None, act=0: chosen.append((mode, tile)))
+    monkeypatch.setattr(halves, 'module', lambda device, mode, act=0: chosen.append((mode, 'halves')))
+    near = set(matmul.FAST) | {'halves'}
+
+    def tiles(fn, dtype, *args):
+        chosen.clear()
+        numbers = fn(0, matmul.TYPES[dtype], *args)
+        return {t for _, t in chosen if t} & near, numbers
+
+    f32, b16 = torch.float32, torch.bfloat16
+    wide = matmul.LD_MAX
+    for K in (wide - 7, wide, wide + 1, 2 * wide + 1, 8 * wide + 3):
+        for R, n in ((128, 128), (4096, 4096)):
+            for ok in (0, 1):
+                got, numbers = tiles(matmul._fwd_plan, b16, R, n, K, 1, 0, ok and K % 8 == 0 and K < wide, 0)
+                assert not got and not any(numbers[4:]), (R, n, K)
+    for N, K in ((2 * wide + 8, 4096), (wide + 8, 512), (512, wide + 8), (wide - 7, 64)):
+        for made in (0, 1):
+            got, numbers = tiles(matmul._bwd_plan, b16, 4096, N, K, 1, 0, made, made, 0, 0, 7)
+            assert not got and not any(numbers[-3:]), (N, K, made)
+    for mode, N, K in itertools.product(('fwd', 'dx', 'dw'), (2048, wide // 2, 2 * wide + 64), (2048, wide // 2, 2 * wide + 64)):
+        assert max(N, K) == 2048 or not matmul._by_halves(2048, N, K, 1, False, mode)
+    # more rows of weights than a launch counts
+    assert not tiles(matmul._fwd_plan, b16, 10 ** 6, 2 ** 15, 9, 2 ** 16, 0, 0, 0)[0]
+    # below the limits
+    assert tiles(matmul._fwd_plan, b16, 4096, 4096, wide - 8, 1, 0, 1, 1)[0]
+    assert tiles(matmul._bwd_plan, b16, 4096, 4096, 4096, 1, 0, 1, 1, 1, 1, 7)[0]
+    assert all(matmul._by_halves(20000, 1024, 1024, 1, False, mode) for mode in ('fwd', 'dx', 'dw'))
+
+
+def test_the_library_refuses_halves_that_a_tile_cannot_address():
+    lib = _native.load()
+    p = np.zeros(64, dtype=np.float32).ctypes.data
+    wide = matmul.LD_MAX
+    for call in (lambda: lib.mh_hv_mm(None, p, p, p, None, None, 0, None, None, p, p, None, 4, 4, wide // 2, 1, None),
+                 lambda: lib.mh_hv_mm(None, p, p, p, None, None, 0, None, None, p, p, p, 4, wide, 4, 1, None),
+                 lambda: lib.mh_hv_outer(None, p, p, p, None, None, p, p, p, p, 4, wide, 4, 1, 0, 1, None),
+                 lambda: lib.mh_hv_outer(None, p, p, p, None, None, p, p, p, p, 4, 4, wide, 1, 0, 1, None)):
+        assert call() != 0 and 'bad sizes' in lib.mh_last_error().decode()

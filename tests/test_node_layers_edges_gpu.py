@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import mace_hip_kernels as mhk
-from mace_hip_kernels import matmul
+from mace_hip_kernels import _native, matmul
 from test_node_layers_gpu import BF16, F16, F32, by_halves, dense_case, dev, near, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -83,3 +83,30 @@ def test_a_slice_of_the_experts(dt):
     part = mhk.expert_dense(rows, w[2:5], order.offsets[2:6], activation='relu')
     a, z = order.offsets[2].item(), order.offsets[5].item()
     assert torch.equal(part[a:z], whole[a:z]) and (part[:a] == 0).all() and (part[z:] == 0).all()
+
+
+# ------------------------------------------------------------------------------------------ operands that a tile cannot take
+def test_the_library_holds_operands_to_whole_steps():
+    """Modules of tiles straight to LDS refuse, before any launch, addresses and distances of rows that such loads cannot
+    take.  (Operands here are of one row, so that no distance would lead out of them.)"""
+    d = dev()
+    print('[case] whole steps', flush=True)
+    lib = _native.load()
+    t, out = torch.ones(1 << 12, dtype=BF16, device=d), torch.zeros(64, 64, dtype=BF16, device=d)
+    p, c, far = t.data_ptr(), out.data_ptr(), matmul.LD_MAX
+    for tile in matmul.FAST:
+        rows = matmul.module(d, BF16, 'fwd', tile).handle
+        outer = matmul.module(d, BF16, 'dw', tile).handle
+
+        def fwd(a, lda, b, ldb):
+            return lib.mh_mm_rows(rows, a, lda, b, ldb, c, None, None, 0, None, None, 1, 1, 64, 1, _native.stream_of(t))
+
+        def dw(a, lda, b, ldb):
+            return lib.mh_mm_outer(outer, a, lda, b, ldb, c, None, None, 1, 64, 64, 1, 0, 1, _native.stream_of(t))
+
+        for call in (fwd, dw):
+            for args in ((p + 2, 64, p, 64), (p, 64, p + 8, 64), (p, 68, p, 64), (p, 64, p, 65), (p, far, p, 64), (p, 64, p, far)):
+                assert call(*args) != 0 and 'whole steps' in lib.mh_last_error().decode(), (tile, call, args)
+        assert fwd(p, 64, p, 64) == 0 and out[0, 0].item() == 64
+        assert dw(p, far - 8, p, 64) == 0 and (out == 1).all()
+        out.zero_()
