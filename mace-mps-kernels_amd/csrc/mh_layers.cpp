@@ -67,6 +67,15 @@ const char* const kDouble =
     "mace_hip_kernels: double backward (create_graph=True) is not available for the trainable node layers "
     "(dense, expert_dense, dispatch, combine, block_norm)";
 
+// A tangent would be lost without a word where nothing asks for a gradient: the kernels then run without an autograd function.
+void no_tangents(c10::ArrayRef<const Tensor*> inputs) {
+    if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+    for (const Tensor* t : inputs)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                    "mace_hip_kernels: forward-mode derivatives are not available for the trainable node layers "
+                                    "(dense, expert_dense, dispatch, combine, block_norm)");
+}
+
 // ---------------------------------------------------------------------------------------------------------- plans
 enum { FORWARD, BACKWARD, ROUTE, NORM };
 // a kind of plan and what it depends on, in the order of Python's planner of that kind
@@ -372,6 +381,7 @@ py::object dense(py::handle x_, py::handle w_, py::handle b_, py::handle r_, int
     if (grouped && (x.dim() != 2 || groups < 1 || off.scalar_type() != at::kInt || off.device() != x.device() ||
                     off.dim() != 1 || off.size(0) != groups + 1))
         return py::none();
+    no_tangents({&x, &w, &b, &r});
     if (grouped) off = off.contiguous();
     int64_t need = 0;
     if (at::GradMode::is_enabled()) need = grad(x) | grad(w) << 1 | grad(b) << 2 | grad(r) << 3;
@@ -495,6 +505,7 @@ bool an_order(const Tensor& place, const Tensor& off, const Tensor& x) {
 py::object dispatch(py::handle x_, const Tensor& place, const Tensor& off) {
     Tensor x;
     if (!tensor(x_, &x) || !fits(x) || x.dim() != 2 || x.size(0) != place.size(0) || !an_order(place, off, x)) return py::none();
+    no_tangents({&x});
     const PlanPtr p = route_plan(x, x.size(1));
     if (at::GradMode::is_enabled() && grad(x)) return py::cast(DispatchFn::apply(x, place, off, p));
     return py::cast(spread(*p, x, place, off));
@@ -507,6 +518,7 @@ py::object combine(py::handle y_, py::handle w_, py::handle r_, const Tensor& pl
         return py::none();
     if (w.defined() && (w.scalar_type() != at::kFloat || w.device() != y.device() || w.sizes() != place.sizes())) return py::none();
     if (r.defined() && (!alike(r, y) || r.dim() != 2 || r.size(0) != place.size(0) || r.size(1) != y.size(1))) return py::none();
+    no_tangents({&y, &w, &r});
     const PlanPtr p = route_plan(y, y.size(1));
     int64_t need = 0;
     if (at::GradMode::is_enabled()) need = grad(y) | grad(w) << 1 | grad(r) << 2;
@@ -598,6 +610,7 @@ py::object block_norm(py::handle x_, py::handle y_, py::handle g_, py::handle s_
         if (!t->defined()) continue;
         if (!alike(*t, x) || t->dim() != 1 || t->size(0) != C) return py::none();
     }
+    no_tangents({&x, &y, &gate, &scale, &wp, &wn});
     for (Tensor* t : {&x, &y, &gate, &scale, &wp, &wn})
         if (t->defined()) *t = t->contiguous();
     const PlanPtr p = plan(Key{{NORM, x.device().index(), type_of(x), x.numel() / C, C, layer, y.defined(), mode}}, N_SIZE);

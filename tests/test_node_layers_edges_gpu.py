@@ -1,5 +1,6 @@
 """
-The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row.
+The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
+that a tile cannot take, forward-mode derivatives.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -110,3 +111,26 @@ def test_the_library_holds_operands_to_whole_steps():
         assert fwd(p, 64, p, 64) == 0 and out[0, 0].item() == 64
         assert dw(p, far - 8, p, 64) == 0 and (out == 1).all()
         out.zero_()
+
+
+# ------------------------------------------------------------------------------------------ forward-mode derivatives
+def test_forward_mode_derivatives_are_refused():
+    d = dev()
+    print('[case] forward mode', flush=True)
+    x, w = torch.randn(6, 8, device=d), torch.randn(8, 8, device=d)
+    o = mhk.expert_order(torch.zeros(6, 1, dtype=torch.int64, device=d), 1)
+    off = torch.tensor([0, 6], dtype=torch.int32, device=d)
+    with torch.autograd.forward_ad.dual_level():
+        t = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        v = torch.autograd.forward_ad.make_dual(w, torch.ones_like(w))
+        for call in (lambda: mhk.dense(t, w), lambda: mhk.dense(x, v, activation='silu'), lambda: mhk.dense(x, w, residual=t),
+                     lambda: mhk.dense(x, w, bias=v[0]), lambda: mhk.expert_dense(t, w[None], off),
+                     lambda: mhk.dispatch(t, o), lambda: mhk.combine(t, None, o), lambda: mhk.combine(x, None, o, residual=t),
+                     lambda: mhk.combine(x, t[:, :1], o), lambda: mhk.block_norm(t), lambda: mhk.block_norm(x, t),
+                     lambda: mhk.block_norm(x, x, gate=t), lambda: mhk.block_norm(x, pre_weight=v[0])):
+            for want in (False, True):
+                w.requires_grad_(want)
+                with pytest.raises((RuntimeError, NotImplementedError), match='forward-mode'):
+                    call()
+        w.requires_grad_(False)
+        assert mhk.dense(x, w).shape == (6, 8)               # tensors without a tangent are taken as ever
