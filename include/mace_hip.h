@@ -716,8 +716,7 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * mh_mm_rows: C[r] = act(A[r] B_e^T + bias_e) + res[r] for the R rows of A [R, K] and their group's weights B [E, N, K]
  * (modules of matmul.source(.., 'fwd')) or [E, K, N] ('dx', where it is the input gradient A B_e); C [R, N]; bias [E, N],
  * res [R, N] and slope may be NULL.  Rows of no group are zero.  act (none, relu, silu, gelu by erf) is compiled in.  slope [R, N]
- * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types uint16 fixed point (steps of 2^-15
- * from -0.5; 0: NaN).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
+ * receives act'(A[r] B_e^T + bias_e) for mh_mm_slope: float32, or for the 16-bit types codes in uint16 (mm_slope_code).  Bind MH_MM_ROWS with the tile's threads, rows_per_block = its rows and grid_y = its columns.
  * Modules of a tile in matmul.FAST (their kernels' names begin with mm_fast_) need every address and row distance to be
  * multiples of 16 bytes, row distances below 2^21 values (both are checked) and rows padded to whole steps, with zeros in
  * operands whose rows are contracted (mh_mm_pad: y [R, Kp] = x [R, K] and zeros, MH_MM_PAD with 256 threads).

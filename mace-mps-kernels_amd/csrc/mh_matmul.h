@@ -199,17 +199,37 @@ __device__ __forceinline__ float mm_activate(float a, float& slope) {
     return a;
 }
 
-// act'(a) as the forward keeps it for the backward: float32, or for the 16-bit types fixed point with steps of 2^-15 from
-// -0.5 (the slopes of all activations lie in [-0.13, 1.13]; 0 and 1 are exact; code 0 stands for NaN): its error of 2^-16
-// is far below the 2^-8 (2^-11) to which these types round the product p, where a slope kept in them would add its own.  Two
-// slopes at a time by the conversion to 65535ths, which rounds to nearest and takes NaN to 0 (165 us at 16,384 x 4,096 x
-// 1,024 in bfloat16, where codes made one by one take 169 and no slopes 156).
+// act'(a) as the forward keeps it for the backward: float32, or for the 16-bit types a code of 16 bits.  The slopes of all
+// activations lie in [-0.13, 1.13], and behind a unit's tail they fall below any fixed step, so a magnitude is coded in even steps
+// of 2^-15 from 2^-7 on (float16: 2^-6), and below in steps of its own binade's 256th (512th) part, down to 2^-54 (2^-29).  Off by
+// at most 2^-16 and, above that end, by 2^-9 (2^-10) of the slope, whichever is less: half of what rounding the product p to bfloat16
+// adds, at most twice that for float16.  0 and 1 are exact.  Magnitudes count up from code 0, those of negative slopes down from
+// 65535; 0xC000, between the two, is NaN.  Coding them is nine operations a value: 160 us at 16,384 x 4,096 x 1,024 in bfloat16 with
+silu, 142 without slopes (even steps alone, which lose the tails, took 153; float32 slopes would be 134 MB more, written and read).
+template <int TY>
+struct mm_slope_code {
+    static constexpr int BITS = TY == MM_F16 ? 9 : 8;                        // of a small magnitude's mantissa
+    static constexpr float EDGE = TY == MM_F16 ? 0x1p-6f : 0x1p-7f;          // where the even steps begin, at code 12288
+    static constexpr float DOWN = TY == MM_F16 ? 0x1p-97f : 0x1p-72f;        // brings it to a float32 whose upper bits are its code
+    static constexpr float UP = TY == MM_F16 ? 0x1p97f : 0x1p72f;
+    static constexpr float FIRST = 12288.f - EDGE * 32768.f;                 // the even steps' code of 0
+    __device__ __forceinline__ static unsigned of(float slope) {
+        const float s = __builtin_fminf(slope, (49152.f - FIRST) * 0x1p-15f);        // NaN: the larger number, whose code is 0xC000
+        const float m = __builtin_fabsf(s);
+        const unsigned fine = (__float_as_uint(m * DOWN) + (1u << (22 - BITS))) >> (23 - BITS);
+        const unsigned even = __float_as_uint(__builtin_fmaf(m, 32768.f, 8388608.f + FIRST));       // in its lower half
+        return ((m < EDGE ? fine : even) ^ (unsigned)((int)__float_as_uint(s) >> 31)) & 0xFFFFu;
+    }
+    __device__ __forceinline__ static float value(unsigned code) {
+        const unsigned sign = code > 0xC000u ? 0x80000000u : 0u, m = sign ? code ^ 0xFFFFu : code;
+        const float v = m < 12288u ? __uint_as_float(m << (23 - BITS)) * UP : ((float)(int)m - FIRST) * 0x1p-15f;
+        return __uint_as_float(code == 0xC000u ? 0x7FC00000u : __float_as_uint(v) | sign);
+    }
+};
+// two at a time, the first in the lower half
+template <int TY>
 __device__ __forceinline__ unsigned mm_slope_codes(float lo, float hi) {
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_pknorm_u16(__builtin_fmaf(lo, 32768.f / 65535.f, 16384.f / 65535.f),
-                                                                        __builtin_fmaf(hi, 32768.f / 65535.f, 16384.f / 65535.f)));
-}
-__device__ __forceinline__ float mm_slope_value(unsigned c) {
-    return c ? (float)(int)c * 3.0517578125e-5f - 0.5f : __uint_as_float(0x7FC00000u);
+    return mm_slope_code<TY>::of(lo) | mm_slope_code<TY>::of(hi) << 16;
 }
 
 // ------------------------------------------------------------------------------------------------ groups of rows
@@ -727,7 +747,7 @@ __device__ __forceinline__ void mm_finish(mh_f4 v, long long at, int c, mh_f4 re
                 mm_put4<MM_F32>(static_cast<float*>(slope_) + at, d, c);
             } else {
                 unsigned short* s = static_cast<unsigned short*>(slope_) + at;
-                const mh_u2 w = {mm_slope_codes(d[0], d[1]), mm_slope_codes(d[2], d[3])};
+                const mh_u2 w = {mm_slope_codes<TY>(d[0], d[1]), mm_slope_codes<TY>(d[2], d[3])};
                 if (c >= 4)
                     *reinterpret_cast<mh_u2x*>(s) = w;
                 else
@@ -811,7 +831,7 @@ __device__ __forceinline__ void mm_store_lines(const tile_t& t, mh_u4* lds, long
             *reinterpret_cast<mh_u2*>(y + at) = mh_u2{mm_round<TY>(v.x) | (unsigned)mm_round<TY>(v.y) << 16,
                                                       mm_round<TY>(v.z) | (unsigned)mm_round<TY>(v.w) << 16};
             if (ACT != MM_NONE && slope)
-                *reinterpret_cast<mh_u2*>(d + at) = mh_u2{mm_slope_codes(c.x, c.y), mm_slope_codes(c.z, c.w)};
+                *reinterpret_cast<mh_u2*>(d + at) = mh_u2{mm_slope_codes<TY>(c.x, c.y), mm_slope_codes<TY>(c.z, c.w)};
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
@@ -1075,8 +1095,9 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
         if constexpr (TY == MM_F32) {
             return v * __builtin_bit_cast(mh_f4, d);
         } else {
-            return v * mh_f4{mm_slope_value(d.x & 0xFFFFu), mm_slope_value(d.x >> 16), mm_slope_value(d.y & 0xFFFFu),
-                             mm_slope_value(d.y >> 16)};
+            typedef mm_slope_code<TY> code;
+            return v * mh_f4{code::value(d.x & 0xFFFFu), code::value(d.x >> 16), code::value(d.y & 0xFFFFu),
+                             code::value(d.y >> 16)};
         }
     };
     if (c >= 4) {
@@ -1106,7 +1127,7 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {            // behind the row: v is zero there, and the slope too
                     if constexpr (TY == MM_F32) d[j] = j < c ? static_cast<const unsigned*>(slope_)[at + j] : 0u;
-                    else d[j / 2] |= (j < c ? static_cast<const unsigned short*>(slope_)[at + j] : 16384u) << (16 * (j & 1));
+                    else d[j / 2] |= (j < c ? static_cast<const unsigned short*>(slope_)[at + j] : 0u) << (16 * (j & 1));
                 }
                 v = times(v, d);
             }

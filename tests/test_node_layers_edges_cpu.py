@@ -33,20 +33,22 @@ static dim threadIdx, blockIdx, blockDim, gridDim;
 static int __shfl_up(int v, int, int) { return v; }
 static int mh_bcast(int v, int) { return v; }
 static unsigned long long __ballot(bool b) { return b; }
+static unsigned __float_as_uint(float v) { unsigned u; memcpy(&u, &v, 4); return u; }
+static float __uint_as_float(unsigned u) { float v; memcpy(&v, &u, 4); return v; }
 static int __ffsll(unsigned long long v) { return v ? 1 + __builtin_ctzll(v) : 0; }
 """
 
 
 def function(header, name):
-    """The text of a function of a device header, its template line and qualifiers included."""
+    """The text of a function or struct of a device header, its template line and qualifiers included."""
     with open(os.path.join(CSRC, header)) as f:
         text = f.read()
-    m = re.search(r'^(template <[^\n]*>\n)?[^\n;]*\b' + name + r'\([^;{]*\{', text, re.M)
+    m = re.search(r'^(template <[^\n]*>\n)?(struct ' + name + r' \{|[^\n;]*\b' + name + r'\([^;{]*\{)', text, re.M)
     depth, end = 1, m.end()
     while depth:
         depth += {'{': 1, '}': -1}.get(text[end], 0)
         end += 1
-    return text[m.start():end] + '\n'
+    return text[m.start():end] + ';\n'
 
 
 def host_library(src, tmp_path):
@@ -176,3 +178,43 @@ def test_the_library_refuses_halves_that_a_tile_cannot_address():
                  lambda: lib.mh_hv_outer(None, p, p, p, None, None, p, p, p, p, 4, wide, 4, 1, 0, 1, None),
                  lambda: lib.mh_hv_outer(None, p, p, p, None, None, p, p, p, p, 4, 4, wide, 1, 0, 1, None)):
         assert call() != 0 and 'bad sizes' in lib.mh_last_error().decode()
+
+
+@needs_gxx
+@pytest.mark.parametrize('bits,rel,least', [(8, 2.0 ** -9, 2.0 ** -54), (9, 2.0 ** -10, 2.0 ** -29)], ids=['bf16', 'f16'])
+def test_codes_of_slopes_are_near_at_every_size(bits, rel, least, tmp_path):
+    """A slope and its code differ by at most 2^-16, and by at most half a step of its own magnitude down to ``least``; 0, 1 and
+    NaN come back as they are, and every code stands for one slope."""
+    lib = host_library('#define MM_F16 2\n' + function('mh_matmul.h', 'mm_slope_code') + f"""
+typedef mm_slope_code<{2 if bits == 9 else 1}> code;
+extern "C" void there(const float* v, unsigned short* c, int n) {{ for (int i = 0; i < n; ++i) c[i] = code::of(v[i]); }}
+extern "C" void back(const unsigned short* c, float* v, int n) {{ for (int i = 0; i < n; ++i) v[i] = code::value(c[i]); }}
+""", tmp_path)
+
+    def there(v):
+        c = np.empty(len(v), dtype=np.uint16)
+        lib.there(v.ctypes.data_as(ctypes.c_void_p), c.ctypes.data_as(ctypes.c_void_p), len(v))
+        return c
+
+    def back(c):
+        v = np.empty(len(c), dtype=np.float32)
+        lib.back(c.ctypes.data_as(ctypes.c_void_p), v.ctypes.data_as(ctypes.c_void_p), len(c))
+        return v
+
+    rng = np.random.default_rng(1)
+    v = np.concatenate([rng.uniform(-0.1290, 1.1290, 400_000), -2.0 ** rng.uniform(-90, -3, 200_000),
+                        2.0 ** rng.uniform(-90, 0, 200_000), -2.0 ** np.arange(-40.0, -3), 2.0 ** np.arange(-60.0, 1)])
+    v = v[(v > -0.129) & (v < 1.129)].astype(np.float32)
+    w = back(there(v))
+    off = np.abs(w.astype(np.float64) - v)
+    assert (off <= 2.0 ** -16).all()
+    inside = np.abs(v) >= least
+    assert (off[inside] <= rel * np.abs(v[inside])).all()
+    # below that half a step of the last binade, and what the scaled magnitude, no normal float32 any more, has lost before
+    assert (off[~inside] <= rel * least + 2.0 ** -150 * least * 2.0 ** 126).all() and (np.signbit(w) == np.signbit(v))[w != 0].all()
+    assert back(there(np.array([0, -0.0, 1, 0.5], dtype=np.float32))).tolist() == [0, 0, 1, 0.5]
+    for nan in (0x7FC00000, 0xFFC00000, 0x7FC12345, 0x7FC02000):     # quiet, as arithmetic leaves them
+        assert np.isnan(back(there(np.array([nan], dtype=np.uint32).view(np.float32))))[0]
+    # the codes in use are each other's inverse
+    used = np.concatenate([np.arange(1, 48771), np.arange(49536, 65535)]).astype(np.uint16)
+    assert (there(back(used)) == used).all() and np.isnan(back(np.array([0xC000], dtype=np.uint16)))[0]

@@ -1,6 +1,6 @@
 """
 The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
-that a tile cannot take, forward-mode derivatives.
+that a tile cannot take, forward-mode derivatives, units far in an activation's tail.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -9,7 +9,7 @@ import torch
 
 import mace_hip_kernels as mhk
 from mace_hip_kernels import _native, matmul
-from test_node_layers_gpu import BF16, F16, F32, by_halves, dense_case, dev, near, rand  # noqa: F401
+from test_node_layers_gpu import BF16, E32, F16, F32, TINY, U, by_halves, dense_case, dev, near, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 TYPES = pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
@@ -134,3 +134,39 @@ def test_forward_mode_derivatives_are_refused():
                     call()
         w.requires_grad_(False)
         assert mhk.dense(x, w).shape == (6, 8)               # tensors without a tangent are taken as ever
+
+
+# ------------------------------------------------------------------------------------------ slopes in an activation's tail
+@pytest.mark.parametrize('dt', [BF16, F16], ids=['bf16', 'f16'])
+@pytest.mark.parametrize('act', ['silu', 'gelu'])
+@pytest.mark.parametrize('T', [50, 700])
+def test_gradients_of_units_in_the_tail(T, act, dt):
+    """Pre-activations between -4 and -12, where act' is down to 1e-30: gradients are right relative to their own size.
+
+    Relative errors of a slope: 2^-9 by its coding, 3e-4 by its evaluation (of which 2.2e-4 the approximation of erf, the most
+    that it is off in the tail), and that of its argument, whose error is (K + 16) 2^-24 of the magnitudes, times |act''/act'| <=
+    |a| + 1.  Slopes below 2^-54 may come out as zero (float16 rounds their products to zero anyway)."""
+    d = dev()
+    print(f'[case] tail T={T} {act} {dt}', flush=True)
+    rng = np.random.default_rng(9)
+    K, N = 16, 72
+    x, w, b = rand(rng, T, K, dt=dt), rand(rng, N, K, dt=dt, scale=0.02), torch.linspace(-4, -12, N).to(dt)
+    g = (rand(rng, T, N) * 0.2 + 1).to(dt)
+    leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+    y = mhk.dense(*leaves[:2], leaves[2], act)
+    dx, dw, db = (t.double().cpu() for t in torch.autograd.grad(y, leaves, g.to(d)))
+    x, w, b, g = (t.double() for t in (x, w, b, g))
+    a = x @ w.t() + b
+    if act == 'silu':
+        q = 1 / (1 + torch.exp(-a))
+        slope = q * (1 + a * (1 - q))
+    else:
+        slope = 0.5 * torch.erfc(-a * 0.5 ** 0.5) + a * torch.exp(-0.5 * a * a) * (2 * np.pi) ** -0.5
+    rel = 2.0 ** -9 + 3e-4 + (K + 16) * E32 * (x.abs() @ w.abs().t() + b.abs()) * (a.abs() + 1)
+    p = g * slope
+    err = p.abs() * (rel + E32) + g * 2.0 ** -54
+    near('db', db, p.sum(0), err.sum(0) + ((T + 16) * E32 + U[dt]) * p.abs().sum(0) + TINY[dt])
+    err = err + U[dt] * p.abs() + TINY[dt]                   # p rounded for the products
+    for name, got, val, e, n in (('dx', dx, p @ w, (err @ w.abs(), p.abs() @ w.abs()), N),
+                                 ('dw', dw, p.t() @ x, (err.t() @ x.abs(), p.abs().t() @ x.abs()), T)):
+        near(name, got, val, e[0] + (n + 16) * E32 * e[1] + U[dt] * (val.abs() + e[0]) + TINY[dt])
