@@ -205,7 +205,7 @@ __device__ __forceinline__ float mm_activate(float a, float& slope) {
 // at most 2^-16 and, above that end, by 2^-9 (2^-10) of the slope, whichever is less: half of what rounding the product p to bfloat16
 // adds, at most twice that for float16.  0 and 1 are exact.  Magnitudes count up from code 0, those of negative slopes down from
 // 65535; 0xC000, between the two, is NaN.  Coding them is nine operations a value: 160 us at 16,384 x 4,096 x 1,024 in bfloat16 with
-silu, 142 without slopes (even steps alone, which lose the tails, took 153; float32 slopes would be 134 MB more, written and read).
+// silu, 142 without slopes (even steps alone, which lose the tails, took 153; float32 slopes would be 134 MB more, written and read).
 template <int TY>
 struct mm_slope_code {
     static constexpr int BITS = TY == MM_F16 ? 9 : 8;                        // of a small magnitude's mantissa
