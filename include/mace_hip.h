@@ -137,7 +137,8 @@ enum mh_kernel_kind {
     MH_HV_MM = 98,       /* MH_MM_ROWS on halves                                                               */
     MH_HV_OUTER = 99,    /* MH_MM_OUTER on halves                                                              */
     MH_MM_PAD = 100,     /* rows of 16-bit values at whole steps of 16 bytes                                   */
-    MH_NUM_KINDS = 101
+    MH_HV_AGAIN = 101,   /* MH_HV_MM's or MH_HV_OUTER's marked tiles from the operands themselves             */
+    MH_NUM_KINDS = 102
 };
 
 /* flags of mh_conv_bwd */
@@ -736,17 +737,20 @@ int mh_geom_bwd(mh_module* m, const float* vec, const float* len, const float* g
  * scratch for the larger of [slots_s, N] and [slots_o, N, K] (the first not needed for one slot without offsets, the
  * second not for Lo = 0).
  *
- * Float32 products by float16 halves (modules of halves.source): every value times a power of two s is hi + lo, s the one
- * that brings the largest finite magnitude of its row, or of its column within a group of rows, to [2^14, 2^15).
- * mh_hv_rows: y [R][Kp / 32][2][32] (hi, lo; Kp = K rounded up to 32, zeros behind K) and peak [R], the bits of the largest
- * finite magnitude, bit 31 where the row holds an infinity or NaN.  mh_hv_columns: y [R][2][Cp] (Cp = C rounded up to 8) and
- * peak [2][E][C] (zero before the call): peaks, then bit 31 of the marks; groups by offsets, or (NULL) E groups of G
- * rows each (R = E G); pieces of L rows, `slots` >= their number.  Rows of no group are not written.
- * mh_hv_mm: mh_mm_rows from halves: A rows with pa [R]; B rows [E N] with pb [E][N] and mb NULL (C = act(A B^T + bias) +
+ * Float32 products by float16 halves (modules of halves.source): every value times a power of two s is hi + lo / 4096, s the
+ * one that brings the largest finite magnitude of its row, or of its column within a group of rows, to [2^14, 2^15).
+ * mh_hv_rows: y [R][Kp / 32][2][32] (hi, lo; Kp = K rounded up to 32, zeros behind K) and peak [R + 1], for each row a word of
+ * its largest and smallest magnitudes (mh_halves.h), then zero.  mh_hv_columns: y [R][2][Cp] (Cp = C rounded up to 8) and
+ * peak [2][E][C] (zero before the call), the words in two parts; groups by offsets, or (NULL) E groups of G rows each
+ * (R = E G); pieces of L rows, `slots` >= their number.  Rows of no group are not written.
+ * mh_hv_mm: mh_mm_rows from halves: A rows with pa [R + 1]; B rows [E N] with pb [E][N] and mb NULL (C = act(A B^T + bias) +
  * res), or columns of E groups of K rows, length N, with pb and mb [E][N] (C = A B).  mh_hv_outer: mh_mm_outer from columns
- * A (pa, ma [E][M]) and B (pb, mb [E][N]).  All buffers 16-byte aligned; rows of halves, 2 K values, and columns, M and N,
- * below 2^21 with their padding.  Bind MH_HV_ROWS, MH_HV_PEAKS and MH_HV_COLUMNS with
- * 256 threads, the others as MH_MM_ROWS.
+ * A (pa [E][M], ma [E][M] and one word more, zero before the call) and B (pb, mb [E][N]).  All buffers 16-byte aligned; rows of
+ * halves, 2 K values, and columns, M and N, below 2^21 with their padding.  Both mark, in pa or ma, rows of results that the
+ * halves do not hold to a float32 sum's accuracy, and set the last word where there are such, infinities or NaN:
+ * mh_hv_again_mm and mh_hv_again_outer then compute the tiles of these from the float32 operands that the halves were made of (the same
+ * arguments, operands with their row distances instead of halves; `most` workgroups at most).  Bind MH_HV_ROWS, MH_HV_PEAKS and
+ * MH_HV_COLUMNS with 256 threads, the others as MH_MM_ROWS.
  *
  * mh_expert_order: the A = T k assignments experts [T, k] (int32, or int64 where wide), values outside [0, E) dropped,
  * stably sorted by expert: offsets [E + 1], rows [A] (flat assignment at each place; -1 from offsets[E] on), place [A]
@@ -781,11 +785,17 @@ int mh_hv_rows(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t*
 int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32_t* peak, const int32_t* offsets, int32_t R,
                   int32_t C, int32_t E, int32_t G, int32_t L, int32_t slots, void* stream);
 int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const float* bias, const float* res, int64_t ldr,
-             float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
+             float* slope, const int32_t* offsets, uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
              int32_t N, int32_t K, int32_t E, void* stream);
 int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, float* part, const int32_t* offsets,
-                const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
+                const uint32_t* pa, uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
                 int32_t N, int32_t E, int32_t L, int32_t slots, void* stream);
+int mh_hv_again_mm(mh_module* m, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, const float* bias,
+                   const float* res, int64_t ldr, float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb,
+                   const uint32_t* mb, int32_t R, int32_t N, int32_t K, int32_t E, int32_t most, void* stream);
+int mh_hv_again_outer(mh_module* m, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, float* part,
+                      const int32_t* offsets, const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb,
+                      int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, int32_t most, void* stream);
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,
                     int32_t* offsets, int32_t* rows, int32_t* place, void* stream);
 int mh_dispatch(mh_module* m, const void* x, int64_t ldx, const int32_t* place, const int32_t* offsets, void* y, int32_t T,

@@ -149,7 +149,7 @@ extern "C" {
 
 const char* mh_last_error(void) { return g_err.c_str(); }
 
-int mh_version(void) { return 50; }
+int mh_version(void) { return 51; }
 
 int mh_launch_log(int enable) {
     std::lock_guard<std::mutex> lock(g_log_mu);
@@ -1355,7 +1355,7 @@ int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32
 }
 
 int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const float* bias, const float* res, int64_t ldr,
-             float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
+             float* slope, const int32_t* offsets, uint32_t* pa, const uint32_t* pb, const uint32_t* mb, int32_t R,
              int32_t N, int32_t K, int32_t E, void* stream) {
     // a row of halves is 2 K values long, rounded up; a column operand's is N
     if (R < 0 || N < 0 || K < 1 || 2LL * K > kStepsLd - 64 || (mb && N > kStepsLd - 8) || E < 1 || (E > 1 && !offsets))
@@ -1372,7 +1372,7 @@ int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const
 }
 
 int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, float* part, const int32_t* offsets,
-                const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
+                const uint32_t* pa, uint32_t* ma, const uint32_t* pb, const uint32_t* mb, int32_t R, int32_t M,
                 int32_t N, int32_t E, int32_t L, int32_t slots, void* stream) {
     if (R < 1 || R > 0x3fffffff || M < 1 || N < 1 || M > kStepsLd - 8 || N > kStepsLd - 8 || E < 1 || (E > 1 && !offsets) ||
         L < 0 || (L && slots < 1) || R > 0x7fffffff - L)
@@ -1384,6 +1384,42 @@ int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, fl
                           ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
     void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &R, &M, &N, &E, &L};
     return launch_blocks(m, MH_HV_OUTER, tiles, args, stream, "mh_hv_outer", L ? slots : E);
+}
+
+int mh_hv_again_mm(mh_module* m, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, const float* bias,
+                   const float* res, int64_t ldr, float* slope, const int32_t* offsets, const uint32_t* pa, const uint32_t* pb,
+                   const uint32_t* mb, int32_t R, int32_t N, int32_t K, int32_t E, int32_t most, void* stream) {
+    if (R < 0 || N < 0 || K < 1 || E < 1 || (E > 1 && !offsets) || most < 1) return fail(-1, "mh_hv_again_mm: bad sizes");
+    if (R == 0 || N == 0) return 0;
+    if (!A || !B || !C || !pa || !pb) return fail(-1, "mh_hv_again_mm: NULL operand");
+    if (lda < K || ldb < (mb ? N : K) || (res && ldr < N))
+        return fail(-1, "mh_hv_again_mm: rows overlap (ld below the row's length)");
+    if (!m || !m->k[MH_HV_AGAIN].fn) return fail(-1, "mh_hv_again_mm: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_HV_AGAIN];
+    if (R > 0x7fffffff - k.rows_per_block) return fail(-1, "mh_hv_again_mm: too many rows");
+    const int64_t all = pieces(offsets, R, E, k.rows_per_block) * ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    if (all > 0x7fffffff - most) return fail(-1, "mh_hv_again_mm: launch too large");
+    int32_t tiles = static_cast<int32_t>(all);
+    void* args[] = {&A, &B, &C, &bias, &res, &slope, &offsets, &pa, &pb, &mb, &lda, &ldb, &ldr, &R, &N, &K, &E, &tiles};
+    return launch_blocks(m, MH_HV_AGAIN, std::min<int64_t>(tiles, most), args, stream, "mh_hv_again_mm");
+}
+
+int mh_hv_again_outer(mh_module* m, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, float* part,
+                      const int32_t* offsets, const uint32_t* pa, const uint32_t* ma, const uint32_t* pb, const uint32_t* mb,
+                      int32_t R, int32_t M, int32_t N, int32_t E, int32_t L, int32_t slots, int32_t most, void* stream) {
+    if (R < 1 || M < 1 || N < 1 || E < 1 || (E > 1 && !offsets) || L < 0 || (L && slots < 1) || R > 0x7fffffff - L || most < 1)
+        return fail(-1, "mh_hv_again_outer: bad sizes");
+    if (!A || !B || !pa || !ma || !pb || !mb || (L ? !part : !C)) return fail(-1, "mh_hv_again_outer: NULL operand");
+    if (lda < M || ldb < N) return fail(-1, "mh_hv_again_outer: rows overlap (ld below the row's length)");
+    if (!m || !m->k[MH_HV_AGAIN].fn) return fail(-1, "mh_hv_again_outer: kernel slot not bound in this module");
+    const Kernel& k = m->k[MH_HV_AGAIN];
+    const int64_t all = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
+                        ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
+    if (all > 0x7fffffff) return fail(-1, "mh_hv_again_outer: launch too large");
+    int32_t tiles = static_cast<int32_t>(all);
+    if (!L) slots = E;
+    void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &lda, &ldb, &R, &M, &N, &E, &L, &tiles, &slots};
+    return launch_blocks(m, MH_HV_AGAIN, std::min<int64_t>(all * slots, most), args, stream, "mh_hv_again_outer");
 }
 
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,

@@ -1,30 +1,51 @@
 // mh_halves.h — float32 matrix products as three float16 ones, prepended with mh_device.h and mh_matmul.h.
 //
-// A row (or column) of values times a power of two s that brings its largest to [2^14, 2^15) is, value by value, hi + lo with
-// hi and lo float16: hi the nearest, lo the nearest to what is left, together off by at most 2^-24 of the value, or 2^-40 of
-// the row's largest where that is more.  a b = (hi_a + lo_a)(hi_b + lo_b) / (s_a s_b), where lo_a lo_b is below 2^-24 of
-// |a b| and left out: three products on the matrix cores where three bf16 parts need six, at the price of a pass that writes
-// the halves (s must not change along the contraction, so one s per row of an operand that is contiguous along it, one per
-// column and group of an operand whose rows are contracted).  Both forms keep the halves next to each other, as matrices of
-// 16-bit values whose contraction is twice as long, which the tiles of mh_matmul.h load as they are:
+// A row (or column) of values times a power of two s that brings its largest to [2^14, 2^15) is, value by value, hi + 2^-12 lo
+// with hi and lo float16: hi the nearest, lo the nearest to 2^12 times what is left.  a b = (hi_a + 2^-12 lo_a)
+// (hi_b + 2^-12 lo_b) / (s_a s_b), where lo_a lo_b, below 2^-22 of |a b|, is left out: three products on the matrix cores where
+// three bf16 parts need six, at the price of a pass that writes the halves (s must not change along the contraction, so one s
+// per row of an operand that is contiguous along it, one per column and group of an operand whose rows are contracted).  Both
+// forms keep the halves next to each other, as matrices of 16-bit values whose contraction is twice as long, which the tiles of
+// mh_matmul.h load as they are:
 //   rows    [R][Kp / 32][2][32]    32 hi, their 32 lo, ...; Kp = K rounded up to 32, zeros behind K
 //   columns [R][2][Cp]             a row of hi, its row of lo; Cp = C rounded up to 8
-// Infinite and NaN values are hi as they are, lo 0.  Their rows and columns are marked, and what they reach is taken from the
-// products hi hi alone, which give what a float32 sum gives.
+//
+// What the halves hold.  A value of at least 2^-14 after scaling is off by at most 2^-23 of itself, a smaller one by at most
+// 2^-37.  So where both operands' values other than zero lie within 2^28 of their row's (column's) largest, a product is off by at
+// most 2^-21 of |a b|, before what float32 sums add.  A row with a smaller value is `wide`: its results are off by up to
+// K 2^-20 more in the units of the scaled sums, which is below K 2^-24 of any sum of at least 16 and so no more than a float32
+// sum of K products may be off by.  What is left, results of a wide row or column below 16 (of largest products of 2^28 and
+// more: one in 10^8 of random ones) and those of rows and columns with an infinity or NaN, are marked by row of the result,
+// and hv_again computes the tiles that hold a marked one as the direct kernels do.
 #pragma once
 
-#define HV_ODD 0x80000000u          // in a peak: the row or column holds an infinity or NaN
+// What is known of a row's or column's values, a word: the exponent field of the largest, from bit 8 on 255 minus that of the
+// smallest but zero (277 for subnormal ones; 0: zeros only), and
+#define HV_AGAIN 0x40000000u        // a result of this row is to be computed again
+#define HV_ODD 0x80000000u          // it holds an infinity or NaN
+#define HV_LARGEST 0xFFu
+#define HV_SMALLEST 0x1FF00u
 
-// exponent of s for the largest finite magnitude (its bits): 2^126 at most, beyond which float32 has no s
-__device__ __forceinline__ int hv_shift(unsigned peak) {
-    const int e = (int)((peak & 0x7FFFFFFFu) >> 23);
-    return (peak & 0x7FFFFFFFu) ? min(14 - (e - 127), 126) : 0;
+__device__ __forceinline__ unsigned hv_word(float v) {
+    const unsigned b = __float_as_uint(v) & 0x7FFFFFFFu, e = b >> 23;
+    return b == 0u ? 0u : e == 255u ? HV_ODD : e | (e ? 255u - e : 277u) << 8;
 }
+
+// of two sets of values
+__device__ __forceinline__ unsigned hv_join(unsigned a, unsigned b) {
+    return max(a & HV_LARGEST, b & HV_LARGEST) | max(a & HV_SMALLEST, b & HV_SMALLEST) | ((a | b) & HV_ODD);
+}
+
+// exponent of s: 126 at most, beyond which float32 has no s
+__device__ __forceinline__ int hv_shift(unsigned word) { return min(141 - (int)(word & HV_LARGEST), 126); }
+
+// whether a value other than zero is below 2^-14 after scaling
+__device__ __forceinline__ bool hv_wide(unsigned word) { return (int)((word & HV_SMALLEST) >> 8) > 142 + hv_shift(word); }
 
 __device__ __forceinline__ void hv_split(float v, int shift, unsigned short& hi, unsigned short& lo) {
     const float t = __builtin_ldexpf(v, shift);
     const _Float16 h = (_Float16)t;
-    const _Float16 l = (_Float16)(t - (float)h);
+    const _Float16 l = (_Float16)((t - (float)h) * 4096.f);
     hi = __builtin_bit_cast(unsigned short, h);
     lo = __builtin_isfinite(v) ? __builtin_bit_cast(unsigned short, l) : (unsigned short)0;
 }
@@ -39,20 +60,11 @@ __device__ __forceinline__ void hv_split4(mh_f4 v, int4 shift, unsigned short* h
     *reinterpret_cast<mh_u2*>(lo) = mh_u2{l[0] | (unsigned)l[1] << 16, l[2] | (unsigned)l[3] << 16};
 }
 
-// the bits of |v| where it is finite, HV_ODD where not
-__device__ __forceinline__ unsigned hv_peak(float v) {
-    const unsigned b = __float_as_uint(v) & 0x7FFFFFFFu;
-    return b < 0x7F800000u ? b : HV_ODD;
-}
-
-// Largest of peaks, odd if any is
-__device__ __forceinline__ unsigned hv_max(unsigned a, unsigned b) {
-    return max(a & 0x7FFFFFFFu, b & 0x7FFFFFFFu) | ((a | b) & HV_ODD);
-}
-
-// Rows: a wave each; the second reading of a row comes from the caches.  Bound by its bytes: 20,000 rows of 1,024 in 38 us, 4.3 TB/s.
+// Rows: a wave each; the second reading of a row comes from the caches.  word [R + 1]: the last, whether anything is to be computed
+// again, zero here.  Bound by its bytes: 20,000 rows of 1,024 in 38 us, 4.3 TB/s.
 extern "C" __global__ __launch_bounds__(256) void hv_rows(const float* __restrict__ x, unsigned short* __restrict__ y,
-                                                          unsigned* __restrict__ peak, long long ld, int R, int K) {
+                                                          unsigned* __restrict__ word, long long ld, int R, int K) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) word[R] = 0u;
     const int lane = threadIdx.x & 63, Kp = (K + 31) / 32 * 32;
     const long long r = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= R) return;
@@ -61,11 +73,11 @@ extern "C" __global__ __launch_bounds__(256) void hv_rows(const float* __restric
     for (int k = 4 * lane; k < K; k += 256) {
         const mh_f4 v = mm_get4<MM_F32>(p + k, K - k);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) m = hv_max(m, hv_peak(v[j]));
+        for (int j = 0; j < 4; ++j) m = hv_join(m, hv_word(v[j]));
     }
 #pragma unroll
-    for (int d = 1; d < MH_WAVE; d <<= 1) m = hv_max(m, (unsigned)__shfl_xor((int)m, d, MH_WAVE));
-    if (lane == 0) peak[r] = m;
+    for (int d = 1; d < MH_WAVE; d <<= 1) m = hv_join(m, (unsigned)__shfl_xor((int)m, d, MH_WAVE));
+    if (lane == 0) word[r] = m;
     const int s = hv_shift(m);
     unsigned short* q = y + r * 2 * Kp;
     for (int k = 4 * lane; k < Kp; k += 256) {
@@ -85,9 +97,10 @@ __device__ __forceinline__ bool hv_slot(const int* off, int E, int R, int G, int
     return e < E;
 }
 
-// Columns, first pass: the peaks [E, C] and marks [E, C] (both zero before) of each group's columns, a workgroup for a piece
-// of rows and 256 columns.  The largest of integers does not depend on the order of the atomics.  Bound, with the second pass, by
-// their bytes: 12 a value, 1,024 x 1,024 weights 5.2 and 5.6 us.
+// Columns, first pass: of each group's columns, the words in two arrays (zero before) whose largest values atomics can find: peak
+// [E, C] the largest's exponents, mark [E, C] the smallest's and the odd ones' bit.  A workgroup for a piece of rows and 256
+// columns.  The largest of integers does not depend on the order of the atomics.  Bound, with the second pass, by their bytes: 12
+// a value, 1,024 x 1,024 weights 5.2 and 5.6 us.
 extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restrict__ x, unsigned* __restrict__ peak,
                                                            unsigned* __restrict__ mark, const int* __restrict__ off,
                                                            long long ld, int R, int C, int E, int G, int L) {
@@ -101,7 +114,7 @@ extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restri
         for (int r = r0 + w; r < r1; r += 4) {
             const mh_f4 v = mm_get4<MM_F32>(x + (long long)r * ld + c, C - c);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) m[j] = hv_max(m[j], hv_peak(v[j]));
+            for (int j = 0; j < 4; ++j) m[j] = hv_join(m[j], hv_word(v[j]));
         }
     }
 #pragma unroll
@@ -111,9 +124,9 @@ extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restri
     if (i >= C) return;
     unsigned b = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) b = hv_max(b, best[k][threadIdx.x >> 2][threadIdx.x & 3]);
-    atomicMax(&peak[(long long)e * C + i], b & 0x7FFFFFFFu);
-    if (b & HV_ODD) atomicOr(&mark[(long long)e * C + i], HV_ODD);
+    for (int k = 0; k < 4; ++k) b = hv_join(b, best[k][threadIdx.x >> 2][threadIdx.x & 3]);
+    atomicMax(&peak[(long long)e * C + i], b & HV_LARGEST);
+    atomicMax(&mark[(long long)e * C + i], b & (HV_SMALLEST | HV_ODD));
 }
 
 // Columns, second pass: the halves.
@@ -138,80 +151,75 @@ extern "C" __global__ __launch_bounds__(256) void hv_columns(const float* __rest
     }
 }
 
-// A finished tile whose sums stand for sums times 2^(row's shift + column's): what mm_store_tile takes.  Where the tile has
-// marked rows or columns (`odd`), the sums are those of the upper halves alone and an unmarked element is taken from C, where
-// its own thread put it before.
+// The word of row or column i: one array, or (columns) two.
+__device__ __forceinline__ unsigned hv_read(const unsigned* peak, const unsigned* mark, long long i) {
+    return peak[i] | (mark ? mark[i] : 0u);
+}
+
+// A finished tile whose sums stand for sums times 2^(row's shift + column's): what mm_store_tile takes.
 template <typename tile_t>
 struct hv_result {
     static constexpr int ROWS = tile_t::ROWS, COLS = tile_t::COLS;
     const tile_t& t;
-    float* C;                                            // the tile's first element, rows N apart
-    long long N;
-    int rows, cols;
-    bool odd = false;
+    const int rows, cols;
     unsigned a[ROWS];
     mh_u4 b[COLS];
     __device__ __forceinline__ static int row(int i) { return tile_t::row(i); }
     __device__ __forceinline__ static int column(int j) { return tile_t::column(j); }
-    // peaks of the tile's rows and columns; their marks apart (ma, mb) or among them (NULL)
-    __device__ __forceinline__ hv_result(const tile_t& tile, float* C, long long N, const unsigned* pa, const unsigned* ma,
-                                         int rows, const unsigned* pb, const unsigned* mb, int cols)
-        : t(tile), C(C), N(N), rows(rows), cols(cols) {
+    // words of the tile's rows and columns
+    __device__ __forceinline__ hv_result(const tile_t& tile, const unsigned* pa, const unsigned* ma, int rows, const unsigned* pb,
+                                         const unsigned* mb, int cols)
+        : t(tile), rows(rows), cols(cols) {
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i) {
-            const int m = min(row(i), rows - 1);
-            a[i] = pa[m] | (ma ? ma[m] : 0u);
-        }
+        for (int i = 0; i < ROWS; ++i) a[i] = hv_read(pa, ma, min(row(i), rows - 1));
 #pragma unroll
         for (int j = 0; j < COLS; ++j)
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const int n = min(column(j) + c, cols - 1);
-                b[j][c] = pb[n] | (mb ? mb[n] : 0u);
-            }
+            for (int c = 0; c < 4; ++c) b[j][c] = hv_read(pb, mb, min(column(j) + c, cols - 1));
     }
-    // the whole workgroup's answer; also the barrier after the tile's products
-    __device__ __forceinline__ bool any_odd() const {
-        unsigned o = 0;
-#pragma unroll
-        for (int i = 0; i < ROWS; ++i) o |= a[i];
-#pragma unroll
-        for (int j = 0; j < COLS; ++j) o |= b[j].x | b[j].y | b[j].z | b[j].w;
-        return __syncthreads_or((o & HV_ODD) != 0);
-    }
-    __device__ __forceinline__ mh_f4 scaled(int i, int j) const {
+    __device__ __forceinline__ mh_f4 value(int i, int j) const {
         mh_f4 v = t.value(i, j);
         const int s = hv_shift(a[i]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) v[c] = __builtin_ldexpf(v[c], -(s + hv_shift(b[j][c])));
         return v;
     }
-    __device__ __forceinline__ void keep() const {
+    // Marks the rows with results that the halves do not hold, in the words' array that keeps the smallest exponents (`at`: where
+    // the tile's rows begin), and sets *any where there are such or odd rows or columns.  Workgroups of the same rows store the
+    // same word.
+    template <bool SPLIT>
+    __device__ __forceinline__ void mark(unsigned* at, unsigned* any) const {
+        unsigned some = 0u;
 #pragma unroll
-        for (int i = 0; i < ROWS; ++i)
+        for (int j = 0; j < COLS; ++j) some |= b[j].x | b[j].y | b[j].z | b[j].w;
 #pragma unroll
-            for (int j = 0; j < COLS; ++j)
-                if (row(i) < rows && column(j) < cols)
-                    mm_put4<MM_F32>(C + row(i) * N + column(j), scaled(i, j), cols - column(j));
-    }
-    __device__ __forceinline__ mh_f4 value(int i, int j) const {
-        mh_f4 v = scaled(i, j);
-        if (odd) {
-            const mh_f4 u = mm_get4<MM_F32>(C + row(i) * N + column(j), cols - column(j));
+        for (int i = 0; i < ROWS; ++i) {
+            const bool wide = hv_wide(a[i]);
+            bool again = false;
+            some |= a[i];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) v[c] = (a[i] | b[j][c]) & HV_ODD ? v[c] : u[c];
+            for (int j = 0; j < COLS; ++j) {
+                const mh_f4 v = t.value(i, j);
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    again |= __builtin_fabsf(v[c]) < 16.f && (wide || hv_wide(b[j][c])) && column(j) + c < cols;
+            }
+            if (again && row(i) < rows) {
+                at[row(i)] = (SPLIT ? a[i] & (HV_SMALLEST | HV_ODD) : a[i]) | HV_AGAIN;
+                some = HV_ODD;
+            }
         }
-        return v;
+        if (some & HV_ODD) *any = 1u;
     }
 };
 
-// mm_rows_body on halves: A rows [R][Kp / 32][2][32] with their peaks pa [R]; B either rows, [E][N][Kp / 32][2][32] with pb
-// [E][N], or (BS) columns of K contracted rows, [E][K][2][Np] with pb and marks mb [E][N].
+// mm_rows_body on halves: A rows [R][Kp / 32][2][32] with their words pa [R + 1]; B either rows, [E][N][Kp / 32][2][32] with words
+// pb [E][N], or (BS) columns of K contracted rows, [E][K][2][Np] with pb and mb [E][N].
 // Bound by the matrix cores: 20,000 x 1,024 x 1,024 in 128 us, 980 TFLOP/s of float16 products (three rounds of workgroups where
 // 2.45 would do), the cores busy 53 % of it.
 template <bool BS, int ACT, typename tile_t>
 __device__ __forceinline__ void hv_rows_body(const unsigned short* A, const unsigned short* B, float* C0, const float* bias,
-                                             const float* res, float* slope, const int* off, const unsigned* pa,
+                                             const float* res, float* slope, const int* off, unsigned* pa,
                                              const unsigned* pb, const unsigned* mb, long long ldr, int R, int N, int K, int E) {
     __shared__ mh_u4 lds[tile_t::LDS];
     const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT, Kp = (K + 31) / 32 * 32, Np = (N + 7) / 8 * 8;
@@ -231,21 +239,17 @@ __device__ __forceinline__ void hv_rows_body(const unsigned short* A, const unsi
     tile_t t;
     t.run(lds, a, 2 * Kp, rows, b, BS ? Np : 2 * Kp, brows, 0, 2 * Kp, BS ? 2 * K : 0);
     const long long col = (long long)e * N + n0;
-    hv_result<tile_t> r(t, C, N, pa + r0, nullptr, rows, pb + col, mb ? mb + col : nullptr, cols);
-    if (r.any_odd()) {
-        r.keep();
-        r.odd = true;
-        t.template run<true>(lds, a, 2 * Kp, rows, b, BS ? Np : 2 * Kp, brows, 0, 2 * Kp, BS ? 2 * K : 0);
-    }
+    const hv_result<tile_t> r(t, pa + r0, nullptr, rows, pb + col, mb ? mb + col : nullptr, cols);
+    r.template mark<false>(pa + r0, pa + R);
     bias = bias ? bias + (long long)e * N : nullptr;
     if (n0 + tile_t::BN <= N) mm_store_tile<MM_F32, ACT, true>(r, r0, rows, n0, N, bias, res, ldr, slope, C0);
     else mm_store_tile<MM_F32, ACT, false>(r, r0, rows, n0, N, bias, res, ldr, slope, C0);
 }
 
-// mm_outer_body on halves: A columns [R][2][Mp], B columns [R][2][Np], peaks and marks [E][M] and [E][N].
+// mm_outer_body on halves: A columns [R][2][Mp], B columns [R][2][Np], their words [E][M], ma with one more behind, and [E][N].
 template <typename tile_t>
 __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const unsigned short* B, float* C0, float* part,
-                                              const int* off, const unsigned* pa, const unsigned* ma, const unsigned* pb,
+                                              const int* off, const unsigned* pa, unsigned* ma, const unsigned* pb,
                                               const unsigned* mb, int R, int M, int N, int E, int L) {
     __shared__ mh_u4 lds[tile_t::LDS];
     const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT, Mp = (M + 7) / 8 * 8, Np = (N + 7) / 8 * 8;
@@ -265,12 +269,8 @@ __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const uns
     t.run(lds, a, Mp, ar, b, Np, br, 0, 2 * (r1 - r0));
     float* C = (L ? part + (long long)blockIdx.y * M * N : C0 + (long long)e * M * N) + (long long)m0 * N + n0;
     const long long ra = (long long)e * M + m0, rb = (long long)e * N + n0;
-    hv_result<tile_t> r(t, C, N, pa + ra, ma + ra, rows, pb + rb, mb + rb, cols);
-    if (r.any_odd()) {
-        r.keep();
-        r.odd = true;
-        t.template run<true>(lds, a, Mp, ar, b, Np, br, 0, 2 * (r1 - r0));
-    }
+    const hv_result<tile_t> r(t, pa + ra, ma + ra, rows, pb + rb, mb + rb, cols);
+    r.template mark<true>(ma + ra, ma + (long long)E * M);
 #pragma unroll
     for (int i = 0; i < tile_t::ROWS; ++i)
 #pragma unroll
@@ -278,4 +278,43 @@ __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const uns
             if (tile_t::row(i) < rows && tile_t::column(j) < cols)
                 mm_put4<MM_F32>(C + (long long)tile_t::row(i) * N + tile_t::column(j), r.value(i, j),
                                 cols - tile_t::column(j));
+}
+
+// Whether a tile's rows or columns hold a marked one: the workgroup's answer, and the barrier between two tiles' products.
+struct hv_marked {
+    const unsigned *pa, *ma, *pb, *mb;
+    int M, N;                                            // words a group of rows (0: none) and of columns
+    __device__ __forceinline__ bool operator()(int e, int m0, int rows, int n0, int cols) const {
+        if (e < 0) return false;
+        unsigned any = 0;
+        for (int i = threadIdx.x; i < rows; i += blockDim.x) any |= hv_read(pa, ma, (long long)e * M + m0 + i);
+        for (int i = threadIdx.x; i < cols; i += blockDim.x) any |= hv_read(pb, mb, (long long)e * N + n0 + i);
+        return __syncthreads_or((any & (HV_AGAIN | HV_ODD)) != 0u);
+    }
+};
+
+// After hv_rows_body: the tiles with marked results once more, by the direct kernel from the operands themselves.  Workgroups walk
+// the `tiles` where there is anything to do; where not, as nearly always, this costs a launch and one load.
+template <bool BS, int ACT, typename tile_t>
+__device__ __forceinline__ void hv_again_rows_body(const float* A, const float* B, float* C, const float* bias, const float* res,
+                                                   float* slope, const int* off, const unsigned* pa, const unsigned* pb,
+                                                   const unsigned* mb, long long lda, long long ldb, long long ldr, int R, int N,
+                                                   int K, int E, int tiles) {
+    if (!pa[R]) return;
+    const hv_marked marked = {pa, nullptr, pb, mb, 0, N};
+    for (int b = blockIdx.x; b < tiles; b += gridDim.x)
+        mm_rows_body<MM_F32, BS, ACT, tile_t>(A, B, C, bias, res, slope, off, lda, ldb, ldr, R, N, K, E, b, tiles, marked);
+}
+
+// After hv_outer_body, of `tiles` tiles in each group or slot.
+template <typename tile_t>
+__device__ __forceinline__ void hv_again_outer_body(const float* A, const float* B, float* C, float* part, const int* off,
+                                                    const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb,
+                                                    long long lda, long long ldb, int R, int M, int N, int E, int L, int tiles,
+                                                    int slots) {
+    if (!ma[(long long)E * M]) return;
+    const hv_marked marked = {pa, ma, pb, mb, M, N};
+    for (long long i = blockIdx.x; i < (long long)tiles * slots; i += gridDim.x)
+        mm_outer_body<MM_F32, tile_t>(A, B, C, part, off, lda, ldb, R, M, N, E, L, (int)(i % tiles), tiles, (int)(i / tiles),
+                                      marked);
 }

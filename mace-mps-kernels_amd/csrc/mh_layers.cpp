@@ -171,16 +171,16 @@ struct Halves {
 };
 
 Halves halves_of_rows(mh_module* split, const Tensor& x, int64_t ld, int64_t R, int64_t K) {
-    Halves h{at::empty({R * 2 * up(K, 32)}, x.options().dtype(at::kUInt16)), at::empty({R}, x.options().dtype(at::kInt))};
+    Halves h{at::empty({R * 2 * up(K, 32)}, x.options().dtype(at::kUInt16)), at::empty({R + 1}, x.options().dtype(at::kInt))};
     launch("hv_rows", [&] { return mh_hv_rows(split, f32(x), ld, u16(h.y), u32(h.peak), R, K, stream_of(x)); });
     return h;
 }
 
-// columns scaled per group of rows: by offsets, else equal groups; peak [2][groups][C]: peaks and marks
+// columns scaled per group of rows: by offsets, else equal groups; peak [2][groups][C] and a word more
 Halves halves_of_columns(mh_module* split, const Tensor& x, int64_t ld, int64_t R, int64_t C, int64_t groups,
                          const Tensor& off) {
     Halves h{at::empty({R * 2 * up(C, 8)}, x.options().dtype(at::kUInt16)),
-             at::zeros({2 * groups * C}, x.options().dtype(at::kInt))};
+             at::zeros({2 * groups * C + 1}, x.options().dtype(at::kInt))};
     const int64_t G = off.defined() ? 0 : R / groups;
     // pieces of rows for about eight workgroups per compute unit
     const int64_t L = std::min<int64_t>(256, std::max<int64_t>(16, up((R * ((C + 255) / 256) + 2047) / 2048, 4)));
@@ -190,6 +190,9 @@ Halves halves_of_columns(mh_module* split, const Tensor& x, int64_t ld, int64_t 
     });
     return h;
 }
+
+// workgroups that compute marked tiles again: three on each compute unit
+const int kAgain = 768;
 
 struct DenseArgs {
     Tensor x, w;         // x [R, K] with ld between rows, w contiguous
@@ -229,6 +232,10 @@ Tensor dense_forward(DenseArgs a, const Tensor& like, const Tensor& b, const Ten
         launch("hv_fwd", [&] {
             return mh_hv_mm(p.module(F_MODULE), u16(h.y), u16(c.y), f32(out), f32(b), f32(r), ldr, static_cast<float*>(sl),
                             i32(off), u32(h.peak), u32(c.peak), nullptr, R, n, K, groups, s);
+        });
+        launch("hv_again", [&] {
+            return mh_hv_again_mm(p.module(F_MODULE), f32(a.x), a.ld, f32(a.w), K, f32(out), f32(b), f32(r), ldr,
+                                  static_cast<float*>(sl), i32(off), u32(h.peak), u32(c.peak), nullptr, R, n, K, groups, kAgain, s);
         });
         return out;
     }
@@ -326,6 +333,10 @@ struct DenseFn : torch::autograd::Function<DenseFn> {
                 return mh_hv_mm(p.module(B_ROWS), u16(a.y), u16(c.y), f32(dx), nullptr, nullptr, 0, nullptr, i32(off),
                                 u32(a.peak), u32(c.peak), u32(c.peak) + groups * K, R, K, N, groups, s);
             });
+            launch("hv_again", [&] {
+                return mh_hv_again_mm(p.module(B_ROWS), f32(g), ldg, f32(w), K, f32(dx), nullptr, nullptr, 0, nullptr, i32(off),
+                                      u32(a.peak), u32(c.peak), u32(c.peak) + groups * K, R, K, N, groups, kAgain, s);
+            });
         }
         if (p[B_DW_HALVES]) {
             const Halves a = halves_of_columns(split, g, ldg, R, N, groups, off);
@@ -334,6 +345,11 @@ struct DenseFn : torch::autograd::Function<DenseFn> {
                 return mh_hv_outer(p.module(B_OUTER), u16(a.y), u16(c.y), f32(dw), f32(part), i32(off), u32(a.peak),
                                    u32(a.peak) + groups * N, u32(c.peak), u32(c.peak) + groups * K, R, N, K, groups, p[B_LO],
                                    p[B_SLOTS_O], s);
+            });
+            launch("hv_again", [&] {
+                return mh_hv_again_outer(p.module(B_OUTER), f32(g), ldg, f32(x), ldx, f32(dw), f32(part), i32(off), u32(a.peak),
+                                         u32(a.peak) + groups * N, u32(c.peak), u32(c.peak) + groups * K, R, N, K, groups,
+                                         p[B_LO], p[B_SLOTS_O], kAgain, s);
             });
             if (p[B_LO])
                 launch("mm_sum", [&] { return mh_mm_sum(sums, f32(part), ptr(dw), i32(off), R, groups, p[B_LO], N * K, s); });

@@ -601,6 +601,7 @@ struct mm_fast_tile {
     static constexpr bool WHOLE_STEPS = true;
     static constexpr int TA = BM * BK / 8, TB = BN * BK / 8, LDS = 2 * (TA + TB);
     mh_f4 acc[FM][FN];
+    mh_f4 low[HALVES ? FM : 1][HALVES ? FN : 1];         // the products with a lower half, which is kept times 2^12
 
     // Fragments of 16 rows each from row0 on at k 32 ks .. + 31: contiguous operands by 16-byte reads; strided ones by
     // transposing reads, where sixteen lanes read four k of 16 rows (lane i: four rows of k i / 4) and lane i receives the
@@ -628,28 +629,26 @@ struct mm_fast_tile {
         }
     }
 
-    template <bool TOP>
     __device__ __forceinline__ void products(mh_u4* a, mh_u4* b) {
         const int wave = threadIdx.x >> 6, ra = (wave / WN) * 16 * FM, rb = (wave % WN) * 16 * FN;
         if constexpr (HALVES) {
-            // upper times upper, upper times lower, lower times upper (TOP: the first alone)
+            // upper times upper, upper times lower, lower times upper
             mh_u4 fa[FM], fb[2][FN];
             fragments<BS, BN, FN>(fb[0], b, rb, 0);
-            if constexpr (!TOP) fragments<BS, BN, FN>(fb[1], b, rb, 1);
+            fragments<BS, BN, FN>(fb[1], b, rb, 1);
             fragments<AS, BM, FM>(fa, a, ra, 0);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
                 for (int j = 0; j < FN; ++j) {
                     acc[i][j] = mm_mfma<TY>(fb[0][j], fa[i], acc[i][j]);
-                    if constexpr (!TOP) acc[i][j] = mm_mfma<TY>(fb[1][j], fa[i], acc[i][j]);
+                    low[i][j] = mm_mfma<TY>(fb[1][j], fa[i], low[i][j]);
                 }
-            if constexpr (TOP) return;
             fragments<AS, BM, FM>(fa, a, ra, 1);
 #pragma unroll
             for (int i = 0; i < FM; ++i)
 #pragma unroll
-                for (int j = 0; j < FN; ++j) acc[i][j] = mm_mfma<TY>(fb[0][j], fa[i], acc[i][j]);
+                for (int j = 0; j < FN; ++j) low[i][j] = mm_mfma<TY>(fb[0][j], fa[i], low[i][j]);
             return;
         }
 #pragma unroll
@@ -666,7 +665,6 @@ struct mm_fast_tile {
 
     // The loads of the next tile (where `left` > 0) and this one's products.  The four places are distinct: without that the
     // compiler waits for the loads before it reads the tile that is there.
-    template <bool TOP>
     __device__ __forceinline__ void step(const mm_mover<AS, BM, BK, THREADS, HALVES>& ma,
                                          const mm_mover<BS, BN, BK, THREADS, HALVES>& mb, const T* A, const T* B, int left,
                                          int bleft, mh_u4* __restrict__ a, mh_u4* __restrict__ b, mh_u4* __restrict__ an,
@@ -675,11 +673,10 @@ struct mm_fast_tile {
             ma.issue(A, left, an);
             mb.issue(B, bleft, bn);
         }
-        products<TOP>(a, b);
+        products(a, b);
     }
 
     // `bend`: where B's k end, if before A's (whose padding is zeros); 0: with A's
-    template <bool TOP = false>
     __device__ __forceinline__ void run(mh_u4* lds, const T* A, long long lda, int arows, const T* B, long long ldb, int brows,
                                         int kbeg, int kend, int bend = 0) {
         if (!bend) bend = kend;
@@ -691,7 +688,10 @@ struct mm_fast_tile {
 #pragma unroll
         for (int i = 0; i < FM; ++i)
 #pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mh_f4{0.f, 0.f, 0.f, 0.f};
+            for (int j = 0; j < FN; ++j) {
+                acc[i][j] = mh_f4{0.f, 0.f, 0.f, 0.f};
+                if constexpr (HALVES) low[i][j] = mh_f4{0.f, 0.f, 0.f, 0.f};
+            }
         if (kbeg >= kend) return;                       // uniform over the workgroup
         mh_u4 *a0 = lds, *a1 = lds + TA, *b0 = lds + 2 * TA, *b1 = lds + 2 * TA + TB;
         ma.issue(A + kbeg * sa, kend - kbeg, a0);
@@ -700,7 +700,7 @@ struct mm_fast_tile {
             // the tile of this step is in LDS, and every wave is done with the other buffer
             __builtin_amdgcn_s_waitcnt(0x0F70);         // vmcnt(0)
             __syncthreads();
-            step<TOP>(ma, mb, A + (k + BK) * sa, B + (k + BK) * sb, kend - k - BK, bend - k - BK, a0, b0, a1, b1);
+            step(ma, mb, A + (k + BK) * sa, B + (k + BK) * sb, kend - k - BK, bend - k - BK, a0, b0, a1, b1);
             mh_u4* t = a0;
             a0 = a1;
             a1 = t;
@@ -714,7 +714,10 @@ struct mm_fast_tile {
     __device__ __forceinline__ static int column(int j) {
         return ((threadIdx.x >> 6) % WN) * 16 * FN + 4 * (threadIdx.x >> 4 & 3) + 16 * j;
     }
-    __device__ __forceinline__ mh_f4 value(int i, int j) const { return acc[i][j]; }
+    __device__ __forceinline__ mh_f4 value(int i, int j) const {
+        if constexpr (HALVES) return acc[i][j] + low[i][j] * 0x1p-12f;
+        else return acc[i][j];
+    }
 };
 
 // The length of a strided operand's rows as a tile may load them: whole steps of 16 bytes where it goes straight to LDS (rows
@@ -851,20 +854,28 @@ __device__ __forceinline__ void mm_store_lines(const tile_t& t, mh_u4* lds, long
     }
 }
 
+// Every tile is wanted: what the bodies below ask before a tile's products (mh_halves.h asks otherwise).
+struct mm_every {
+    __device__ __forceinline__ bool operator()(int, int, int, int, int) const { return true; }
+};
+
 // Forward and input gradient: R rows of A [R, K] in groups, B the group's weights ([N, K], or [K, N] where BS), the
-// epilogue v = sums + bias[e]; slope = act'(v); C = act(v) + res.  Rows of no group are written as zeros.
-template <int TY, bool BS, int ACT, typename tile_t>
+// epilogue v = sums + bias[e]; slope = act'(v); C = act(v) + res.  Rows of no group are written as zeros.  `b` of `blocks`
+// tiles; wanted(e, first row, rows, first column, columns): whether to write it (e -1: rows of no group).
+template <int TY, bool BS, int ACT, typename tile_t, typename wanted_t = mm_every>
 __device__ __forceinline__ void mm_rows_body(const void* A_, const void* B_, void* C_, const void* bias_, const void* res_,
                                              void* slope_, const int* off, long long lda, long long ldb, long long ldr, int R, int N,
-                                             int K, int E) {
+                                             int K, int E, int b = blockIdx.x, int blocks = gridDim.x,
+                                             wanted_t wanted = wanted_t()) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
-    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT;
+    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = blocks / NT;
     int mt, nt, e, r0, r1;
-    mm_tile_of(blockIdx.x, gridDim.x, MT, NT, mt, nt);
+    mm_tile_of(b, blocks, MT, NT, mt, nt);
     const bool live = mm_slot(off, E, R, tile_t::BM, mt, e, r0, r1);
     if (r0 >= R) return;
     const int n0 = nt * tile_t::BN, rows = r1 - r0;
+    if (!wanted(e, r0, rows, n0, min(N - n0, tile_t::BN))) return;
     T* C = static_cast<T*>(C_) + (long long)r0 * N + n0;
     tile_t t;
     if (!live) {
@@ -996,31 +1007,34 @@ __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void
     }
 }
 
-// Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  blockIdx.y is
-// the group (L 0: all its rows; none give zeros), or a slot of at most L of its rows whose sums go to part[slot] in float32.
+// Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  y is the group
+// (L 0: all its rows; none give zeros), or a slot of at most L of its rows whose sums go to part[slot] in float32; tile `b` of
+// `blocks`; wanted as in mm_rows_body, of the result's rows and columns.
 // Bound as the other products; 16,384 rows of 4,096 by 1,024 in bfloat16 in four pieces take 140 us and 10 for their sum
 // (980 TFLOP/s), eight groups of 2,048 rows of 2,048 by 1,024 whole 75 us.
-template <int TY, typename tile_t>
+template <int TY, typename tile_t, typename wanted_t = mm_every>
 __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, void* C_, float* part, const int* off,
-                                              long long lda, long long ldb, int R, int M, int N, int E, int L) {
+                                              long long lda, long long ldb, int R, int M, int N, int E, int L, int b = blockIdx.x,
+                                              int blocks = gridDim.x, int y = blockIdx.y, wanted_t wanted = wanted_t()) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
-    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT;
+    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = blocks / NT;
     int mt, nt, e = 0, r0 = 0, r1 = R;
-    mm_tile_of(blockIdx.x, gridDim.x, MT, NT, mt, nt);
+    mm_tile_of(b, blocks, MT, NT, mt, nt);
     if (L) {
-        if (!mm_slot(off, E, R, L, blockIdx.y, e, r0, r1)) return;
+        if (!mm_slot(off, E, R, L, y, e, r0, r1)) return;
     } else if (off) {
-        e = mm_by_length(off, E, blockIdx.y);
+        e = mm_by_length(off, E, y);
         r0 = min(max(off[e], 0), R);
         r1 = min(max(off[e + 1], r0), R);
     }
     const int m0 = mt * tile_t::BM, n0 = nt * tile_t::BN;
+    if (!wanted(e, m0, min(M - m0, tile_t::BM), n0, min(N - n0, tile_t::BN))) return;
     tile_t t;
     t.run(lds, static_cast<const T*>(A_) + (long long)r0 * lda + m0, lda, min(mm_wide<tile_t, true>(M) - m0, tile_t::BM),
           static_cast<const T*>(B_) + (long long)r0 * ldb + n0, ldb, min(mm_wide<tile_t, true>(N) - n0, tile_t::BN), 0,
           r1 - r0);
-    const long long at = (long long)(L ? (int)blockIdx.y : e) * M * N;
+    const long long at = (long long)(L ? y : e) * M * N;
 #pragma unroll
     for (int i = 0; i < tile_t::ROWS; ++i)
 #pragma unroll

@@ -30,9 +30,9 @@ MH_CONV_FWD, MH_CONV_BWD, MH_CONV_BWD_WY, MH_SC_FWD, MH_SC_BWD, MH_CONV_BWD_R, M
     MH_EDGE_BWD, MH_MLP_BWD_P, MH_LIN_BWD_SUM, MH_MLP_H3T, MH_CONV_BWD_T, \
     MH_GEOM_STRAIN, MH_GEOM_DET, MH_MLP_BWD_W, MH_MM_ROWS, MH_MM_OUTER, MH_MM_SUM, MH_MM_SLOPE, MH_EXPERT_HIST, \
     MH_EXPERT_PLACE, MH_DISPATCH, MH_COMBINE, MH_COMBINE_BWD, MH_NORM_FWD, MH_NORM_BWD, MH_HV_ROWS, \
-    MH_HV_PEAKS, MH_HV_COLUMNS, MH_HV_MM, MH_HV_OUTER, MH_MM_PAD = range(101)
+    MH_HV_PEAKS, MH_HV_COLUMNS, MH_HV_MM, MH_HV_OUTER, MH_MM_PAD, MH_HV_AGAIN = range(102)
 MH_WANT_GX, MH_WANT_GWY, MH_CUT_MASKED, MH_CUT_NOZERO = 1, 2, 4, 8
-ABI_VERSION = 50
+ABI_VERSION = 51
 
 # hipcc/hipRTC options for every generated layer: gfx950 code, -O3, and packed-FP32 instructions disabled.
 ARCH = os.environ.get('MACE_HIP_ARCH', 'gfx950')
@@ -143,6 +143,8 @@ _SIGS = {
     'mh_hv_columns': (ctypes.c_int, [_P, _P, _L] + [_P] * 3 + [_I] * 6 + [_P]),
     'mh_hv_mm': (ctypes.c_int, [_P] * 6 + [_L] + [_P] * 5 + [_I] * 4 + [_P]),
     'mh_hv_outer': (ctypes.c_int, [_P] * 10 + [_I] * 6 + [_P]),
+    'mh_hv_again_mm': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 3 + [_L] + [_P] * 5 + [_I] * 5 + [_P]),
+    'mh_hv_again_outer': (ctypes.c_int, [_P, _P, _L, _P, _L] + [_P] * 7 + [_I] * 7 + [_P]),
     'mh_expert_order': (ctypes.c_int, [_P, _P] + [_I] * 3 + [_P, _I] + [_P] * 4),
     'mh_dispatch': (ctypes.c_int, [_P, _P, _L] + [_P] * 3 + [_I] * 5 + [_P]),
     'mh_combine': (ctypes.c_int, [_P] * 5 + [_L, _P] + [_I] * 4 + [_P]),

@@ -14,6 +14,8 @@ from . import _native
 # (with four waves 171 us where these take 166, at 20,000 x 1,024 x 1,024 with the halves' making; 256 x 256 about 220)
 TILE = 2, 4, 4, 2
 SIDE = 128
+# the direct tile of what is computed again (matmul.SLOW's of 64 x 64)
+AGAIN, AGAIN_SIDE = (4, 2, 1, 2, 64), 64
 
 
 def pays(rows, n, K, groups, mode, product, direct):
@@ -24,7 +26,7 @@ def pays(rows, n, K, groups, mode, product, direct):
     91, 126 / 132; 5,000 x 512 x 512 26 / 36, 28 / 28, 41 / 58; 20,000 x 128 x 512 forward 30 / 40."""
     moved = {'fwd': 8 * (rows * K + groups * n * K), 'dx': 8 * rows * n + 12 * groups * n * K,
              'dw': 12 * rows * (n + K)}[mode]
-    return 1.1 * (product + moved / 4.5e12 + (15e-6 if mode == 'dw' else 8e-6)) < direct
+    return 1.1 * (product + moved / 4.5e12 + (18e-6 if mode == 'dw' else 11e-6)) < direct
 
 
 def source(mode, act=0):
@@ -37,15 +39,25 @@ def source(mode, act=0):
           'tile_t;',
           f'extern "C" __global__ __launch_bounds__(tile_t::THREADS) void hv_{mode}(const unsigned short* A, '
           'const unsigned short* B, float* C, ']
+    again = [f'typedef mm_tile<MM_F32, {b(mode == "dw")}, {b(mode != "fwd")}, {", ".join(map(str, AGAIN))}> again_t;',
+             f'extern "C" __global__ __launch_bounds__(again_t::THREADS) void hv_again_{mode}(const float* A, const float* B, '
+             'float* C, ']
     if mode == 'dw':
-        L += ['float* part, const int* off, const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb, '
+        L += ['float* part, const int* off, const unsigned* pa, unsigned* ma, const unsigned* pb, const unsigned* mb, '
               'int R, int M, int N, int E, int L) {',
-              '  hv_outer_body<tile_t>(A, B, C, part, off, pa, ma, pb, mb, R, M, N, E, L);', '}']
+              '  hv_outer_body<tile_t>(A, B, C, part, off, pa, ma, pb, mb, R, M, N, E, L);', '}', *again,
+              'float* part, const int* off, const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb, '
+              'long long lda, long long ldb, int R, int M, int N, int E, int L, int tiles, int slots) {',
+              '  hv_again_outer_body<again_t>(A, B, C, part, off, pa, ma, pb, mb, lda, ldb, R, M, N, E, L, tiles, slots);', '}']
     else:
-        L += ['const float* bias, const float* res, float* slope, const int* off, const unsigned* pa, const unsigned* pb, '
+        L += ['const float* bias, const float* res, float* slope, const int* off, unsigned* pa, const unsigned* pb, '
               'const unsigned* mb, long long ldr, int R, int N, int K, int E) {',
               f'  hv_rows_body<{b(mode == "dx")}, {act}, tile_t>(A, B, C, bias, res, slope, off, pa, pb, mb, ldr, R, N, K, E);',
-              '}']
+              '}', *again,
+              'const float* bias, const float* res, float* slope, const int* off, const unsigned* pa, const unsigned* pb, '
+              'const unsigned* mb, long long lda, long long ldb, long long ldr, int R, int N, int K, int E, int tiles) {',
+              f'  hv_again_rows_body<{b(mode == "dx")}, {act}, again_t>(A, B, C, bias, res, slope, off, pa, pb, mb, lda, ldb, ldr, '
+              'R, N, K, E, tiles);', '}']
     return '\n'.join(L) + '\n'
 
 
@@ -58,4 +70,5 @@ def module(device, mode, act=0):
             return _native.Module(code, {_native.MH_HV_ROWS: ('hv_rows', 256, 1), _native.MH_HV_PEAKS: ('hv_peaks', 256, 1),
                                          _native.MH_HV_COLUMNS: ('hv_columns', 256, 1)})
         kind = _native.MH_HV_OUTER if mode == 'dw' else _native.MH_HV_MM
-        return _native.Module(code, {kind: (f'hv_{mode}', 64 * TILE[0] * TILE[1], SIDE, SIDE)})
+        return _native.Module(code, {kind: (f'hv_{mode}', 64 * TILE[0] * TILE[1], SIDE, SIDE), _native.MH_HV_AGAIN: (
+            f'hv_again_{mode}', 64 * AGAIN[0] * AGAIN[1], AGAIN_SIDE, AGAIN_SIDE)})

@@ -10,7 +10,8 @@ bfloat16 and float16, for any number of rows from none on and any widths.
 A drop-in of ``patch_model`` holds its weights as constants; these are what a model trains next to it.  The kernels are in
 ``csrc/mh_matmul.h``, one hipRTC module per type, product and tile; here is what chooses between them by sizes, types and
 alignment, and ``csrc/mh_layers.cpp`` runs them.  A float32 product runs on the bf16 matrix cores at float32 accuracy
-(operands split into three bf16 parts, six partial products; large ones as three products of float16 halves, ``halves``);
+(operands split into three bf16 parts, six partial products; large ones as three products of float16 halves, ``halves``,
+with what these do not hold computed the first way);
 16-bit operands run as they are; every sum is float32 and rounded once.  The backward keeps act'(a) of the forward, not a
 itself, and rounds p = g act'(a) to the type before the products that contract it.  Sums over rows that are split over
 workgroups are added in a fixed order, so results are bitwise repeatable.  The reference has no such layers.

@@ -1,6 +1,7 @@
 """
 The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
-that a tile cannot take, forward-mode derivatives, units far in an activation's tail.
+that a tile cannot take, forward-mode derivatives, units far in an activation's tail, products of very unlike
+magnitudes.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -170,3 +171,67 @@ def test_gradients_of_units_in_the_tail(T, act, dt):
     for name, got, val, e, n in (('dx', dx, p @ w, (err @ w.abs(), p.abs() @ w.abs()), N),
                                  ('dw', dw, p.t() @ x, (err.t() @ x.abs(), p.abs().t() @ x.abs()), T)):
         near(name, got, val, e[0] + (n + 16) * E32 * e[1] + U[dt] * (val.abs() + e[0]) + TINY[dt])
+
+
+# ------------------------------------------------------------------------------------------ unlike magnitudes
+def _products(x, w, g, scale=None):
+    """y, dx and dw of float32 tensors within the bound of a float32 sum: (n + 16) 2^-24 of the magnitudes added."""
+    lx, lw = x.cuda().requires_grad_(), w.cuda().requires_grad_()
+    y = mhk.dense(lx, lw)
+    dx, dw = torch.autograd.grad(y, (lx, lw), g.cuda())
+    x, w, g = x.double(), w.double(), g.double()
+    for name, got, a, b in (('y', y, x, w.t()), ('dx', dx, g, w), ('dw', dw, g.t(), x)):
+        near(name, got, a @ b, (a.shape[1] + 16) * E32 * (a.abs() @ b.abs()))
+
+
+@pytest.mark.parametrize('power', [4, 5, 9])
+@pytest.mark.parametrize('K', [64, 1024])
+def test_contractions_of_unlike_magnitudes_by_halves(K, power, by_halves):  # noqa: F811
+    """Operands whose magnitudes along the contraction are each other's inverse, in units that differ by up to 10^18: every
+    product counts alike, however small its factor is in its row."""
+    dev()
+    print(f'[case] unlike magnitudes K={K} power={power}', flush=True)
+    rng = np.random.default_rng(K + power)
+    T, N = 200, 160
+    s = torch.logspace(-power, power, K)[torch.randperm(K, generator=torch.Generator().manual_seed(1))]
+    _products(rand(rng, T, K) * s, rand(rng, N, K) / s, rand(rng, T, N))
+    s = torch.logspace(-power, power, N)
+    _products(rand(rng, T, K), rand(rng, N, K) / s[:, None], rand(rng, T, N) * s)
+    s = torch.logspace(-power, power, T)
+    _products(rand(rng, T, K) / s[:, None], rand(rng, N, K), rand(rng, T, N) * s[:, None])
+
+
+@pytest.mark.parametrize('size', [1e8, 1e10, 1e20])
+def test_one_large_value_by_halves(size, by_halves):  # noqa: F811
+    """A value far above its row's others that meets a weight of zero leaves the others' sum its accuracy."""
+    d = dev()
+    print(f'[case] one value of {size}', flush=True)
+    rng = np.random.default_rng(3)
+    T, K, N = 150, 300, 140
+    x, w, g = rand(rng, T, K), rand(rng, N, K), rand(rng, T, N)
+    x[7, 5], x[90, 250], w[33, 7], g[50, 60] = size, -size, size, size
+    w[::2, 5], w[1::2, 250], x[::2, 7], w[60, ::3], x[50, ::2] = 0, 0, 0, 0, 0
+    _products(x, w, g)
+    off = torch.tensor([0, 100, 150], dtype=torch.int32, device=d)
+    lx, lw = x.to(d).requires_grad_(), torch.stack([w, w.flip(0)]).to(d).requires_grad_()
+    y = mhk.expert_dense(lx, lw, off)
+    dx, dw = torch.autograd.grad(y, (lx, lw), g.to(d))
+    for e, (i, j) in enumerate(((0, 100), (100, 150))):
+        a, b, c = x[i:j].double(), lw[e].detach().cpu().double(), g[i:j].double()
+        for name, got, l, r in (('y', y[i:j], a, b.t()), ('dx', dx[i:j], c, b), ('dw', dw[e], c.t(), a)):
+            near(f'{name} of {e}', got, l @ r, (l.shape[1] + 16) * E32 * (l.abs() @ r.abs()))
+
+
+def test_infinities_that_meet_small_values_by_halves(by_halves):  # noqa: F811
+    """An infinity times any other value than zero is infinite, however small that is in its row."""
+    d = dev()
+    print('[case] infinities and small values', flush=True)
+    rng = np.random.default_rng(4)
+    T, K, N = 150, 96, 140
+    x, w = rand(rng, T, K), rand(rng, N, K)
+    w[:, 5] = torch.where(torch.arange(N) % 2 == 0, 1e-30, -1e-25)
+    w[3, 5] = 0
+    x[2, 5], x[100, 5] = float('inf'), float('-inf')
+    got, want = mhk.dense(x.to(d), w.to(d)).cpu(), (x.double() @ w.double().t())
+    assert torch.isnan(want[2, 3]) and torch.isinf(want[2, :3]).all()
+    assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[[2, 100]].double().nan_to_num(7), want[[2, 100]].nan_to_num(7))
