@@ -258,9 +258,7 @@ __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const uns
     if (L) {
         if (!mm_slot(off, E, R, L, blockIdx.y, e, r0, r1)) return;
     } else if (off) {
-        e = mm_by_length(off, E, blockIdx.y);
-        r0 = min(max(off[e], 0), R);
-        r1 = min(max(off[e + 1], r0), R);
+        mm_by_length(off, E, R, blockIdx.y, e, r0, r1);
     }
     const int m0 = mt * tile_t::BM, n0 = nt * tile_t::BN, rows = min(M - m0, tile_t::BM), cols = min(N - n0, tile_t::BN);
     const unsigned short *a = A + (long long)r0 * 2 * Mp + m0, *b = B + (long long)r0 * 2 * Np + n0;

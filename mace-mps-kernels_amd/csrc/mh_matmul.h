@@ -233,12 +233,35 @@ __device__ __forceinline__ unsigned mm_slope_codes(float lo, float hi) {
 }
 
 // ------------------------------------------------------------------------------------------------ groups of rows
-// Rows [0, R) in E groups, group e from off[e] to off[e + 1]; each group is cut into pieces of L rows, and slot s is the
-// s-th piece.  False past the last one; the rows of no group then follow as pieces with e = -1, those before the first group
-// and those behind the last.  off NULL: one group of all rows.  Offsets are clamped into [0, R] and to the largest before
-// them, so whatever they hold, groups are disjoint, no piece leads out of the tensors, and there are at most R / L + E
-// of them (R / L + E + 2 with those of no group).  Every lane of a wave calls (64 groups at a time are scanned across it);
-// R + L < 2^31.
+// Rows [0, R) in E groups, group e from off[e] to off[e + 1].  Offsets are clamped into [0, R] and to the largest before them:
+// whatever they hold, groups are disjoint and lead nowhere out of the tensors, and every kernel takes the same rows for a
+// group.  64 groups at a time are scanned across a wave, every lane of which calls.
+struct mm_groups {
+    const int* __restrict__ off;
+    int E, R;
+    int lead;                                            // rows before the first group
+    int top;                                             // where the groups scanned so far end
+    int lo, hi;                                          // this lane's group of the 64 scanned last (empty past the last)
+    __device__ __forceinline__ mm_groups(const int* offsets, int groups, int rows) : off(offsets), E(groups), R(rows) {
+        top = lead = min(max(off[0], 0), R);
+    }
+    __device__ __forceinline__ void scan(int g0) {
+        const int lane = threadIdx.x & (MH_WAVE - 1);
+        hi = max(top, min(off[min(g0 + lane, E - 1) + 1], R));
+#pragma unroll
+        for (int d = 1; d < MH_WAVE; d <<= 1) {
+            const int t = __shfl_up(hi, d, MH_WAVE);
+            if (lane >= d) hi = max(hi, t);
+        }
+        const int prev = __shfl_up(hi, 1, MH_WAVE);
+        lo = lane ? prev : top;
+        top = mh_bcast(hi, MH_WAVE - 1);
+    }
+};
+
+// Each group is cut into pieces of L rows, and slot s is the s-th piece.  False past the last one; the rows of no group then
+// follow as pieces with e = -1, those before the first group and those behind the last.  off NULL: one group of all rows.
+// There are at most R / L + E pieces (R / L + E + 2 with those of no group); R + L < 2^31.
 __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int R, int L, int s, int& e, int& r0, int& r1) {
     if (!off) {
         e = 0;
@@ -246,17 +269,12 @@ __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int 
         r1 = min(R, r0 + L);
         return r0 < R;
     }
-    const int lane = threadIdx.x & (MH_WAVE - 1), lead = min(max(off[0], 0), R);
-    int base = 0, top = lead;                            // pieces and rows before these 64 groups
+    const int lane = threadIdx.x & (MH_WAVE - 1);
+    mm_groups g(off, E, R);
+    int base = 0;                                        // pieces before these 64 groups
     for (int g0 = 0; g0 < E; g0 += MH_WAVE) {
-        int hi = max(top, min(off[min(g0 + lane, E - 1) + 1], R));
-#pragma unroll
-        for (int d = 1; d < MH_WAVE; d <<= 1) {
-            const int t = __shfl_up(hi, d, MH_WAVE);
-            if (lane >= d) hi = max(hi, t);
-        }
-        const int prev = __shfl_up(hi, 1, MH_WAVE), lo = lane ? prev : top;
-        const int n = g0 + lane < E ? (hi - lo + L - 1) / L : 0;
+        g.scan(g0);
+        const int n = (g.hi - g.lo + L - 1) / L;
         int inc = n;
 #pragma unroll
         for (int d = 1; d < MH_WAVE; d <<= 1) {
@@ -266,39 +284,46 @@ __device__ __forceinline__ bool mm_slot(const int* __restrict__ off, int E, int 
         const int total = mh_bcast(inc, MH_WAVE - 1);
         if (s < base + total) {
             const int l = __ffsll((unsigned long long)__ballot(base + inc > s)) - 1;
-            const int glo = mh_bcast(lo, l), ghi = mh_bcast(hi, l), before = mh_bcast(inc - n, l);
+            const int glo = mh_bcast(g.lo, l), ghi = mh_bcast(g.hi, l), before = mh_bcast(inc - n, l);
             e = g0 + l;
             r0 = glo + (s - base - before) * L;
             r1 = min(ghi, r0 + L);
             return true;
         }
         base += total;
-        top = mh_bcast(hi, MH_WAVE - 1);
     }
     e = -1;
-    const int d = s - base, first = (lead + L - 1) / L;  // pieces before the first group
+    const int d = s - base, first = (g.lead + L - 1) / L;        // pieces before the first group
     if (d < first) {
         r0 = d * L;
-        r1 = min(lead, r0 + L);
+        r1 = min(g.lead, r0 + L);
     } else {
-        r0 = (int)min(top + (long long)(d - first) * L, (long long)R);
+        r0 = (int)min(g.top + (long long)(d - first) * L, (long long)R);
         r1 = min(R, r0 + L);
     }
     return false;
 }
 
-// The group that is k-th by length, longest first (up to 64 groups; more are taken as they come): workgroups start in the order
-// of their index, and a long group that starts last is what all others wait for.  Every lane of a wave calls.
-__device__ __forceinline__ int mm_by_length(const int* __restrict__ off, int E, int k) {
-    if (E > MH_WAVE) return k;
+// The rows of the group that is k-th by length, longest first (up to 64 groups; more are taken as they come): workgroups start in
+// the order of their index, and a long group that starts last is what all others wait for.  Every lane of a wave calls.
+__device__ __forceinline__ void mm_by_length(const int* __restrict__ off, int E, int R, int k, int& e, int& r0, int& r1) {
     const int lane = threadIdx.x & (MH_WAVE - 1);
-    const int n = lane < E ? off[lane + 1] - off[lane] : 0;
-    int rank = 0;
-    for (int g = 0; g < E; ++g) {
-        const int m = mh_bcast(n, g);
-        rank += m > n || (m == n && g < lane) ? 1 : 0;
+    mm_groups g(off, E, R);
+    int l = k % MH_WAVE;
+    for (int g0 = 0; g0 <= k - l; g0 += MH_WAVE) g.scan(g0);
+    if (E <= MH_WAVE) {
+        const int n = g.hi - g.lo;
+        int rank = 0;
+        for (int i = 0; i < E; ++i) {
+            const int m = mh_bcast(n, i);
+            rank += m > n || (m == n && i < lane) ? 1 : 0;
+        }
+        l = __ffsll((unsigned long long)__ballot(lane < E && rank == k)) - 1;
+        k = l;
     }
-    return __ffsll((unsigned long long)__ballot(lane < E && rank == k)) - 1;
+    e = k;
+    r0 = mh_bcast(g.lo, l);
+    r1 = mh_bcast(g.hi, l);
 }
 
 // ------------------------------------------------------------------------------------------------ operand tiles
@@ -1024,9 +1049,7 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
     if (L) {
         if (!mm_slot(off, E, R, L, y, e, r0, r1)) return;
     } else if (off) {
-        e = mm_by_length(off, E, y);
-        r0 = min(max(off[e], 0), R);
-        r1 = min(max(off[e + 1], r0), R);
+        mm_by_length(off, E, R, y, e, r0, r1);
     }
     const int m0 = mt * tile_t::BM, n0 = nt * tile_t::BN;
     if (!wanted(e, m0, min(M - m0, tile_t::BM), n0, min(N - n0, tile_t::BN))) return;

@@ -64,13 +64,16 @@ needs_gxx = pytest.mark.skipif(shutil.which('g++') is None, reason='needs g++')
 @needs_gxx
 def test_slots_cover_every_row_once(tmp_path):
     """Whatever the offsets hold, the pieces that a launch has room for cover every row once: a group's by its own, the rows
-    before, between and behind the groups by pieces of no group."""
-    lib = host_library(function('mh_matmul.h', 'mm_slot') + function('mace_hip.cpp', 'pieces') + """
+    before and behind the groups by pieces of no group; and whole groups are the rows that their pieces are."""
+    lib = host_library(function('mh_matmul.h', 'mm_groups') + function('mh_matmul.h', 'mm_slot') +
+                       function('mh_matmul.h', 'mm_by_length') + function('mace_hip.cpp', 'pieces') + """
 extern "C" long long count(const int* off, long long R, long long E, long long L) { return pieces(off, R, E, L); }
 extern "C" int slot(const int* off, int E, int R, int L, int s, int* out) { return mm_slot(off, E, R, L, s, out[0], out[1], out[2]); }
+extern "C" void group(const int* off, int E, int R, int k, int* out) { mm_by_length(off, E, R, k, out[0], out[1], out[2]); }
 """, tmp_path)
     lib.count.restype, lib.count.argtypes = ctypes.c_longlong, [ctypes.c_void_p] + [ctypes.c_longlong] * 3
     lib.slot.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 4 + [ctypes.c_void_p]
+    lib.group.argtypes = [ctypes.c_void_p] + [ctypes.c_int] * 3 + [ctypes.c_void_p]
     rng = random.Random(3)
     for n in range(600):
         R, E, L = rng.choice([1, 12, 100, 700]), rng.choice([1, 2, 3, 9, 130]), rng.choice([1, 16, 64, 256])
@@ -95,6 +98,13 @@ extern "C" int slot(const int* off, int E, int R, int L, int s, int* out) { retu
                 assert (got[r0:r1] == -2).all()
                 got[r0:r1] = e
         assert (got == of).all(), (off, R, L)
+        # whole groups are the same rows
+        got[:] = -1
+        for k in range(E):
+            lib.group(o.ctypes.data, E, R, k, out.ctypes.data)
+            assert 0 <= out[1] <= out[2] <= R
+            got[out[1]:out[2]] = out[0]
+        assert (got == of).all(), (off, R)
 
 
 @needs_gxx

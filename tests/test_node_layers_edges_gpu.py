@@ -87,6 +87,33 @@ def test_a_slice_of_the_experts(dt):
     assert torch.equal(part[a:z], whole[a:z]) and (part[:a] == 0).all() and (part[z:] == 0).all()
 
 
+@pytest.mark.parametrize('dt', [F32, BF16], ids=['f32', 'bf16'])
+def test_every_product_takes_the_same_rows_for_a_group(dt, monkeypatch):
+    """Offsets that decrease: a row belongs to the group that the forward gives it in every gradient too, whether sums over rows
+    are cut into pieces or not."""
+    d = dev()
+    rng = np.random.default_rng(12)
+    R, K, N = 60, 24, 16
+    x, w, b, g = rand(rng, R, K, dt=dt), rand(rng, 3, N, K, dt=dt), rand(rng, 3, N, dt=dt), rand(rng, R, N, dt=dt)
+    off = torch.tensor([-4, 10, 5, 50], dtype=torch.int32, device=d)       # rows 0 to 9, none, 10 to 49
+    for L, slots in ((0, 3), (64, 4)):
+        print(f'[case] decreasing offsets {dt} L={L}', flush=True)
+        monkeypatch.setattr(matmul, '_outer_plan', lambda *a: ('slow64', L, slots))
+        matmul._bwd_plan.cache_clear()
+        try:
+            leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+            y = mhk.expert_dense(*leaves[:2], off, leaves[2], 'silu')
+            grads = torch.autograd.grad(y, leaves, g.to(d))
+        finally:
+            monkeypatch.undo()
+            matmul._bwd_plan.cache_clear()
+        assert (y[50:] == 0).all() and (grads[0][50:] == 0).all() and (grads[1][1] == 0).all() and (grads[2][1] == 0).all()
+        for e, i in ((0, slice(0, 10)), (2, slice(10, 50))):
+            want = dense_case(x[i], w[e], b[e], 'silu', None, g[i], dt)
+            for name, t in zip(('y', 'dx', 'dw', 'db'), (y[i], grads[0][i], grads[1][e], grads[2][e])):
+                near(f'{name} of {e}', t, *want[name])
+
+
 # ------------------------------------------------------------------------------------------ operands that a tile cannot take
 def test_the_library_holds_operands_to_whole_steps():
     """Modules of tiles straight to LDS refuse, before any launch, addresses and distances of rows that such loads cannot
