@@ -105,14 +105,13 @@ int launch(mh_module* m, int kind, int64_t rows, void** args, void* stream, cons
     return 0;
 }
 
-// Launch `kind` on an explicit grid of `blocks` x `grid_y` workgroups (kernels that size their own grid).
-int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* stream, const char* what,
-                  int64_t grid_y = 1) {
+// Launch `kind` on an explicit 1-D grid of `blocks` workgroups (kernels that size their own grid).
+int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* stream, const char* what) {
     if (!m) return fail(-1, std::string(what) + ": null module");
     const Kernel& k = m->k[kind];
     if (!k.fn) return fail(-1, std::string(what) + ": kernel slot not bound in this module");
-    if (blocks <= 0 || grid_y <= 0) return 0;
-    if (blocks > 0x7fffffffLL || grid_y > 65535) return fail(-1, std::string(what) + ": launch too large");
+    if (blocks <= 0) return 0;
+    if (blocks > 0x7fffffffLL) return fail(-1, std::string(what) + ": launch too large");
     int dev = -1;
     MH_HIP(hipGetDevice(&dev));
     if (dev != m->device) {
@@ -120,8 +119,8 @@ int launch_blocks(mh_module* m, int kind, int64_t blocks, void** args, void* str
         os << what << ": module was loaded on device " << m->device << " but device " << dev << " is current";
         return fail(-1, os.str());
     }
-    hipError_t e = hipModuleLaunchKernel(k.fn, static_cast<unsigned>(blocks), static_cast<unsigned>(grid_y), 1,
-                                         static_cast<unsigned>(k.block), 1, 1, 0, static_cast<hipStream_t>(stream), args, nullptr);
+    hipError_t e = hipModuleLaunchKernel(k.fn, static_cast<unsigned>(blocks), 1, 1, static_cast<unsigned>(k.block), 1,
+                                         1, 0, static_cast<hipStream_t>(stream), args, nullptr);
     if (e != hipSuccess) return hip_fail(e, what);
     {
         std::lock_guard<std::mutex> lock(g_log_mu);
@@ -1219,6 +1218,12 @@ int64_t pieces(const int32_t* offsets, int64_t R, int64_t E, int64_t L) {
     return (R + L - 1) / L + (offsets ? std::min(E, R) + 2 : 0);
 }
 
+// Workgroups of a launch that counts `a` of them for each of `b`; more than a launch takes where that passes 64 bits.
+int64_t product(int64_t a, int64_t b) {
+    int64_t n;
+    return __builtin_mul_overflow(a, b, &n) ? INT64_MAX : n;
+}
+
 // Rows that a tile loads straight to LDS lie fewer values apart than this: it holds the byte offsets of up to 256 rows of 16-bit
 // values in 31 bits, and what lies behind is taken as zero.
 constexpr int64_t kStepsLd = int64_t(1) << 21;
@@ -1261,7 +1266,7 @@ int mh_mm_outer(mh_module* m, const void* A, int64_t lda, const void* B, int64_t
     const int64_t tiles = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
                           ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
     void* args[] = {&A, &B, &C, &part, &offsets, &lda, &ldb, &R, &M, &N, &E, &L};
-    return launch_blocks(m, MH_MM_OUTER, tiles, args, stream, "mh_mm_outer", L ? slots : E);
+    return launch_blocks(m, MH_MM_OUTER, product(tiles, L ? slots : E), args, stream, "mh_mm_outer");
 }
 
 int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets, int32_t R, int32_t E, int32_t L, int64_t n,
@@ -1276,7 +1281,7 @@ int mh_mm_sum(mh_module* m, const float* part, void* out, const int32_t* offsets
     while (lg < 4 && (1LL << lg) < slots) ++lg;
     const int64_t columns = 256LL * (16 >> lg);
     void* args[] = {&part, &out, &offsets, &R, &E, &L, &lg, &n};
-    return launch_blocks(m, MH_MM_SUM, (n + columns - 1) / columns, args, stream, "mh_mm_sum", E);
+    return launch_blocks(m, MH_MM_SUM, product((n + columns - 1) / columns, E), args, stream, "mh_mm_sum");
 }
 
 int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, void* p, int64_t ldp, float* part,
@@ -1289,8 +1294,8 @@ int mh_mm_slope(mh_module* m, const void* g, int64_t ldg, const void* slope, voi
     if (ldg < N || (p && (ldp < N || ldp > N + 8LL)))
         return fail(-1, "mh_mm_slope: rows overlap (ld below the row's length), or p padded by more than 8");
     const int64_t width = p ? ldp : N;
-    void* args[] = {&g, &slope, &p, &part, &db, &offsets, &ldg, &ldp, &R, &N, &E, &L};
-    return launch_blocks(m, MH_MM_SLOPE, slots, args, stream, "mh_mm_slope", (width + 255) / 256);
+    void* args[] = {&g, &slope, &p, &part, &db, &offsets, &ldg, &ldp, &R, &N, &E, &L, &slots};
+    return launch_blocks(m, MH_MM_SLOPE, product(slots, (width + 255) / 256), args, stream, "mh_mm_slope");
 }
 
 int mh_mm_bwd(mh_module* sums, mh_module* rows, mh_module* outer, const void* g, int64_t ldg, const void* slope,
@@ -1347,11 +1352,11 @@ int mh_hv_columns(mh_module* m, const float* x, int64_t ldx, uint16_t* y, uint32
     if (!x || !y || !peak) return fail(-1, "mh_hv_columns: NULL operand");
     if (ldx < C) return fail(-1, "mh_hv_columns: rows overlap (ld below the row's length)");
     uint32_t* mark = peak + static_cast<int64_t>(E) * C;
-    const int64_t ny = (static_cast<int64_t>(C) + 255) / 256;
-    void* first[] = {&x, &peak, &mark, &offsets, &ldx, &R, &C, &E, &G, &L};
-    if (int rc = launch_blocks(m, MH_HV_PEAKS, slots, first, stream, "mh_hv_columns", ny)) return rc;
-    void* second[] = {&x, &y, &peak, &offsets, &ldx, &R, &C, &E, &G, &L};
-    return launch_blocks(m, MH_HV_COLUMNS, slots, second, stream, "mh_hv_columns", ny);
+    const int64_t blocks = product(slots, (static_cast<int64_t>(C) + 255) / 256);
+    void* first[] = {&x, &peak, &mark, &offsets, &ldx, &R, &C, &E, &G, &L, &slots};
+    if (int rc = launch_blocks(m, MH_HV_PEAKS, blocks, first, stream, "mh_hv_columns")) return rc;
+    void* second[] = {&x, &y, &peak, &offsets, &ldx, &R, &C, &E, &G, &L, &slots};
+    return launch_blocks(m, MH_HV_COLUMNS, blocks, second, stream, "mh_hv_columns");
 }
 
 int mh_hv_mm(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, const float* bias, const float* res, int64_t ldr,
@@ -1383,7 +1388,7 @@ int mh_hv_outer(mh_module* m, const uint16_t* A, const uint16_t* B, float* C, fl
     const int64_t tiles = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
                           ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
     void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &R, &M, &N, &E, &L};
-    return launch_blocks(m, MH_HV_OUTER, tiles, args, stream, "mh_hv_outer", L ? slots : E);
+    return launch_blocks(m, MH_HV_OUTER, product(tiles, L ? slots : E), args, stream, "mh_hv_outer");
 }
 
 int mh_hv_again_mm(mh_module* m, const float* A, int64_t lda, const float* B, int64_t ldb, float* C, const float* bias,
@@ -1415,11 +1420,11 @@ int mh_hv_again_outer(mh_module* m, const float* A, int64_t lda, const float* B,
     const Kernel& k = m->k[MH_HV_AGAIN];
     const int64_t all = ((static_cast<int64_t>(M) + k.rows_per_block - 1) / k.rows_per_block) *
                         ((static_cast<int64_t>(N) + k.grid_y - 1) / k.grid_y);
-    if (all > 0x7fffffff) return fail(-1, "mh_hv_again_outer: launch too large");
-    int32_t tiles = static_cast<int32_t>(all);
-    if (!L) slots = E;
-    void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &lda, &ldb, &R, &M, &N, &E, &L, &tiles, &slots};
-    return launch_blocks(m, MH_HV_AGAIN, std::min<int64_t>(all * slots, most), args, stream, "mh_hv_again_outer");
+    const int64_t blocks64 = product(all, L ? slots : E);
+    if (blocks64 > 0x7fffffff - most) return fail(-1, "mh_hv_again_outer: launch too large");
+    int32_t blocks = static_cast<int32_t>(blocks64);
+    void* args[] = {&A, &B, &C, &part, &offsets, &pa, &ma, &pb, &mb, &lda, &ldb, &R, &M, &N, &E, &L, &blocks};
+    return launch_blocks(m, MH_HV_AGAIN, std::min<int64_t>(blocks, most), args, stream, "mh_hv_again_outer");
 }
 
 int mh_expert_order(mh_module* m, const void* experts, int32_t wide, int32_t A, int32_t E, int32_t* hist, int32_t blocks,

@@ -103,11 +103,12 @@ __device__ __forceinline__ bool hv_slot(const int* off, int E, int R, int G, int
 // a value, 1,024 x 1,024 weights 5.2 and 5.6 us.
 extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restrict__ x, unsigned* __restrict__ peak,
                                                            unsigned* __restrict__ mark, const int* __restrict__ off,
-                                                           long long ld, int R, int C, int E, int G, int L) {
+                                                           long long ld, int R, int C, int E, int G, int L, int slots) {
     __shared__ unsigned best[4][64][4];
     int e, r0, r1;
-    if (!hv_slot(off, E, R, G, L, blockIdx.x, e, r0, r1)) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 256 + 4 * lane;
+    const int c0 = blockIdx.x / slots * 256;
+    if (!hv_slot(off, E, R, G, L, blockIdx.x % slots, e, r0, r1)) return;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = c0 + 4 * lane;
     unsigned m[4] = {0u, 0u, 0u, 0u};
     if (c < C) {
 #pragma unroll 4
@@ -120,7 +121,7 @@ extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restri
 #pragma unroll
     for (int j = 0; j < 4; ++j) best[w][lane][j] = m[j];
     __syncthreads();
-    const int i = blockIdx.y * 256 + threadIdx.x;        // a column a thread from here on
+    const int i = c0 + threadIdx.x;                      // a column a thread from here on
     if (i >= C) return;
     unsigned b = 0;
 #pragma unroll
@@ -132,10 +133,10 @@ extern "C" __global__ __launch_bounds__(256) void hv_peaks(const float* __restri
 // Columns, second pass: the halves.
 extern "C" __global__ __launch_bounds__(256) void hv_columns(const float* __restrict__ x, unsigned short* __restrict__ y,
                                                              const unsigned* __restrict__ peak, const int* __restrict__ off,
-                                                             long long ld, int R, int C, int E, int G, int L) {
+                                                             long long ld, int R, int C, int E, int G, int L, int slots) {
     int e, r0, r1;
-    if (!hv_slot(off, E, R, G, L, blockIdx.x, e, r0, r1)) return;
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.y * 256 + 4 * lane, Cp = (C + 7) / 8 * 8;
+    if (!hv_slot(off, E, R, G, L, blockIdx.x % slots, e, r0, r1)) return;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, c = blockIdx.x / slots * 256 + 4 * lane, Cp = (C + 7) / 8 * 8;
     if (c >= Cp) return;
     int4 s = make_int4(0, 0, 0, 0);
     const unsigned* p = peak + (long long)e * C;
@@ -252,20 +253,21 @@ __device__ __forceinline__ void hv_outer_body(const unsigned short* A, const uns
                                               const int* off, const unsigned* pa, unsigned* ma, const unsigned* pb,
                                               const unsigned* mb, int R, int M, int N, int E, int L) {
     __shared__ mh_u4 lds[tile_t::LDS];
-    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = gridDim.x / NT, Mp = (M + 7) / 8 * 8, Np = (N + 7) / 8 * 8;
+    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = (M + tile_t::BM - 1) / tile_t::BM, y = blockIdx.x / (MT * NT);
+    const int Mp = (M + 7) / 8 * 8, Np = (N + 7) / 8 * 8;
     int mt, nt, e = 0, r0 = 0, r1 = R;
-    mm_tile_of(blockIdx.x, gridDim.x, MT, NT, mt, nt);
+    mm_tile_of(blockIdx.x % (MT * NT), MT * NT, MT, NT, mt, nt);
     if (L) {
-        if (!mm_slot(off, E, R, L, blockIdx.y, e, r0, r1)) return;
+        if (!mm_slot(off, E, R, L, y, e, r0, r1)) return;
     } else if (off) {
-        mm_by_length(off, E, R, blockIdx.y, e, r0, r1);
+        mm_by_length(off, E, R, y, e, r0, r1);
     }
     const int m0 = mt * tile_t::BM, n0 = nt * tile_t::BN, rows = min(M - m0, tile_t::BM), cols = min(N - n0, tile_t::BN);
     const unsigned short *a = A + (long long)r0 * 2 * Mp + m0, *b = B + (long long)r0 * 2 * Np + n0;
     const int ar = min(Mp - m0, tile_t::BM), br = min(Np - n0, tile_t::BN);
     tile_t t;
     t.run(lds, a, Mp, ar, b, Np, br, 0, 2 * (r1 - r0));
-    float* C = (L ? part + (long long)blockIdx.y * M * N : C0 + (long long)e * M * N) + (long long)m0 * N + n0;
+    float* C = (L ? part + (long long)y * M * N : C0 + (long long)e * M * N) + (long long)m0 * N + n0;
     const long long ra = (long long)e * M + m0, rb = (long long)e * N + n0;
     const hv_result<tile_t> r(t, pa + ra, ma + ra, rows, pb + rb, mb + rb, cols);
     r.template mark<true>(ma + ra, ma + (long long)E * M);
@@ -304,15 +306,13 @@ __device__ __forceinline__ void hv_again_rows_body(const float* A, const float* 
         mm_rows_body<MM_F32, BS, ACT, tile_t>(A, B, C, bias, res, slope, off, lda, ldb, ldr, R, N, K, E, b, tiles, marked);
 }
 
-// After hv_outer_body, of `tiles` tiles in each group or slot.
+// After hv_outer_body, of `blocks` tiles in all groups or slots.
 template <typename tile_t>
 __device__ __forceinline__ void hv_again_outer_body(const float* A, const float* B, float* C, float* part, const int* off,
                                                     const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb,
-                                                    long long lda, long long ldb, int R, int M, int N, int E, int L, int tiles,
-                                                    int slots) {
+                                                    long long lda, long long ldb, int R, int M, int N, int E, int L, int blocks) {
     if (!ma[(long long)E * M]) return;
     const hv_marked marked = {pa, ma, pb, mb, M, N};
-    for (long long i = blockIdx.x; i < (long long)tiles * slots; i += gridDim.x)
-        mm_outer_body<MM_F32, tile_t>(A, B, C, part, off, lda, ldb, R, M, N, E, L, (int)(i % tiles), tiles, (int)(i / tiles),
-                                      marked);
+    for (int b = blockIdx.x; b < blocks; b += gridDim.x)
+        mm_outer_body<MM_F32, tile_t>(A, B, C, part, off, lda, ldb, R, M, N, E, L, b, marked);
 }

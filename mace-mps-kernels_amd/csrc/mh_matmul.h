@@ -1032,20 +1032,20 @@ __device__ __forceinline__ void mm_few_body(const void* A_, const void* B_, void
     }
 }
 
-// Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  y is the group
-// (L 0: all its rows; none give zeros), or a slot of at most L of its rows whose sums go to part[slot] in float32; tile `b` of
-// `blocks`; wanted as in mm_rows_body, of the result's rows and columns.
+// Weight gradients: D[e] [M, N] = sum over the group's rows of A[r, m] B[r, n] (A = p [R, M], B = x [R, N]).  Blocks count the
+// tiles of the result, and these for one y after the other: the group (L 0: all its rows; none give zeros), or a slot of at most L
+// of its rows whose sums go to part[slot] in float32.  wanted as in mm_rows_body, of the result's rows and columns.
 // Bound as the other products; 16,384 rows of 4,096 by 1,024 in bfloat16 in four pieces take 140 us and 10 for their sum
 // (980 TFLOP/s), eight groups of 2,048 rows of 2,048 by 1,024 whole 75 us.
 template <int TY, typename tile_t, typename wanted_t = mm_every>
 __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, void* C_, float* part, const int* off,
-                                              long long lda, long long ldb, int R, int M, int N, int E, int L, int b = blockIdx.x,
-                                              int blocks = gridDim.x, int y = blockIdx.y, wanted_t wanted = wanted_t()) {
+                                              long long lda, long long ldb, int R, int M, int N, int E, int L,
+                                              unsigned block = blockIdx.x, wanted_t wanted = wanted_t()) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_u4 lds[tile_t::LDS];
-    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = blocks / NT;
+    const int NT = (N + tile_t::BN - 1) / tile_t::BN, MT = (M + tile_t::BM - 1) / tile_t::BM, y = block / (MT * NT);
     int mt, nt, e = 0, r0 = 0, r1 = R;
-    mm_tile_of(b, blocks, MT, NT, mt, nt);
+    mm_tile_of(block % (MT * NT), MT * NT, MT, NT, mt, nt);
     if (L) {
         if (!mm_slot(off, E, R, L, y, e, r0, r1)) return;
     } else if (off) {
@@ -1070,6 +1070,31 @@ __device__ __forceinline__ void mm_outer_body(const void* A_, const void* B_, vo
         }
 }
 
+// The slots of group e, as mm_slot numbers them.  Every lane of a wave calls.
+__device__ __forceinline__ void mm_slots_of(const int* __restrict__ off, int E, int R, int L, int e, int& s0, int& s1) {
+    s0 = 0;
+    s1 = (R + L - 1) / L;
+    if (!off) return;
+    mm_groups g(off, E, R);
+    int base = 0;
+    for (int g0 = 0;; g0 += MH_WAVE) {
+        g.scan(g0);
+        const int l = e - g0, n = (g.hi - g.lo + L - 1) / L;
+        int inc = n;
+#pragma unroll
+        for (int d = 1; d < MH_WAVE; d <<= 1) {
+            const int t = __shfl_up(inc, d, MH_WAVE);
+            if ((int)(threadIdx.x & (MH_WAVE - 1)) >= d) inc += t;
+        }
+        if (l < MH_WAVE) {
+            s1 = base + mh_bcast(inc, l);
+            s0 = s1 - mh_bcast(n, l);
+            return;
+        }
+        base += mh_bcast(inc, MH_WAVE - 1);
+    }
+}
+
 // out[e, i] = sum of part[s, i] over the group's slots in a fixed order: what ends a sum that was split over rows.  2^lg waves
 // share a column's slots (wave w takes every 2^lg-th) and are added in wave order, so that few columns of many slots are
 // not one wave's chain of loads; 1024 threads, four columns a lane.  Bound by its bytes: 4 slots of 4,096 x 1,024 in 10 us, 512
@@ -1079,20 +1104,11 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
                                             long long n) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_f4 sums[16][64];
-    const int e = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & ((1 << lg) - 1);
-    const long long i = ((long long)blockIdx.x * (16 >> lg) + (wave >> lg)) * 256 + 4 * lane;
-    int s0 = 0, s1 = 0;
-    if (!off) {
-        s1 = (R + L - 1) / L;
-    } else {
-        int top = min(max(off[0], 0), R);               // as mm_slot
-        for (int g = 0; g <= e; ++g) {
-            const int hi = max(top, min(off[g + 1], R));
-            s0 = s1;
-            s1 += (hi - top + L - 1) / L;
-            top = hi;
-        }
-    }
+    const long long columns = 256 * (16 >> lg), per = (n + columns - 1) / columns;       // blocks of a group
+    const int e = (int)(blockIdx.x / per), lane = threadIdx.x & 63, wave = threadIdx.x >> 6, w = wave & ((1 << lg) - 1);
+    const long long i = blockIdx.x % per * columns + (wave >> lg) * 256 + 4 * lane;
+    int s0, s1;
+    mm_slots_of(off, E, R, L, e, s0, s1);
     const int c = (int)max((long long)0, min((long long)4, n - i));
     mh_f4 v = {0.f, 0.f, 0.f, 0.f};
     if (c >= 4) {
@@ -1113,18 +1129,19 @@ __device__ __forceinline__ void mm_sum_body(const float* part, void* out_, const
 // p = g act'(a) in the type (P NULL: not stored, slope NULL: act' = 1), rows ldp >= N apart with zeros behind N, and the sums of
 // its columns in float32, before rounding: into part [slots, N] for each slot of L rows, or, where one slot holds all rows,
 // rounded into db (both NULL: none).  For 16-bit types p is rounded once here, as the matrix products take it: the error of a
-// gradient is then that of a product of rounded operands.  A workgroup takes a slot and 256 columns, 64 threads of four
-// columns each by four rows at a time.  Bound by its bytes; the slope is read for the last time, past the caches: 69 us at
+// gradient is then that of a product of rounded operands.  A workgroup takes a slot and 256 columns (blocks count the slots of
+// the first 256, then of the next), 64 threads of four columns each by four rows at a time.  Bound by its bytes; the slope is read for the last time, past the caches: 69 us at
 // 16,384 x 4,096 bfloat16, 5.8 TB/s (81 as an ordinary read).
 template <int TY>
 __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_, void* P_, float* part, void* db, const int* off,
-                                              long long ldg, long long ldp, int R, int N, int E, int L) {
+                                              long long ldg, long long ldp, int R, int N, int E, int L, int slots) {
     typedef typename mm_type<TY>::t T;
     __shared__ mh_f4 sums[4][64];
     int e, r0, r1;
-    if (!mm_slot(off, E, R, L, blockIdx.x, e, r0, r1) && !db) return;      // db without rows: zeros
+    const int slot = blockIdx.x % slots;
+    if (!mm_slot(off, E, R, L, slot, e, r0, r1) && !db) return;            // db without rows: zeros
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int n = blockIdx.y * 256 + 4 * lane, c = N - n;
+    const int n = blockIdx.x / slots * 256 + 4 * lane, c = N - n;
     const T* g = static_cast<const T*>(g_) + n;
     T* P = static_cast<T*>(P_);
     mh_f4 s = {0.f, 0.f, 0.f, 0.f};
@@ -1182,7 +1199,7 @@ __device__ __forceinline__ void mm_slope_body(const void* g_, const void* slope_
         s += sums[2][lane];
         s += sums[3][lane];
         if (db) mm_put4<TY>(static_cast<T*>(db) + n, s, c);
-        else mm_put4<MM_F32>(part + (long long)blockIdx.x * N + n, s, c);
+        else mm_put4<MM_F32>(part + (long long)slot * N + n, s, c);
     }
 }
 

@@ -47,8 +47,8 @@ def source(mode, act=0):
               'int R, int M, int N, int E, int L) {',
               '  hv_outer_body<tile_t>(A, B, C, part, off, pa, ma, pb, mb, R, M, N, E, L);', '}', *again,
               'float* part, const int* off, const unsigned* pa, const unsigned* ma, const unsigned* pb, const unsigned* mb, '
-              'long long lda, long long ldb, int R, int M, int N, int E, int L, int tiles, int slots) {',
-              '  hv_again_outer_body<again_t>(A, B, C, part, off, pa, ma, pb, mb, lda, ldb, R, M, N, E, L, tiles, slots);', '}']
+              'long long lda, long long ldb, int R, int M, int N, int E, int L, int blocks) {',
+              '  hv_again_outer_body<again_t>(A, B, C, part, off, pa, ma, pb, mb, lda, ldb, R, M, N, E, L, blocks);', '}']
     else:
         L += ['const float* bias, const float* res, float* slope, const int* off, unsigned* pa, const unsigned* pb, '
               'const unsigned* mb, long long ldr, int R, int N, int K, int E) {',

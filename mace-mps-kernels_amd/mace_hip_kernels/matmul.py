@@ -98,8 +98,8 @@ def source(dtype, mode, tile=None, act=0):
         L += ['extern "C" __global__ __launch_bounds__(1024) void mm_sum(const float* part, void* out, const int* off, int R, '
               'int E, int L, int lg, long long n) {', f'  mm_sum_body<{ty}>(part, out, off, R, E, L, lg, n);', '}',
               'extern "C" __global__ __launch_bounds__(256) void mm_slope(const void* g, const void* slope, void* P, '
-              'float* part, void* db, const int* off, long long ldg, long long ldp, int R, int N, int E, int L) {',
-              f'  mm_slope_body<{ty}>(g, slope, P, part, db, off, ldg, ldp, R, N, E, L);', '}']
+              'float* part, void* db, const int* off, long long ldg, long long ldp, int R, int N, int E, int L, int slots) {',
+              f'  mm_slope_body<{ty}>(g, slope, P, part, db, off, ldg, ldp, R, N, E, L, slots);', '}']
         if dtype.itemsize == 2:
             L += ['extern "C" __global__ __launch_bounds__(256) void mm_pad(const void* x, void* y, long long ld, int R, int K, '
                   'int Kp) {', f'  mm_pad_body<{ty}>(x, y, ld, R, K, Kp);', '}']

@@ -1,7 +1,7 @@
 """
 The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
 that a tile cannot take, forward-mode derivatives, units far in an activation's tail, products of very unlike
-magnitudes.
+magnitudes, more groups or columns than a grid dimension holds.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -10,7 +10,7 @@ import torch
 
 import mace_hip_kernels as mhk
 from mace_hip_kernels import _native, matmul
-from test_node_layers_gpu import BF16, E32, F16, F32, TINY, U, by_halves, dense_case, dev, near, rand  # noqa: F401
+from test_node_layers_gpu import ACTS, BF16, E32, F16, F32, TINY, U, by_halves, dense_case, dev, near, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 TYPES = pytest.mark.parametrize('dt', [F32, BF16, F16], ids=['f32', 'bf16', 'f16'])
@@ -262,3 +262,50 @@ def test_infinities_that_meet_small_values_by_halves(by_halves):  # noqa: F811
     got, want = mhk.dense(x.to(d), w.to(d)).cpu(), (x.double() @ w.double().t())
     assert torch.isnan(want[2, 3]) and torch.isinf(want[2, :3]).all()
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[[2, 100]].double().nan_to_num(7), want[[2, 100]].nan_to_num(7))
+
+
+# ------------------------------------------------------------------------------------------ many groups, many columns
+def test_more_groups_than_a_grid_dimension_holds():
+    d = dev()
+    rng = np.random.default_rng(8)
+    E, K, N = 70_001, 5, 3
+    sizes = rng.integers(0, 3, E)
+    off = torch.tensor(np.concatenate([[0], np.cumsum(sizes)]), dtype=torch.int32)
+    R = int(off[-1])
+    e = torch.repeat_interleave(torch.arange(E), torch.tensor(sizes))
+    for dt in (F32, BF16):
+        for act in (None, 'relu'):
+            print(f'[case] {E} groups {dt} {act}', flush=True)
+            x, w, b, g = rand(rng, R, K, dt=dt), rand(rng, E, N, K, dt=dt), rand(rng, E, N, dt=dt), rand(rng, R, N, dt=dt)
+            leaves = [t.to(d).requires_grad_() for t in (x, w, b)]
+            y = mhk.expert_dense(*leaves[:2], off.to(d), leaves[2], act)
+            dx, dw, db = torch.autograd.grad(y, leaves, g.to(d))
+            a = (w.double()[e] @ x.double()[:, :, None])[:, :, 0] + b.double()[e]
+            p = g.double() * ((a > 0) if act else 1)
+            zero = torch.zeros(E, N, dtype=torch.float64)
+            # five products of order one, rounded once (p is exact: a gradient or zero)
+            near('y', y, ACTS[act](a), 40 * E32 * (a.abs() + 10) + U[dt] * (a.abs() + 1))
+            near('dx', dx, (p[:, None] @ w.double()[e])[:, 0], 40 * E32 * 20 + U[dt] * (p[:, None] @ w.double()[e])[:, 0].abs())
+            want = zero.index_add(0, e, p)
+            near('db', db, want, 40 * E32 * 20 + U[dt] * want.abs())
+            want = torch.zeros(E, N, K, dtype=torch.float64).index_add(0, e, p[:, :, None] * x.double()[:, None])
+            near('dw', dw, want, 40 * E32 * 20 + U[dt] * want.abs())
+
+
+def test_more_columns_than_a_grid_dimension_holds_workgroups():
+    """Rows so wide that their pieces of 256 columns are more than 65,535."""
+    d = dev()
+    print('[case] wide rows', flush=True)
+    N = 256 * 65535 + 300
+    x = torch.tensor([[0.5, -2.0], [1.0, 3.0]], dtype=BF16, device=d, requires_grad=True)
+    k = torch.arange(N, device=d)
+    w = torch.stack([(k % 3).to(BF16), torch.ones_like(k, dtype=BF16)], 1).requires_grad_()
+    b = (-(k % 2)).to(BF16).requires_grad_()
+    y = mhk.dense(x, w, b, 'relu')
+    a = x.detach().float() @ w.detach().float().t() + b.detach().float()              # small whole numbers and halves: exact
+    assert torch.equal(y.float(), a.clamp_min(0))
+    p = (a > 0).float()
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    assert torch.equal(db.float(), p.sum(0)) and torch.equal(dw.float(), p.t() @ x.detach().float())
+    want = p.double() @ w.detach().double()
+    near('dx', dx, want.cpu(), 2.0 ** -7 * want.abs().cpu())   # sums of up to 5 10^7 in some order, rounded to bfloat16
