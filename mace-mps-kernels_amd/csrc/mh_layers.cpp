@@ -514,13 +514,16 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
     }
 };
 
+// places [T, k] and offsets [E + 1] as expert_order makes them: what the kernels read as rows of int32
 bool an_order(const Tensor& place, const Tensor& off, const Tensor& x) {
-    return place.device() == x.device() && off.device() == x.device();
+    return place.device() == x.device() && off.device() == x.device() && place.scalar_type() == at::kInt &&
+           off.scalar_type() == at::kInt && place.dim() == 2 && off.dim() == 1 && place.size(1) >= 1 && off.size(0) >= 2 &&
+           place.is_contiguous() && off.is_contiguous() && place.numel() < kMost;
 }
 
 py::object dispatch(py::handle x_, const Tensor& place, const Tensor& off) {
     Tensor x;
-    if (!tensor(x_, &x) || !fits(x) || x.dim() != 2 || x.size(0) != place.size(0) || !an_order(place, off, x)) return py::none();
+    if (!tensor(x_, &x) || !fits(x) || x.dim() != 2 || !an_order(place, off, x) || x.size(0) != place.size(0)) return py::none();
     no_tangents({&x});
     const PlanPtr p = route_plan(x, x.size(1));
     if (at::GradMode::is_enabled() && grad(x)) return py::cast(DispatchFn::apply(x, place, off, p));

@@ -96,6 +96,12 @@ def _check_order(order, device):
         raise TypeError(f'order must come from expert_order, got {type(order).__name__}')
     if order.place.device != device:
         raise TypeError(f'the order is on {order.place.device}, the rows on {device}')
+    for name, t, dims in (('place', order.place, 2), ('offsets', order.offsets, 1)):
+        if t.dtype != torch.int32 or t.dim() != dims or not t.is_contiguous():
+            raise ValueError(f'order.{name} must be as expert_order made it (int32, {dims} dimensions, contiguous), got {t.dtype} '
+                             f'{list(t.shape)}')
+    if order.place.shape[1] < 1 or order.offsets.shape[0] < 2:
+        raise ValueError(f'the order has no experts: place {list(order.place.shape)}, offsets {list(order.offsets.shape)}')
 
 
 def dispatch(x, order):

@@ -1,7 +1,8 @@
 """
 The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
 that a tile cannot take, forward-mode derivatives, units far in an activation's tail, products of very unlike
-magnitudes, more groups or columns than a grid dimension holds.
+magnitudes, more groups or columns than a grid dimension holds,
+orders made by hand.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -309,3 +310,23 @@ def test_more_columns_than_a_grid_dimension_holds_workgroups():
     assert torch.equal(db.float(), p.sum(0)) and torch.equal(dw.float(), p.t() @ x.detach().float())
     want = p.double() @ w.detach().double()
     near('dx', dx, want.cpu(), 2.0 ** -7 * want.abs().cpu())   # sums of up to 5 10^7 in some order, rounded to bfloat16
+
+
+# ------------------------------------------------------------------------------------------ orders made by hand
+def test_orders_that_expert_order_did_not_make_are_refused():
+    """Places and offsets of another type, shape or layout are refused where the kernels would read past them."""
+    d = dev()
+    print('[case] orders by hand', flush=True)
+    x = torch.zeros(6, 8, device=d)
+    o = mhk.expert_order(torch.zeros(6, 2, dtype=torch.int64, device=d), 3)
+    y = mhk.dispatch(x, o)
+    for place, offsets in ((o.place[:1].expand(6, 2), o.offsets), (o.place.t().contiguous().t(), o.offsets),
+                           (o.place.reshape(-1), o.offsets), (o.place.short(), o.offsets), (o.place, o.offsets.short()),
+                           (o.place, o.offsets[:1].expand(4)), (o.place, o.offsets[None]), (o.place, o.offsets[:1]),
+                           (o.place[:, :0].contiguous(), o.offsets)):
+        bad = mhk.ExpertOrder(offsets, o.rows, place, 3)
+        for call in (lambda: mhk.dispatch(x, bad), lambda: mhk.combine(y, None, bad)):
+            with pytest.raises(ValueError, match='order'):
+                call()
+    again = mhk.ExpertOrder(o.offsets.clone(), o.rows, o.place.clone(), 3)
+    assert torch.equal(mhk.dispatch(x, again), y) and mhk.combine(y, None, again).shape == (6, 8)
