@@ -63,6 +63,14 @@ int type_of(const Tensor& t) {
     }
 }
 
+// A saved tensor may have been given other data since (`p.data = ...`, a module moved to another device or type): the kernels
+// would read that as what it was.
+void unchanged(const Tensor& t, const Tensor& grad, at::ScalarType type, int64_t numel, int64_t last) {
+    TORCH_CHECK(!t.defined() || (t.device() == grad.device() && t.scalar_type() == type && t.numel() == numel && t.dim() &&
+                                 t.size(-1) == last),
+                "mace_hip_kernels: a tensor of a trainable layer has changed its shape, type or device since its forward");
+}
+
 const char* const kDouble =
     "mace_hip_kernels: double backward (create_graph=True) is not available for the trainable node layers "
     "(dense, expert_dense, dispatch, combine, block_norm)";
@@ -283,9 +291,11 @@ struct DenseFn : torch::autograd::Function<DenseFn> {
         int64_t ldg, ldx = 0, ldw = std::max<int64_t>(1, K), ldp = 0;
         Tensor g = rows_of(grads[0], N, &ldg);
         const bool f = g.scalar_type() == at::kFloat;
+        unchanged(x, g, g.scalar_type(), R * K, K);
+        unchanged(w, g, g.scalar_type(), groups * N * K, K);
+        unchanged(off, g, at::kInt, groups + 1, groups + 1);
         if (x.defined()) x = rows_of(x, K, &ldx);
-        TORCH_CHECK((!x.defined() || (x.size(0) == R && x.size(1) == K)) && (!w.defined() || w.numel() == groups * N * K) &&
-                        g.size(0) == R, "mace_hip_kernels: a tensor of a dense layer has changed its shape since its forward");
+        if (w.defined()) w = w.contiguous();
         key.v[9] = made || f || steps(g, ldg, N);
         key.v[10] = w.defined() && !f && steps(w, K, K);
         key.v[11] = x.defined() && !f && steps(x, ldx, K);
@@ -502,12 +512,15 @@ struct CombineFn : torch::autograd::Function<CombineFn> {
         if (need & 4) out[2] = grads[0];
         if (!(need & 3)) return out;
         int64_t ldg;
+        if (need & 2) unchanged(saved[0], grads[0], grads[0].scalar_type(), T * k * C, C);
+        unchanged(saved[1], grads[0], at::kFloat, T * k, k);
         const Tensor g = rows_of(grads[0], C, &ldg), y = need & 2 ? saved[0].contiguous() : Tensor();
+        const Tensor w = saved[1].defined() ? saved[1].contiguous() : Tensor();
         if (need & 1) out[0] = at::empty({T * k, C}, g.options());
         if (need & 2) out[1] = at::empty({T, k}, g.options().dtype(at::kFloat));
         if (T && (C || (need & 2)))
             launch("ex_combine_bwd", [&] {
-                return mh_combine_bwd(p->module(R_MODULE), ptr(g), ldg, ptr(y), f32(saved[1]), i32(place), i32(off), ptr(out[0]),
+                return mh_combine_bwd(p->module(R_MODULE), ptr(g), ldg, ptr(y), f32(w), i32(place), i32(off), ptr(out[0]),
                                       f32(out[1]), T, k, C, off.size(0) - 1, (*p)[R_LANES], stream_of(g));
             });
         return out;
@@ -580,7 +593,7 @@ struct NormFn : torch::autograd::Function<NormFn> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         TORCH_CHECK(!at::GradMode::is_enabled(), kDouble);
-        const auto s = ctx->get_saved_variables();
+        auto s = ctx->get_saved_variables();
         const PlanPtr p = saved_plan(ctx);
         const int64_t need = ctx->saved_data["n"].toInt();
         const Tensor &x = s[0], &y = s[1], &gate = s[2];
@@ -589,7 +602,13 @@ struct NormFn : torch::autograd::Function<NormFn> {
         if (!gh.defined() && !gn.defined()) return out;
         if (gh.defined()) gh = gh.contiguous();
         if (gn.defined()) gn = gn.contiguous();
-        const int64_t C = x.size(-1), T = x.numel() / C;
+        const int64_t T = p->key.v[3], C = p->key.v[4];
+        const int64_t gates = p->key.v[7] == 1 ? 1 : C, numel[6] = {T * C, T * C, T * gates, C, C, C};
+        for (int k = 0; k < 6; ++k) {
+            if (!s[k].defined()) continue;
+            unchanged(s[k], gn.defined() ? gn : gh, (gn.defined() ? gn : gh).scalar_type(), numel[k], k == 2 ? gates : C);
+            s[k] = s[k].contiguous();
+        }
         if (need & 1) out[0] = at::empty(x.sizes(), x.options());
         if (need & 2) out[1] = at::empty(x.sizes(), x.options());
         if (need & 4) out[2] = at::empty(gate.sizes(), x.options());

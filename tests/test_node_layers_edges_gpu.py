@@ -2,7 +2,7 @@
 The trainable node layers where their inputs are out of the ordinary: groups that begin behind the first row, operands
 that a tile cannot take, forward-mode derivatives, units far in an activation's tail, products of very unlike
 magnitudes, more groups or columns than a grid dimension holds,
-orders made by hand.
+orders made by hand, inputs given other data before the backward.
 Tolerances as in the layers' other tests, derived beside each.
 """
 import numpy as np
@@ -330,3 +330,36 @@ def test_orders_that_expert_order_did_not_make_are_refused():
                 call()
     again = mhk.ExpertOrder(o.offsets.clone(), o.rows, o.place.clone(), 3)
     assert torch.equal(mhk.dispatch(x, again), y) and mhk.combine(y, None, again).shape == (6, 8)
+
+
+# ------------------------------------------------------------------------------------------ inputs given other data
+def test_inputs_given_other_data_before_the_backward():
+    """An input whose data was replaced between forward and backward, as moving a module to another device or type does, is
+    refused; data of the same shape in another layout is read as it lies."""
+    d = dev()
+    print('[case] other data', flush=True)
+    rng = np.random.default_rng(2)
+    off = torch.tensor([0, 4, 6], dtype=torch.int32, device=d)
+    o = mhk.expert_order(torch.tensor(rng.integers(0, 3, (6, 2)), device=d), 3)
+
+    def leaves():
+        return [rand(rng, *s).to(d).requires_grad_() for s in ((6, 8), (8, 8), (2, 8, 8), (8,), (12, 8), (6, 2), (6, 8))]
+
+    layers = [(lambda x, w, ws, b, y, c, h: mhk.dense(x, w, b, 'silu'), (0, 1)),
+              (lambda x, w, ws, b, y, c, h: mhk.expert_dense(x, ws, off), (0, 2)),
+              (lambda x, w, ws, b, y, c, h: mhk.combine(y, c, o), (4, 5)),
+              (lambda x, w, ws, b, y, c, h: mhk.block_norm(x, h, gate=x[:, :1], scale=b)[0], (0, 3, 6))]
+    for call, used in layers:
+        for i in used:
+            for other in (lambda t: t.cpu(), lambda t: t.half(), lambda t: t.double(), lambda t: t[..., :1].contiguous()):
+                ins = leaves()
+                out = call(*ins)
+                ins[i].data = other(ins[i].detach())
+                with pytest.raises(RuntimeError, match='changed its shape|Expected|expected|same'):
+                    out.sum().backward()
+            ins = leaves()
+            out = call(*ins)
+            want = torch.autograd.grad(out.sum(), [ins[k] for k in used], retain_graph=True)
+            ins[i].data = torch.stack([ins[i].detach()] * 2, -1)[..., 0]      # the same values, two apart
+            got = torch.autograd.grad(out.sum(), [ins[k] for k in used])
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), i
