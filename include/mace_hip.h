@@ -154,7 +154,8 @@ enum mh_kernel_kind {
  * from torch there). */
 const char* mh_last_error(void);
 
-/* ABI version of this header (bumped on any signature change). */
+/* ABI version of this header (bumped on any change of a signature, or of what a buffer has to hold), and the library's own. */
+#define MH_ABI_VERSION 51
 int mh_version(void);
 
 /* Launch log of the process, for profiling and tests that check which kernels ran: while enabled, every successful

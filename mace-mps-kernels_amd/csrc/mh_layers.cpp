@@ -666,6 +666,7 @@ py::object block_norm(py::handle x_, py::handle y_, py::handle g_, py::handle s_
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
+    m.attr("abi") = MH_ABI_VERSION;                      // of the header that this was built with
     // planner(kind, ...) -> numbers; timed: launch(tag, fn) while launches are timed, else None
     m.def("set_planner", [](py::object f) { g_planner = f.release().ptr(); });
     m.def("set_timed", [](py::object f) { Py_XDECREF(g_timed.exchange(f.is_none() ? nullptr : f.release().ptr())); });

@@ -196,6 +196,9 @@ def layers():
         except ImportError as e:
             raise RuntimeError(f'mace_hip_kernels: _layers.so is missing or stale ({e}); build it with '
                                '__graft_entry__.build()') from e
+        if getattr(module, 'abi', None) != ABI_VERSION:
+            raise RuntimeError('mace_hip_kernels: _layers.so was built for another libmace_hip.so; rebuild it with '
+                               '__graft_entry__.build()')
         module.set_planner(lambda kind, *key: PLANNERS[kind](*key))
         module.set_timed(launch if timing.active is not None else None)
         _layers = module

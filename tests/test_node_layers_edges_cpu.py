@@ -10,11 +10,14 @@ import random
 import re
 import shutil
 import subprocess
+import sys
+import types
 
 import numpy as np
 import pytest
 import torch
 
+import mace_hip_kernels
 from mace_hip_kernels import _native, halves, matmul
 
 CSRC = os.path.dirname(_native.DEVICE_HEADER)
@@ -228,3 +231,14 @@ extern "C" void back(const unsigned short* c, float* v, int n) {{ for (int i = 0
     # the codes in use are each other's inverse
     used = np.concatenate([np.arange(1, 48771), np.arange(49536, 65535)]).astype(np.uint16)
     assert (there(back(used)) == used).all() and np.isnan(back(np.array([0xC000], dtype=np.uint16)))[0]
+
+
+def test_a_host_side_built_for_another_library_is_refused(monkeypatch):
+    """_layers.so allocates what libmace_hip.so's kernels write: built from another header it is not used."""
+    assert _native.layers().abi == _native.ABI_VERSION == _native.load().mh_version()
+    for fake in (types.SimpleNamespace(abi=_native.ABI_VERSION - 1), types.SimpleNamespace()):
+        monkeypatch.setattr(_native, '_layers', None)
+        monkeypatch.setitem(sys.modules, 'mace_hip_kernels._layers', fake)
+        monkeypatch.setattr(mace_hip_kernels, '_layers', fake)
+        with pytest.raises(RuntimeError, match='another libmace_hip.so'):
+            _native.layers()
