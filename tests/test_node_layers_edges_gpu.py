@@ -265,6 +265,48 @@ def test_infinities_that_meet_small_values_by_halves(by_halves):  # noqa: F811
     assert torch.equal(got.isnan(), want.isnan()) and torch.equal(got[[2, 100]].double().nan_to_num(7), want[[2, 100]].nan_to_num(7))
 
 
+def test_products_by_halves_in_a_captured_graph(by_halves):  # noqa: F811
+    """A captured forward and backward, replayed over inputs with and without values that the halves do not hold: every replay
+    gives what the same calls give, and nothing of the replay before."""
+    d = dev()
+    print('[case] halves in a graph', flush=True)
+    torch.manual_seed(3)
+    T, K, N = 200, 96, 160
+    x, w = torch.randn(T, K, device=d, requires_grad=True), torch.randn(N, K, device=d, requires_grad=True)
+    g = torch.randn(T, N, device=d)
+
+    def call():
+        y = mhk.dense(x, w, activation='silu')
+        return [y, *torch.autograd.grad(y, (x, w), g)]
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        call()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for i in range(6):
+        with torch.no_grad():
+            x.normal_()
+            w.normal_()
+            g.normal_()
+            if i in (1, 2, 4):                               # not held: one value, one row, an infinity
+                x[5, 7], w[:, 7] = (1e12, 0) if i != 4 else (float('inf'), 1e-20)
+            if i == 2:
+                g[:, 9] *= 1e-15
+                g[3] *= 1e9
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(out, call()):
+            assert torch.equal(a.nan_to_num(3), b.nan_to_num(3)), i
+        if i != 4:
+            want = dense_case(x.detach().cpu(), w.detach().cpu(), None, 'silu', None, g.cpu(), F32)
+            for name, a in zip(('y', 'dx', 'dw'), out):
+                near(f'{name} of replay {i}', a, *want[name])
+
+
 # ------------------------------------------------------------------------------------------ many groups, many columns
 def test_more_groups_than_a_grid_dimension_holds():
     d = dev()
