@@ -61,7 +61,7 @@ __device__ __forceinline__ void hv_split4(mh_f4 v, int4 shift, unsigned short* h
 }
 
 // Rows: a wave each; the second reading of a row comes from the caches.  word [R + 1]: the last, whether anything is to be computed
-// again, zero here.  Bound by its bytes: 20,000 rows of 1,024 in 38 us, 4.3 TB/s.
+// again, zero here.  Bound by its bytes: 20,000 rows of 1,024 in 39 us, 4.2 TB/s.
 extern "C" __global__ __launch_bounds__(256) void hv_rows(const float* __restrict__ x, unsigned short* __restrict__ y,
                                                           unsigned* __restrict__ word, long long ld, int R, int K) {
     if (blockIdx.x == 0 && threadIdx.x == 0) word[R] = 0u;
@@ -216,8 +216,8 @@ struct hv_result {
 
 // mm_rows_body on halves: A rows [R][Kp / 32][2][32] with their words pa [R + 1]; B either rows, [E][N][Kp / 32][2][32] with words
 // pb [E][N], or (BS) columns of K contracted rows, [E][K][2][Np] with pb and mb [E][N].
-// Bound by the matrix cores: 20,000 x 1,024 x 1,024 in 128 us, 980 TFLOP/s of float16 products (three rounds of workgroups where
-// 2.45 would do), the cores busy 53 % of it.
+// Bound by the matrix cores: 20,000 x 1,024 x 1,024 in 133 us, 950 TFLOP/s of float16 products (three rounds of workgroups where
+// 2.45 would do), the cores busy 51 % of it.
 template <bool BS, int ACT, typename tile_t>
 __device__ __forceinline__ void hv_rows_body(const unsigned short* A, const unsigned short* B, float* C0, const float* bias,
                                              const float* res, float* slope, const int* off, unsigned* pa,
@@ -294,7 +294,8 @@ struct hv_marked {
 };
 
 // After hv_rows_body: the tiles with marked results once more, by the direct kernel from the operands themselves.  Workgroups walk
-// the `tiles` where there is anything to do; where not, as nearly always, this costs a launch and one load.
+// the `tiles` where there is anything to do (all of 20,000 x 1,024 x 1,024: 330 us); where not, as nearly always, this costs a
+// launch and one load, 4 us.
 template <bool BS, int ACT, typename tile_t>
 __device__ __forceinline__ void hv_again_rows_body(const float* A, const float* B, float* C, const float* bias, const float* res,
                                                    float* slope, const int* off, const unsigned* pa, const unsigned* pb,

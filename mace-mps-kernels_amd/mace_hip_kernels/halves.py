@@ -22,8 +22,8 @@ def pays(rows, n, K, groups, mode, product, direct):
     """Whether a product of [rows, K] and [groups, n, K] that takes ``direct`` seconds is faster by halves: by the seconds of
     the ``product`` of halves itself, the bytes of the halves (read and written once by rows, read twice by columns), the
     launches, and a margin of a tenth for what these leave out.  Measured (us, direct / halves): 20,000 x 1,024 x 1,024 forward
-    268 / 166, dx 269 / 168, dw 290 / 247; 4,096 x 1,024 x 1,024 52 / 49, 60 / 46, 73 / 82; 8,192 x 512 x 2,048 107 / 72, 113 /
-    91, 126 / 132; 5,000 x 512 x 512 26 / 36, 28 / 28, 41 / 58; 20,000 x 128 x 512 forward 30 / 40."""
+    247 / 165, dx 298 / 174, dw 287 / 259; 4,096 x 1,024 x 1,024 54 / 49, 63 / 54, 68 / 96; 8,192 x 512 x 2,048 106 / 70, 117 /
+    95, 123 / 133; 5,000 x 512 x 512 28 / 36, 35 / 52, 38 / 61; 20,000 x 128 x 512 forward 26 / 41."""
     moved = {'fwd': 8 * (rows * K + groups * n * K), 'dx': 8 * rows * n + 12 * groups * n * K,
              'dw': 12 * rows * (n + K)}[mode]
     return 1.1 * (product + moved / 4.5e12 + (18e-6 if mode == 'dw' else 11e-6)) < direct
