@@ -187,7 +187,7 @@ struct hv_result {
     }
     // Marks the rows with results that the halves do not hold, in the words' array that keeps the smallest exponents (`at`: where
     // the tile's rows begin), and sets *any where there are such or odd rows or columns.  Workgroups of the same rows store the
-    // same word.
+    // same word.  Rows and columns of zeros alone give zeros, which are right.
     template <bool SPLIT>
     __device__ __forceinline__ void mark(unsigned* at, unsigned* any) const {
         unsigned some = 0u;
@@ -203,9 +203,10 @@ struct hv_result {
                 const mh_f4 v = t.value(i, j);
 #pragma unroll
                 for (int c = 0; c < 4; ++c)
-                    again |= __builtin_fabsf(v[c]) < 16.f && (wide || hv_wide(b[j][c])) && column(j) + c < cols;
+                    again |= __builtin_fabsf(v[c]) < 16.f && (wide || hv_wide(b[j][c])) && (b[j][c] & HV_SMALLEST) &&
+                             column(j) + c < cols;
             }
-            if (again && row(i) < rows) {
+            if (again && row(i) < rows && (a[i] & HV_SMALLEST)) {
                 at[row(i)] = (SPLIT ? a[i] & (HV_SMALLEST | HV_ODD) : a[i]) | HV_AGAIN;
                 some = HV_ODD;
             }

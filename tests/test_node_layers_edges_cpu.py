@@ -233,6 +233,24 @@ extern "C" void back(const unsigned short* c, float* v, int n) {{ for (int i = 0
     assert (there(back(used)) == used).all() and np.isnan(back(np.array([0xC000], dtype=np.uint16)))[0]
 
 
+def test_the_library_refuses_bad_arguments_for_what_is_computed_again():
+    lib = _native.load()
+    p = np.zeros(64, dtype=np.float32).ctypes.data
+    for call, text in (
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, p, p, None, 2, 4, 0, 1, 8, None), 'bad sizes'),
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, p, p, None, 2, 4, 4, 2, 8, None), 'bad sizes'),
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, p, p, None, 2, 4, 4, 1, 0, None), 'bad sizes'),
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, None, p, None, 2, 4, 4, 1, 8, None), 'NULL'),
+            (lambda: lib.mh_hv_again_mm(None, p, 3, p, 4, p, None, None, 0, None, None, p, p, None, 2, 4, 4, 1, 8, None), 'overlap'),
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, p, p, p, 2, 5, 4, 1, 8, None), 'overlap'),
+            (lambda: lib.mh_hv_again_mm(None, p, 4, p, 4, p, None, None, 0, None, None, p, p, None, 2, 4, 4, 1, 8, None), 'not bound'),
+            (lambda: lib.mh_hv_again_outer(None, p, 4, p, 4, p, None, None, p, p, p, p, 2, 4, 4, 1, 4, 0, 8, None), 'bad sizes'),
+            (lambda: lib.mh_hv_again_outer(None, p, 4, p, 4, p, None, None, p, p, p, p, 2, 4, 4, 1, 4, 1, 8, None), 'NULL'),
+            (lambda: lib.mh_hv_again_outer(None, p, 3, p, 4, p, None, None, p, p, p, p, 2, 4, 4, 1, 0, 1, 8, None), 'overlap'),
+            (lambda: lib.mh_hv_again_outer(None, p, 4, p, 4, p, None, None, p, p, p, p, 2, 4, 4, 1, 0, 1, 8, None), 'not bound')):
+        assert call() != 0 and text in lib.mh_last_error().decode(), (text, lib.mh_last_error())
+
+
 def test_a_host_side_built_for_another_library_is_refused(monkeypatch):
     """_layers.so allocates what libmace_hip.so's kernels write: built from another header it is not used."""
     assert _native.layers().abi == _native.ABI_VERSION == _native.load().mh_version()

@@ -10,7 +10,7 @@ import pytest
 import torch
 
 import mace_hip_kernels as mhk
-from mace_hip_kernels import _native, matmul
+from mace_hip_kernels import _native, halves, matmul
 from test_node_layers_gpu import ACTS, BF16, E32, F16, F32, TINY, U, by_halves, dense_case, dev, near, rand  # noqa: F401
 
 pytestmark = pytest.mark.gpu
@@ -248,6 +248,31 @@ def test_one_large_value_by_halves(size, by_halves):  # noqa: F811
         a, b, c = x[i:j].double(), lw[e].detach().cpu().double(), g[i:j].double()
         for name, got, l, r in (('y', y[i:j], a, b.t()), ('dx', dx[i:j], c, b), ('dw', dw[e], c.t(), a)):
             near(f'{name} of {e}', got, l @ r, (l.shape[1] + 16) * E32 * (l.abs() @ r.abs()))
+
+
+def test_rows_of_zeros_are_not_computed_again_by_halves(by_halves):  # noqa: F811
+    """Zeros from rows or columns of zeros are right whatever the other operand holds; sums that cancel beside it are not."""
+    d = dev()
+    print('[case] rows of zeros', flush=True)
+    rng = np.random.default_rng(6)
+    T, K, N = 300, 64, 130
+    x, w = rand(rng, T, K), rand(rng, N, K)
+    x[::2], w[::3] = 0, 0
+    w[1, 3] = 1e-25                                          # a wide row
+    for again, x0 in ((False, x), (True, torch.cat([x[:-1], torch.tensor([[1e15] + [0.0] * (K - 2) + [1e-9]])]))):
+        w[:, 0] = 0 if again else w[:, 0]
+        words = torch.zeros(T + 1, dtype=torch.int32, device=d)
+        y = torch.empty(T, N, device=d)
+        h, c = (torch.empty(n, 2 * K, dtype=torch.int16, device=d) for n in (T, N))
+        cw = torch.zeros(N + 1, dtype=torch.int32, device=d)
+        xd, wd, s = x0.to(d), w.to(d), _native.stream_of(y)
+        lib, split, mod = _native.load(), halves.module(d, 'split').handle, halves.module(d, 'fwd').handle
+        P = lambda t: t.data_ptr()  # noqa: E731
+        _native.check(lib.mh_hv_rows(split, P(xd), K, P(h), P(words), T, K, s))
+        _native.check(lib.mh_hv_rows(split, P(wd), K, P(c), P(cw), N, K, s))
+        _native.check(lib.mh_hv_mm(mod, P(h), P(c), P(y), None, None, 0, None, None, P(words), P(cw), None, T, N, K, 1, s))
+        assert bool(words[T]) == again and (words[:T] >> 30 & 1).nonzero().flatten().tolist() == ([T - 1] if again else [])
+    near('y', mhk.dense(xd, wd), x0.double() @ w.double().t(), (K + 16) * E32 * (x0.double().abs() @ w.double().abs().t()))
 
 
 def test_infinities_that_meet_small_values_by_halves(by_halves):  # noqa: F811
